@@ -14,6 +14,7 @@
 #include "common.cuh"
 #include "gen9blas_ml.h"
 #include "internal.h"
+#include "mma_sync.cuh"
 #include "sm100.cuh"
 #include <cmath>
 #include <cstring>
@@ -683,34 +684,6 @@ __host__ __device__ constexpr int at2_rowb(int D) { return D * 2 + 16; }
 __host__ __device__ constexpr size_t at2_stage(int D) { return (size_t)AT2_WARPS * 2 * AT2_KEYS * at2_rowb(D); }
 __host__ __device__ constexpr size_t at2_smem(int D) { return at2_stage(D) + AT2_WARPS * 2 * sizeof(uint64_t); }
 
-__device__ __forceinline__ void at_ldsm(unsigned addr, unsigned (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void at_ldsm_t(unsigned addr, unsigned (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ unsigned at_movt(unsigned x) {
-    unsigned y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ void at_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// (x0, x1) as FP16 hi and lo parts: hi = fp16(x), lo = fp16(x − hi), element 0 in the low half of each word
-__device__ __forceinline__ void at_split(float x0, float x1, unsigned &hi, unsigned &lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 hf = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - hf.x, x1 - hf.y);
-    hi = *reinterpret_cast<const unsigned *>(&h);
-    lo = *reinterpret_cast<const unsigned *>(&l);
-}
-__device__ __forceinline__ float at_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }   // |e| <= 126
 // one contiguous row of `bytes` bytes (multiple of 16, both addresses 16-byte aligned) into shared memory, completing on
 // the mbarrier; no multicast
 __device__ __forceinline__ void at_bulk_row(void *dst, const void *src, unsigned bytes, uint64_t *bar) {

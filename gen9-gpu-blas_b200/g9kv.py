@@ -1,0 +1,226 @@
+"""g9kv -- the paged key-value cache of libgen9blas.so (include/gen9blas_kv.h) over torch tensors.
+
+    kv = g9kv.PagedKV(K, V, table, bounds=bounds)           # pool tensors and the page table of a batch of streams
+    kv.append(k, v, length)                                 # the new tokens' keys and values enter the pages
+    out = kv.attend(q, length + k.shape[1])                 # attention of the new tokens over the pages
+    sel = kv.select(q, visible, 64)                         # or: the 64 pages of each head that may matter most,
+    out = kv.attend(q, visible, sel=sel)                    #     and attention over those alone
+    out = kv.attend(q, visible, acc=acc)                    # also adds up the attention each slot receives
+    length = kv.evict(length, 4096, acc, pos, recent=64)    # keeps the 4096 slots of each head that received most
+
+K and V: float16 [pages, kv heads, page size, head size], unit stride in the last dimension, any others a multiple of 8
+elements (so both [page][head][slot] and [page][slot][head] pools serve, the latter as a permuted view). table: int32
+[streams, pages per stream], -1 where a stream has no page. q, k, v: float32 [streams, tokens, heads, head size], unit
+stride in the last dimension. Everything lies on one GPU; calls run on torch's current stream and do not wait. Shape and
+type errors raise ValueError, library errors RuntimeError with gen9blas_error().
+
+One cache object is used by one thread at a time, as the library is. A captured call (torch.cuda.graph) needs a workspace
+of its own: pass `workspace=g9kv.Workspace()` to the constructor and make one call of each shape before the capture.
+"""
+import ctypes
+import os
+
+import torch
+
+_HERE = os.path.dirname(os.path.realpath(__file__))
+_I, _P, _L, _F = ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
+
+
+class _Cache(ctypes.Structure):   # gen9blas_kv_cache
+    _fields_ = [("D", _I), ("HKV", _I), ("page", _I), ("n_pages", _I),
+                ("K", _P), ("kp", _L), ("kk", _L), ("kh", _L), ("k_bytes", ctypes.c_size_t),
+                ("V", _P), ("vp", _L), ("vk", _L), ("vh", _L), ("v_bytes", ctypes.c_size_t),
+                ("bounds", _P), ("table", _P), ("ts", _L), ("mp", _I), ("ns", _I)]
+
+
+_C = ctypes.POINTER(_Cache)
+_SIGNATURES = {
+    "init": ([], _I), "error": ([], ctypes.c_char_p), "set_device": ([_I], _I), "get_device": ([], _I),
+    "set_stream": ([_P], _I), "get_stream": ([], _P),
+    "kv_supported": ([_I, _I, _I], _I), "kv_ws_create": ([], _P), "kv_ws_free": ([_P], None),
+    "kv_append": ([_C, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _L, _L, _P, _I, _P], _I),
+    "attn_paged": ([_C, _I, _I, _P, _L, _L, _L, _P, _I, _I, _P, _I, _F, _P, _P, _P, _L, _L, _P, _I], _I),
+    "kv_select": ([_C, _I, _I, _P, _L, _L, _L, _P, _I, _I, _I, _I, _P, _P, _I], _I),
+    "kv_evict": ([_C, _P, _I, _I, _I, _P, _P, _L, _L, _P, _P, _I], _I),
+}
+_lib = ctypes.CDLL(os.environ.get("GEN9BLAS_LIB") or os.path.join(_HERE, "libgen9blas.so"))
+_fn = {}
+for _name, (_args, _res) in _SIGNATURES.items():
+    _f = getattr(_lib, "gen9blas_" + _name)
+    _f.argtypes, _f.restype = _args, _res
+    _fn[_name] = _f
+_append, _attend, _select, _evict = (_fn[n] for n in ("kv_append", "attn_paged", "kv_select", "kv_evict"))
+_set_stream, _get_stream, _get_device = _fn["set_stream"], _fn["get_stream"], _fn["get_device"]
+_LEGACY = 1   # cudaStreamLegacy: torch's default stream (a null stream would mean the library's own)
+
+
+def _check(status, what):
+    if status == 1:
+        raise ValueError(f"{what}: shape outside gen9blas_kv_supported (head size a multiple of 8 up to 256)")
+    if status:
+        raise RuntimeError(_fn["error"]().decode(errors="replace"))
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+class Workspace:
+    """Device memory for attend, select and evict of calls that run one after the other (see gen9blas_kv_ws_create)."""
+
+    def __init__(self):
+        self.handle = _fn["kv_ws_create"]()
+        if not self.handle:
+            raise RuntimeError(_fn["error"]().decode(errors="replace"))
+
+    def free(self):
+        if self.handle:
+            _fn["kv_ws_free"](self.handle)
+            self.handle = None
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _fn:
+            self.free()
+
+
+class PagedKV:
+    """A batch's view of one layer's cache: the pool, the page table and, on request, the bounds of the pages."""
+
+    def __init__(self, K, V, table, bounds=None, workspace=None):
+        for name, x in (("K", K), ("V", V)):
+            _need(x.dtype == torch.float16 and x.dim() == 4 and x.is_cuda,
+                  f"{name}: float16 [pages, kv heads, page size, head size] on a GPU")
+            _need(x.stride(3) == 1 or x.shape[3] == 1, f"{name}: the last dimension has stride {x.stride(3)}")
+        _need(K.shape == V.shape and K.device == V.device, "K and V differ in shape or device")
+        _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == K.device, "table: int32 [streams, pages]")
+        _need(table.stride(1) == 1 or table.shape[1] <= 1, "table: the last dimension is not contiguous")
+        pages, heads, page, dim = K.shape
+        if bounds is not None:
+            _need(bounds.dtype == torch.float16 and tuple(bounds.shape) == (pages, heads, 2, dim) and
+                  bounds.is_contiguous() and bounds.device == K.device,
+                  "bounds: contiguous float16 [pages, kv heads, 2, head size] beside K")
+        self.K, self.V, self.table, self.bounds, self.workspace = K, V, table, bounds, workspace
+        self.device, self.streams, self.slots = K.device, table.shape[0], table.shape[1] * page
+        self.heads, self.page, self.dim = heads, page, dim
+        self._index = K.device.index
+        self._ws = workspace.handle if workspace is not None else None
+
+        def span(x):
+            return 2 * (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) if x.numel() else 0
+        ks, vs = K.stride(), V.stride()
+        self._c = _Cache(dim, heads, page, pages, K.data_ptr(), ks[0], ks[2], ks[1], span(K), V.data_ptr(), vs[0], vs[2],
+                         vs[1], span(V), bounds.data_ptr() if bounds is not None else None, table.data_ptr(),
+                         table.stride(0), table.shape[1], table.shape[0])
+        if _fn["init"]():
+            raise RuntimeError(_fn["error"]().decode(errors="replace"))
+
+    def _run(self, what, fn, *args):
+        """One library call on this cache's device and torch's current stream there; both are put back after it."""
+        stream, device = _get_stream(), _get_device()
+        if device != self._index:
+            _check(_fn["set_device"](self._index), what)
+        _set_stream(torch.cuda.current_stream(self._index).cuda_stream or _LEGACY)
+        try:
+            status = fn(self._c, *args)
+        finally:
+            if device != self._index:
+                _fn["set_device"](device)
+            _set_stream(stream)
+        if status:
+            _check(status, what)
+
+    def _rows(self, name, x, heads):
+        _need(x.dtype == torch.float32 and x.dim() == 4 and x.device == self.device and x.shape[0] == self.streams and
+              x.shape[3] == self.dim and (heads is None or x.shape[2] == heads) and (x.stride(3) == 1 or self.dim == 1),
+              f"{name}: float32 [{self.streams}, tokens, heads, {self.dim}] on {self.device}, unit stride last")
+
+    def _ints(self, name, x):
+        _need(x.dtype == torch.int32 and x.dim() == 1 and x.shape[0] == self.streams and x.device == self.device and
+              (x.stride(0) == 1 or self.streams <= 1), f"{name}: contiguous int32 [{self.streams}] on {self.device}")
+        return x.data_ptr()
+
+    def _marks(self, acc, pos):
+        ms = mh = 0
+        for name, x, dt in (("acc", acc, torch.float32), ("pos", pos, torch.int32)):
+            if x is None:
+                continue
+            _need(x.dtype == dt and x.dim() == 3 and x.shape[0] == self.streams and x.shape[1] == self.heads and
+                  x.shape[2] >= self.slots and x.device == self.device and (x.stride(2) == 1 or x.shape[2] <= 1),
+                  f"{name}: {dt} [{self.streams}, {self.heads}, at least {self.slots}] on {self.device}, unit stride last")
+            ms, mh = x.stride(0), x.stride(1)
+        _need(acc is None or pos is None or acc.stride() == pos.stride(), "acc and pos differ in their strides")
+        return acc.data_ptr() if acc is not None else None, pos.data_ptr() if pos is not None else None, ms, mh
+
+    def append(self, k, v, length, count=None, acc=None, pos=None, pos0=None, wait=False):
+        """Writes the tokens k, v [streams, tokens, kv heads, dim] behind each stream's `length` slots, of stream s the
+        first count[s] (all without count); bounds follow. acc and pos [streams, kv heads, slots]: set to 0 and
+        pos0[s] + t (the slot's number without pos0). With wait, returns whether every token found a page."""
+        self._rows("k", k, self.heads)
+        self._rows("v", v, self.heads)
+        _need(k.shape == v.shape, "k and v differ in shape")
+        a, p, ms, mh = self._marks(acc, pos)
+        n = self._ints("length", length)
+        cn = self._ints("count", count) if count is not None else None
+        p0 = self._ints("pos0", pos0) if pos0 is not None else None
+        bad = _I(0)
+        ks, vs = k.stride(), v.stride()
+        self._run("append", _append, k.shape[1], k.data_ptr(), ks[1], ks[2], ks[0], v.data_ptr(), vs[1], vs[2], vs[0], n, cn, a, p,
+                       ms, mh, p0, int(wait), ctypes.addressof(bad))
+        return not bad.value if wait else None
+
+    def attend(self, q, visible, step=1, scale=None, window=0, sel=None, acc=None, out=None, lse=False):
+        """Attention of the tokens q [streams, tokens, heads, dim]: token t of stream s sees visible[s] + step·t slots
+        (the last `window` of them, if given; those of the pages sel[s, t, g], if given). acc gains the weights each slot
+        received. Returns out (float32, as q), and with lse=True also the logarithms of the softmax sums
+        [streams, tokens, heads]."""
+        self._rows("q", q, None)
+        ns, nq, h, d = q.shape
+        see = self._ints("visible", visible)
+        a, _, ms, mh = self._marks(acc, None)
+        nsel = sp = None
+        if sel is not None:
+            _need(sel.dtype == torch.int32 and sel.dim() == 4 and sel.shape[:3] == (ns, nq, self.heads) and
+                  sel.is_contiguous() and sel.device == self.device,
+                  f"sel: contiguous int32 [{ns}, {nq}, {self.heads}, pages] on {self.device}")
+            nsel, sp = sel.shape[3], sel.data_ptr() or see   # no pages at all: the list is there, and nothing is read
+        if out is None:
+            out = torch.empty((ns, nq, h, d), device=self.device, dtype=torch.float32)
+        else:
+            _need(out.dtype == torch.float32 and out.shape == q.shape and out.is_contiguous() and out.device == self.device,
+                  "out: contiguous float32 of q's shape")
+        logs = torch.empty((ns, nq, h), device=self.device, dtype=torch.float32) if lse else None
+        qs = q.stride()
+        self._run("attend", _attend, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, window, sp, nsel or 0,
+                       d ** -0.5 if scale is None else scale, out.data_ptr(), logs.data_ptr() if lse else None, a, ms, mh,
+                  self._ws, 0)
+        return (out, logs) if lse else out
+
+    def select(self, q, visible, pages, step=1, first=1, last=1, out=None):
+        """The `pages` pages that each token and kv head attends to: the first and the last ones it sees, then those whose
+        bounds allow the largest q·k. int32 [streams, tokens, kv heads, pages], ascending, -1 behind."""
+        self._rows("q", q, None)
+        ns, nq, h, _ = q.shape
+        see = self._ints("visible", visible)
+        if out is None:
+            out = torch.empty((ns, nq, self.heads, pages), device=self.device, dtype=torch.int32)
+        else:
+            _need(out.dtype == torch.int32 and tuple(out.shape) == (ns, nq, self.heads, pages) and out.is_contiguous() and
+                  out.device == self.device, "out: contiguous int32 [streams, tokens, kv heads, pages]")
+        qs = q.stride()
+        self._run("select", _select, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, first, last, pages, out.data_ptr(),
+                  self._ws, 0)
+        return out
+
+    def evict(self, length, keep, acc, pos=None, first=0, recent=0, out=None):
+        """Thins every stream and head to `keep` slots: those whose position is below `first` or among the `recent` newest,
+        then those with the largest acc; the slots that stay from behind `keep` fill the free ones, in K, V, acc and pos.
+        Returns the new lengths."""
+        a, p, ms, mh = self._marks(acc, pos)
+        n = self._ints("length", length)
+        if out is None:
+            out = torch.empty_like(length)
+        else:
+            self._ints("out", out)
+        self._run("evict", _evict, n, keep, first, recent, a, p, ms, mh, out.data_ptr(), self._ws, 0)
+        return out
