@@ -3,6 +3,8 @@
 // reference, whose attention (lib/gen9blas_ml.h:122-149) reads one contiguous cache per stream.
 #include "kv.h"
 #include "common.cuh"
+#include "mma_sync.cuh"
+#include "sm100.cuh"
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -190,6 +192,11 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void cp16(unsigned dst, const void *src, int bytes) {   // bytes 16, or 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------------------------- cache writes
@@ -303,82 +310,204 @@ __global__ void __launch_bounds__(256) kv_append_k(AppendArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- page selection
+// Two kernels. kv_score_k reads the bounds once and scores every page in FP32 on the tensor cores; kv_choose_k takes the
+// nsel best of a row, and where the FP32 scores cannot tell which side of the border a page lies on (they differ by less
+// than twice their error bound) it computes those pages' scores again in 64 bits: the choice is the one of the 64-bit
+// scores. Scoring everything in 64 bits took 118 µs at 16 streams × 8 heads × 2048 pages of D 128 (101 MB of bounds), its
+// conversions and FP64 multiply-adds the limit.
 struct SelectArgs {
     KvDev c;
     int G, H, nq, dvis, first, last, nsel;
+    int hg, tiles, tg, zt, steps;   // 8-head groups of a token, row tiles (token, group) in all, at once in a CTA, and in all
+                                    // of a CTA (whole tokens; more than tg only where one token's groups are more); steps
+                                    // of a warp
     const float *Q;
     long long qt, qh, qs;
     const int *vis;
-    unsigned long long *key;   // [row (s, t, g)][mp]
+    float *score;               // [row (s, t, g)][mp]: FP32 scores; kv_choose_k overwrites those that it decided by hand
+    float *l1;                  // [(s, t, h)]: sum of |q|
+    float *peak;                // [(s, g)][CTA][warp]: largest |bound| seen; infinity where a score is not finite
+    unsigned long long *key;    // [row][mp]: 64-bit keys of pages decided by hand, where they are many
     int *sel;
 };
 
-// Scores: one CTA of 128 threads per (64 pages, row (s, t, g)). The 64 pages' bounds pass through shared memory; thread i
-// sums half of the head's elements of page i % 64 for every query head in 64 bits.
-constexpr int SEL_PAGES = 64;
-__global__ void __launch_bounds__(128) kv_score_k(SelectArgs a) {
-    extern __shared__ __align__(16) uint8_t sel_sm[];
+__device__ __forceinline__ int pages_seen(const SelectArgs &a, int s, int t) {
+    const int n = seen_slots(a.vis[s], a.dvis, t, a.c.cap);
+    return n / a.c.page + (n % a.c.page != 0);
+}
+
+constexpr int SW = 4, SPAGES = 16, SNST = 3;   // warps of a CTA, pages of a step, stages of a warp's ring
+template <int DP>
+struct ScoreCfg {
+    static constexpr int STAGE = SPAGES * DP * 2 * 2;               // lower and upper rows of 16 pages
+    static constexpr int RING = SW * SNST * STAGE;
+    static constexpr int QF = 2 * (DP / 16) * 32 * 16;              // fragments of one row tile: q < 0 and q > 0
+    static constexpr int TG = DP == 256 ? 1 : DP == 128 ? 4 : 8;    // row tiles a CTA holds at most
+    static constexpr int smem(int tg) { return RING + tg * (QF + 8 * 4); }
+};
+
+// Score of (page, query head): Σ_d max(q_d·lo_d, q_d·hi_d) = Σ min(q, 0)·lo + Σ max(q, 0)·hi, a product of the bounds (A, 16
+// pages × 16 elements, FP16 as they are) with the two halves of the query (B, 8 heads) in two FP16 parts each, as in
+// attn_paged_k. A CTA's four warps take every fourth step of 16 pages of one (stream, head) through rings of their own,
+// for all its row tiles (token, 8 heads); a page's score is the largest over the heads of a token. Where a token has more
+// head groups than shared memory holds, the CTA reads its pages again for the next ones. Bound by the reading of the
+// bounds.
+template <int DP>
+__global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ SelectArgs a) {
+    using C = ScoreCfg<DP>;
+    constexpr int KT = DP / 16, PITCH = DP * 2, CH = DP / 8;
+    extern __shared__ __align__(128) uint8_t ss[];
+    uint4 *qf = reinterpret_cast<uint4 *>(ss + C::RING);                       // [tile][half][kt][lane]
+    float *qinv = reinterpret_cast<float *>(ss + C::RING + a.tg * C::QF);      // [tile][8]
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const long long row = blockIdx.y;
-    const int g = (int)(row % c.HKV);
-    const long long st = row / c.HKV;
-    const int t = (int)(st % a.nq), s = (int)(st / a.nq);
-    const int have = (seen_slots(a.vis[s], a.dvis, t, c.cap) + c.page - 1) / c.page;
-    const int p0 = blockIdx.x * SEL_PAGES;
-    if (p0 >= have) return;
-    double *q = reinterpret_cast<double *>(sel_sm);                 // [G][D]
-    const int pitch = 2 * c.D * 2 + 16;                             // bytes of a page's bounds, padded
-    uint8_t *bs = sel_sm + (size_t)a.G * c.D * sizeof(double);     // [64][pitch]
-    double *part = reinterpret_cast<double *>(bs + (size_t)SEL_PAGES * pitch);   // [64]
-    for (int i = threadIdx.x; i < a.G * c.D; i += blockDim.x) {
-        const int h = i / c.D, d = i - h * c.D;
-        q[i] = (double)a.Q[s * a.qs + t * a.qt + (long long)(g * a.G + h) * a.qh + d];
-    }
-    const int cpr = c.D / 4;   // 16-byte chunks of one page's bounds
-    for (int i = threadIdx.x; i < SEL_PAGES * cpr; i += blockDim.x) {
-        const int p = i / cpr, ch = i - p * cpr;
-        const int id = p0 + p < have ? page_id(c.table, c.ts, s, p0 + p, c.mp, c.n_pages) : -1;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (id >= 0) v = __ldg(reinterpret_cast<const uint4 *>(c.bounds + ((long long)id * c.HKV + g) * 2 * c.D) + ch);
-        *reinterpret_cast<uint4 *>(bs + p * pitch + ch * 16) = v;
-    }
-    __syncthreads();
-    const int p = threadIdx.x & (SEL_PAGES - 1), part_no = threadIdx.x / SEL_PAGES;
-    const int d0 = part_no ? (c.D / 2 + 1) / 2 * 2 : 0, d1 = part_no ? c.D : (c.D / 2 + 1) / 2 * 2;
-    const __half2 *lo = reinterpret_cast<const __half2 *>(bs + p * pitch), *hi = lo + c.D / 2;
-    double best = -INFINITY;
-    bool nan = false;
-    for (int h = 0; h < a.G; h++) {
-        double x = 0.0;
-        const double *qh = q + h * c.D;
-        for (int d = d0; d < d1; d += 2) {
-            const float2 l = __half22float2(lo[d / 2]), u = __half22float2(hi[d / 2]);
-            const double q0 = qh[d], q1 = qh[d + 1];
-            x = fma(q0, (double)(q0 >= 0.0 ? u.x : l.x), x);
-            x = fma(q1, (double)(q1 >= 0.0 ? u.y : l.y), x);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
+    const int sg = blockIdx.y, s = sg / c.HKV, g = sg - s * c.HKV;
+    const int z0 = blockIdx.z * a.zt, z1 = min(z0 + a.zt, a.tiles);
+    const int have = pages_seen(a, s, (z1 - 1) / a.hg);
+    const int step0 = blockIdx.x * SW * a.steps, all = (have + SPAGES - 1) / SPAGES;
+    if (step0 >= all) return;
+    const int my = min(a.steps, max(0, (all - step0 - warp + SW - 1) / SW));
+    uint8_t *wring = ss + warp * SNST * C::STAGE;
+    const unsigned wbase = sm100::smem_u32(wring);
+    auto id_of = [&](int i) {
+        const int p = (step0 + warp + SW * i) * SPAGES + (lane & 15);
+        return i < my && p < have ? page_id(c.table, c.ts, s, p, c.mp, c.n_pages) : -1;
+    };
+    auto copy = [&](int i, int id) {
+        if (i < my) {
+            const unsigned at = wbase + (i % SNST) * C::STAGE;
+#pragma unroll
+            for (int j = 0; j < SPAGES * 2 * CH / 32; j++) {
+                const int e = j * 32 + lane, pg = e / (2 * CH), half = e / CH & 1, ch = e % CH;
+                const int pid = __shfl_sync(kAll, id, pg);
+                const int bytes = pid >= 0 && ch * 8 < c.D ? 16 : 0;
+                const __half *src = c.bounds + (((long long)max(pid, 0) * c.HKV + g) * 2 + half) * c.D + ch * 8;
+                cp16(at + half * SPAGES * PITCH + pg * PITCH + ((ch ^ (pg & 7)) << 4), bytes ? src : c.bounds, bytes);
+            }
         }
-        if (part_no) part[p] = x;
-        __syncthreads();
-        if (!part_no) {
-            x += part[p];
-            nan = nan || x != x;
-            best = fmax(best, x);
+        cp_commit();
+    };
+    const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = lane >> 4;
+    __half2 peak = __half2half2(__ushort_as_half(0));
+    bool wild = false;
+    for (int tile0 = z0; tile0 < z1; tile0 += a.tg) {
+        const int ntile = min(a.tg, z1 - tile0);
+        if (tile0 > z0) __syncthreads();   // every warp has left the last tiles' fragments
+        int ids[SNST - 1];
+#pragma unroll
+        for (int i = 0; i < SNST - 1; i++) ids[i] = id_of(i);
+#pragma unroll
+        for (int i = 0; i < SNST - 1; i++) copy(i, ids[i]);
+        int next = id_of(SNST - 1), now = ids[0], after = ids[1];
+        // ---- query fragments: a warp prepares every fourth row of the tiles
+        for (int r = warp; r < ntile * 8; r += SW) {
+            const int tile = tile0 + (r >> 3), t = tile / a.hg, h = (tile - t * a.hg) * 8 + (r & 7);
+            const bool live = h < a.G;
+            const float *qp = a.Q + s * a.qs + t * a.qt + (long long)(g * a.G + (live ? h : 0)) * a.qh;
+            float x[DP / 32], big = 0.0f, l1 = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int d = 64 * i + 2 * lane + j;
+                    const float v = live && d < c.D ? qp[d] : 0.0f;
+                    x[2 * i + j] = v;
+                    big = fmaxf(big, fabsf(v));
+                    l1 += fabsf(v);
+                }
+            for (int i = 16; i > 0; i >>= 1) {
+                big = fmaxf(big, __shfl_xor_sync(kAll, big, i));
+                l1 += __shfl_xor_sync(kAll, l1, i);
+            }
+            int ex = 0;
+            if (big > 0.0f) ex = min(max(140 - (int)((__float_as_uint(big) >> 23) & 0xffu), -126), 126);
+            const float up = at_pow2(ex);
+            if (lane == 0) {
+                qinv[r] = at_pow2(-ex);
+                if (live && blockIdx.x == 0) a.l1[((long long)s * a.nq + t) * a.H + g * a.G + h] = l1;
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
+                    y0 = half ? fmaxf(y0, 0.0f) : fminf(y0, 0.0f);
+                    y1 = half ? fmaxf(y1, 0.0f) : fminf(y1, 0.0f);
+                    unsigned h2, l2;
+                    at_split(y0, y1, h2, l2);
+                    const int d = 64 * i + 2 * lane, kt = d >> 4, dd = d & 15;
+                    unsigned *f = reinterpret_cast<unsigned *>(qf + (((r >> 3) * 2 + half) * KT + kt) * 32 + (r & 7) * 4 + ((dd & 7) >> 1));
+                    f[dd >> 3] = h2;
+                    f[2 + (dd >> 3)] = l2;
+                }
         }
         __syncthreads();
+        for (int i = 0; i < my; i++) {
+            cp_wait<SNST - 2>();
+            __syncwarp();
+            copy(i + SNST - 1, next);
+            const unsigned lo = wbase + (i % SNST) * C::STAGE, hi = lo + SPAGES * PITCH;
+            const int p = (step0 + warp + SW * i) * SPAGES + gq;
+            const bool in0 = __shfl_sync(kAll, now, gq) >= 0, in1 = __shfl_sync(kAll, now, gq + 8) >= 0;
+            float top[2] = {-INFINITY, -INFINITY};
+            for (int tile = 0; tile < ntile; tile++) {
+                float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                const uint4 *q0 = qf + tile * 2 * KT * 32 + lane, *q1 = q0 + KT * 32;
+#pragma unroll
+                for (int kt = 0; kt < KT; kt++) {
+                    const unsigned off = arow * PITCH + (((2 * kt + acol) ^ (arow & 7)) << 4);
+                    unsigned l4[4], u4[4];
+                    at_ldsm(lo + off, l4);
+                    at_ldsm(hi + off, u4);
+                    if (tile == 0) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) peak = __hmax2(peak, __hmax2(__habs2(as_h2(l4[e])), __habs2(as_h2(u4[e]))));
+                    }
+                    const uint4 f = q0[kt * 32], h = q1[kt * 32];
+                    at_mma(sc[0], l4, f.x, f.y);
+                    at_mma(sc[1], u4, h.x, h.y);
+                    at_mma(sc[0], l4, f.z, f.w);
+                    at_mma(sc[1], u4, h.z, h.w);
+                }
+                const int t = (tile0 + tile) / a.hg, hb = (tile0 + tile - t * a.hg) * 8;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (hb + 2 * tq + j >= a.G) continue;
+                    const float inv = qinv[tile * 8 + 2 * tq + j];
+                    const float x0 = (sc[0][j] + sc[1][j]) * inv, x1 = (sc[0][2 + j] + sc[1][2 + j]) * inv;
+                    wild = wild || (in0 && !(fabsf(x0) < INFINITY)) || (in1 && !(fabsf(x1) < INFINITY));
+                    top[0] = fmaxf(top[0], x0);
+                    top[1] = fmaxf(top[1], x1);
+                }
+                if ((tile0 + tile) % a.hg != a.hg - 1 && tile != ntile - 1) continue;   // more heads of this token follow
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 1));
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 2));
+                }
+                if (tq == 0) {
+                    float *out = a.score + (((long long)s * a.nq + t) * c.HKV + g) * c.mp;
+                    const bool more = tile0 > z0;   // the token's earlier groups have left their largest
+                    if (p < have) out[p] = in0 ? (more ? fmaxf(out[p], top[0]) : top[0]) : -INFINITY;
+                    if (p + 8 < have) out[p + 8] = in1 ? (more ? fmaxf(out[p + 8], top[1]) : top[1]) : -INFINITY;
+                }
+                top[0] = top[1] = -INFINITY;
+            }
+            now = after;
+            after = next;
+            next = id_of(i + SNST);
+        }
+        cp_wait<0>();
     }
-    if (part_no || p0 + p >= have) return;
-    const int at = p0 + p;
-    unsigned long long key = nan ? 0ull : score_key(best);
-    if (page_id(c.table, c.ts, s, at, c.mp, c.n_pages) < 0) key = 0ull;
-    if (at < a.first || at >= have - a.last) key = ~0ull;
-    a.key[row * c.mp + at] = key;
+    float pk = fmaxf(__low2float(peak), __high2float(peak));
+    for (int i = 16; i > 0; i >>= 1) pk = fmaxf(pk, __shfl_xor_sync(kAll, pk, i));
+    if (__any_sync(kAll, wild)) pk = INFINITY;
+    if (lane == 0) a.peak[(((long long)blockIdx.z * gridDim.y + sg) * gridDim.x + blockIdx.x) * SW + warp] = pk;
 }
 
-// The nsel largest keys of a row (ties: lowest place), ascending by place: the threshold by radix selection over 8-bit
-// digits from the top, then one ordered pass. One CTA per row.
-__device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   // blockDim.x = 1024 at most, multiple of 32
+__device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   // whole CTA, at most 1024 threads
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
     int x = v;
 #pragma unroll
@@ -389,91 +518,218 @@ __device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   /
     __syncthreads();
     if (lane == 31) sh[w] = x;
     __syncthreads();
-    if (w == 0) {
-        int y = lane < nw ? sh[lane] : 0;
+    int y = lane < nw ? sh[lane] : 0, before = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(kAll, y, o);
-            if (lane >= o) y += z;
-        }
-        sh[lane] = y;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(kAll, y, o);
+        if (lane >= o) y += z;
     }
-    __syncthreads();
-    *total = sh[nw - 1];
-    return x + (w ? sh[w - 1] : 0);
+    *total = __shfl_sync(kAll, y, 31);
+    before = __shfl_sync(kAll, y, max(w - 1, 0));
+    return x + (w ? before : 0);
 }
 
-__global__ void __launch_bounds__(512) kv_choose_k(SelectArgs a) {
-    __shared__ int hist[256], scan[32];
-    __shared__ int sh_digit, sh_above, sh_in;
+// Adds one to hist[bin] for the lanes with in: lanes of a warp with the same bin together (keys crowd in few bins).
+__device__ __forceinline__ void hist_add(int *hist, int bin, bool in) {
+    const unsigned live = __ballot_sync(kAll, in);
+    if (!in) return;
+    const unsigned same = __match_any_sync(live, bin);
+    if ((int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+}
+
+// Finds the bin that holds the need-th item from the top, how many lie above it and how many in it. hist: 2·blockDim bins.
+__device__ __forceinline__ void pick_bin(const int *hist, int need, int *scan, int *out) {
+    const int b0 = 2 * (int)blockDim.x - 1 - 2 * (int)threadIdx.x, v0 = hist[b0], v1 = hist[b0 - 1];
+    int total;
+    const int incl = block_scan_incl(v0 + v1, scan, &total), above = incl - v0 - v1;
+    if (above < need && incl >= need) {
+        const bool second = above + v0 < need;
+        out[0] = second ? b0 - 1 : b0;
+        out[1] = second ? above + v0 : above;
+        out[2] = second ? v1 : v0;
+    }
+    __syncthreads();
+}
+
+// A page's score in 64 bits, by one warp: the key of the largest over the heads.
+__device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int s, int t, int g, int place) {
+    const KvDev &c = a.c;
+    const int lane = threadIdx.x & 31;
+    const int id = page_id(c.table, c.ts, s, place, c.mp, c.n_pages);
+    if (id < 0) return 0ull;
+    const __half *lo = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D, *hi = lo + c.D;
+    double best = -INFINITY;
+    bool nan = false;
+    for (int h = 0; h < a.G; h++) {
+        const float *q = a.Q + s * a.qs + t * a.qt + (long long)(g * a.G + h) * a.qh;
+        double x = 0.0;
+        for (int d = lane; d < c.D; d += 32) {
+            const float v = q[d];
+            x = fma((double)v, (double)__half2float(v >= 0.0f ? hi[d] : lo[d]), x);
+        }
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
+        nan = nan || x != x;
+        best = fmax(best, x);
+    }
+    return nan ? 0ull : score_key(best);
+}
+
+constexpr int CT = 512, CLIST = 512;
+// One CTA per row (s, t, g). Keys are the FP32 scores' order-preserving bits (pages that are always taken above all); the
+// nsel-th largest, tau, by radix selection over digits of 10, 11 and 11 bits. With E the bound of a score's error, a page above
+// tau + 2E is taken, one below tau - 2E is not: nsel pages have scores of at least tau - E, and fewer than nsel more than tau + E.
+// The pages between are ranked by their 64-bit scores.
+__global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ SelectArgs a, int score_ctas) {
+    __shared__ int hist[2 * CT], hist2[2 * CT], scan[32], got[3];
+    __shared__ float red[CT / 32];
+    __shared__ int list[CLIST];
+    __shared__ unsigned long long lkey[CLIST];
+    __shared__ int sure, nlist;
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const long long row = blockIdx.x;
-    const long long st = row / c.HKV;
-    const int t = (int)(st % a.nq), s = (int)(st / a.nq);
-    const int have = (seen_slots(a.vis[s], a.dvis, t, c.cap) + c.page - 1) / c.page;
-    int *out = a.sel + row * a.nsel;
-    if (have <= a.nsel) {
-        for (int i = threadIdx.x; i < a.nsel; i += blockDim.x) out[i] = i < have ? i : -1;
+    const int row = blockIdx.x, st = row / c.HKV, g = row - st * c.HKV;
+    const int s = st / a.nq, t = st - s * a.nq;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int have = pages_seen(a, s, t), m = a.nsel;
+    int *out = a.sel + (long long)row * m;
+    if (have <= m) {
+        for (int i = tid; i < m; i += CT) out[i] = i < have ? i : -1;
         return;
     }
-    const unsigned long long *key = a.key + row * c.mp;
-    unsigned long long prefix = 0, mask = 0;
-    int need = a.nsel;          // how many of the keys that share the prefix are still to be taken
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
+    float *score = a.score + (long long)row * c.mp;
+    auto always = [&](int p) { return p < a.first || p >= have - a.last; };
+    auto key_of = [&](int p) { return always(p) ? kAll : weight_key(__ldcg(score + p)); };
+    // ---- E = 2^-14 · max |q|_1 · max |bound| (2^-13 for D > 128): each of the 4·D/16 tensor-core steps adds 17 numbers, each cut
+    // off at worst 2^-23 below the largest, which is at most |q|_1·|bound|, 2^-18.9 in all; 32 steps at D = 128 make 2^-13.9
+    // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21
+    float big = 0.0f, l1 = 0.0f;
+    {
+        const int sg = s * c.HKV + g, z = t * a.hg / a.zt;
+        const int used = ((pages_seen(a, s, t) + SPAGES - 1) / SPAGES + SW * a.steps - 1) / (SW * a.steps);   // CTAs with pages
+        for (int i = tid; i < used * SW; i += CT)
+            big = fmaxf(big, __ldcg(a.peak + ((long long)z * c.ns * c.HKV + sg) * score_ctas * SW + i));
+        for (int h = tid; h < a.G; h += CT) l1 = fmaxf(l1, __ldcg(a.l1 + (long long)st * a.H + g * a.G + h));
+        for (int o = 16; o > 0; o >>= 1) {
+            big = fmaxf(big, __shfl_xor_sync(kAll, big, o));
+            l1 = fmaxf(l1, __shfl_xor_sync(kAll, l1, o));
+        }
+        if (tid == 0) nlist = sure = 0;
+        // l1 lives in the first warps only when G is small: both maxima go through shared memory
+        if (lane == 0) {
+            red[warp] = big;
+            scan[warp] = __float_as_int(l1);
+        }
+        for (int i = tid; i < 2 * CT; i += CT) hist[i] = hist2[i] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < have; i += blockDim.x) {
-            const unsigned long long k = key[i];
-            if ((k & mask) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+        for (int w = 0; w < CT / 32; w++) {
+            big = fmaxf(big, red[w]);
+            l1 = fmaxf(l1, __int_as_float(scan[w]));
         }
         __syncthreads();
-        if (threadIdx.x < 32) {   // lane l holds digits 255 - 8l .. 248 - 8l, from the top
-            int v[8], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) sum += v[j] = hist[255 - 8 * (int)threadIdx.x - j];
-            int incl = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(kAll, incl, o);
-                if ((int)threadIdx.x >= o) incl += y;
-            }
-            int above = incl - sum;
-            if (above < need && incl >= need) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (above + v[j] >= need) {
-                        sh_digit = 255 - 8 * (int)threadIdx.x - j;
-                        sh_above = above;
-                        sh_in = v[j];
-                        break;
-                    }
-                    above += v[j];
-                }
-            }
-        }
-        __syncthreads();
-        need -= sh_above;
-        prefix |= (unsigned long long)sh_digit << shift;
-        mask |= 255ull << shift;
-        const bool whole = sh_in == need;   // every key of this prefix is taken: no further digit matters
-        __syncthreads();
-        if (whole) break;
     }
-    // taken: keys above the prefix (masked), and the first `need` that share it
-    int base = 0, eq_base = 0;
-    for (int i0 = 0; i0 < have; i0 += blockDim.x) {
-        const int i = i0 + threadIdx.x;
-        const unsigned long long k = i < have ? key[i] & mask : 0ull;
-        const bool eq = i < have && k == prefix;
-        int total_eq, total;
-        const int eq_rank = block_scan_incl(eq, scan, &total_eq) + eq_base;
-        const bool take = i < have && (k > prefix || (eq && eq_rank <= need));
+    const float E = (c.D > 128 ? 0x1p-13f : 0x1p-14f) * l1 * big;
+    // ---- tau: the m-th largest key
+    unsigned prefix = 0, mask = 0;
+    int need = m;
+    for (int d = 0; d < 4; d++) {
+        const int shift = d == 0 ? 22 : d == 1 ? 12 : d == 2 ? 2 : 0, bits = d == 3 ? 2 : 10;
+        int *hs = d & 1 ? hist2 : hist, *other = d & 1 ? hist : hist2;
+        for (int i = tid; i < (have + CT - 1) / CT * CT; i += CT) {
+            const unsigned k = i < have ? key_of(i) : 0u;
+            hist_add(hs, (k >> shift) & ((1u << bits) - 1), i < have && (k & mask) == prefix);
+        }
+        __syncthreads();
+        pick_bin(hs, need, scan, got);
+        need -= got[1];
+        prefix |= (unsigned)got[0] << shift;
+        mask |= ((1u << bits) - 1) << shift;
+        if (d < 3) {
+            for (int i = tid; i < 2 * CT; i += CT) other[i] = 0;
+            __syncthreads();   // got is read, the next histogram clear
+        }
+    }
+    const bool full = prefix == kAll;   // enough pages that are always taken: the lowest of them
+    const unsigned tb = prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix;
+    const float tau = __uint_as_float(tb);
+    const bool know = E < INFINITY && prefix != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
+    const float above = know ? tau + 2.0f * E : 3.4e38f, below = know ? tau - 2.0f * E : -INFINITY;
+    if (!full) {
+        for (int i = tid; i < have; i += CT) {
+            if (always(i)) {
+                atomicAdd(&sure, 1);
+                continue;
+            }
+            const float x = __ldcg(score + i);
+            if (know && x > above) atomicAdd(&sure, 1);
+            else if (!know || x >= below) {
+                const int at = atomicAdd(&nlist, 1);
+                if (at < CLIST) list[at] = i;
+            }
+        }
+        __syncthreads();
+        const int r = m - sure, nb = nlist;   // r >= 1 of the nb pages between are taken
+        if (nb <= CLIST) {
+            if (nb > r)
+                for (int i = warp; i < nb; i += CT / 32) {
+                    const unsigned long long k = exact_key(a, s, t, g, list[i]);
+                    if (lane == 0) lkey[i] = k;
+                }
+            __syncthreads();
+            for (int i = tid; i < nb; i += CT) {
+                int better = 0;
+                if (nb > r)
+                    for (int j = 0; j < nb; j++)
+                        better += lkey[j] > lkey[i] || (lkey[j] == lkey[i] && list[j] < list[i]);
+                score[list[i]] = better < r ? INFINITY : -INFINITY;
+            }
+        } else {   // very many: 64-bit keys of all of them, and radix selection over these
+            unsigned long long *key = a.key + (long long)row * c.mp;
+            for (int i = warp; i < have; i += CT / 32) {
+                const float x = __ldcg(score + i);
+                const bool in = !always(i) && !(know && x > above) && (!know || x >= below);
+                const unsigned long long k = in ? exact_key(a, s, t, g, i) : 0ull;
+                // a page of the list has a key of at least 1, so that 0 marks the others; NaN and missing pages get 1
+                if (lane == 0) key[i] = in ? max(k, 1ull) : 0ull;
+            }
+            __syncthreads();
+            unsigned long long pre = 0, msk = 0;
+            int left = r;
+            for (int shift = 54; shift >= -6; shift -= 10) {
+                const int sh = max(shift, 0), bits = shift < 0 ? 4 : 10;
+                for (int i = tid; i < 2 * CT; i += CT) hist[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < (have + CT - 1) / CT * CT; i += CT) {
+                    const unsigned long long k = i < have ? key[i] : 0ull;
+                    hist_add(hist, (int)(k >> sh) & ((1 << bits) - 1), k != 0ull && (k & msk) == pre);
+                }
+                __syncthreads();
+                pick_bin(hist, left, scan, got);
+                left -= got[1];
+                pre |= (unsigned long long)got[0] << sh;
+                msk |= (unsigned long long)((1 << bits) - 1) << sh;
+                __syncthreads();
+            }
+            int eq0 = 0;
+            for (int i0 = 0; i0 < have; i0 += CT) {   // ties: the lowest places
+                const int i = i0 + tid;
+                const unsigned long long k = i < have ? key[i] : 0ull;
+                int total;
+                const int rank = block_scan_incl(k != 0ull && k == pre, scan, &total) + eq0;
+                if (k != 0ull) score[i] = k > pre || (k == pre && rank <= left) ? INFINITY : -INFINITY;
+                eq0 += total;
+            }
+        }
+        __syncthreads();   // the decided scores are written
+    }
+    int base = 0;
+    for (int i0 = 0; i0 < have && base < m; i0 += CT) {
+        const int i = i0 + tid;
+        const bool take = i < have && (always(i) || (!full && __ldcg(score + i) > above));
+        int total;
         const int at = block_scan_incl(take, scan, &total) + base;
-        if (take) out[at - 1] = i;
+        if (take && at <= m) out[at - 1] = i;
         base += total;
-        eq_base += total_eq;
     }
 }
 
@@ -481,147 +737,141 @@ __global__ void __launch_bounds__(512) kv_choose_k(SelectArgs a) {
 struct EvictArgs {
     KvDev c;
     const int *len;
-    int keep, first, recent;
+    int keep, first, recent, pages;
     float *acc;
     int *pos;
     long long ms, mh;
     int *src;        // [row (s, g)][keep]: the slot that moves into slot k, or -1
     int *holes;      // [row][keep]: given-up slots below keep
-    int *used;       // [row]: slots in use
+    int *flag;       // [row][pages]: the page loses or gets a row
+    int *todo;       // [row][pages]: those pages
+    int *used;       // [row][2]: slots in use, pages to do
     int *len_out;
 };
 
-constexpr int EV_BINS = 2048;
-// Which slots stay, and where the movers go: one CTA per row (s, g). The threshold key by radix selection over digits of
-// 11, 11 and 10 bits, then one ordered pass: below `keep` the given-up slots are listed, from there on the j-th staying
-// slot becomes the source of the j-th of them.
-__global__ void __launch_bounds__(1024) kv_rank_k(EvictArgs a) {
-    __shared__ int hist[EV_BINS];
-    __shared__ int scan[32];
-    __shared__ int sh_digit, sh_above, sh_in, sh_new;
+constexpr int ET = 1024, EIPT = 8;   // threads, slots a thread takes in a row in the ordered passes
+// Which slots stay, and where the movers go: one CTA per row (s, g). The threshold key (the keep-th largest) by radix
+// selection over digits of 11, 11 and 10 bits, warps adding equal digits together; then one ordered pass: below `keep` the
+// given-up slots are listed and their pages marked, from there on the j-th staying slot becomes the source of the j-th of
+// them. acc and pos come from L1 after the first pass.
+__global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArgs a) {
+    __shared__ int hist[2 * ET], hist2[2 * ET];
+    __shared__ int scan[32], got[3], sh_new;
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const int row = blockIdx.x, s = row / c.HKV, g = row - s * c.HKV;
+    const int row = blockIdx.x, s = row / c.HKV, g = row - s * c.HKV, tid = threadIdx.x;
     const int n = min(max(a.len[s], 0), c.cap), keep = a.keep;
-    if (threadIdx.x == 0) a.used[row] = n;
+    if (tid == 0) {
+        a.used[2 * row] = n;
+        a.used[2 * row + 1] = 0;
+        sh_new = INT_MIN;
+    }
     if (n <= keep) return;
     const float *acc = a.acc + s * a.ms + g * a.mh;
     const int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
-    int *src = a.src + (long long)row * keep, *holes = a.holes + (long long)row * keep;
-    if (threadIdx.x == 0) sh_new = INT_MIN;
+    int *src = a.src + (long long)row * keep, *holes = a.holes + (long long)row * keep, *flag = a.flag + (long long)row * a.pages;
+    for (int i = tid; i < a.pages; i += ET) flag[i] = 0;
+    for (int i = tid; i < 2 * ET; i += ET) hist[i] = hist2[i] = 0;
     __syncthreads();
     int newest = n - 1;
     if (pos) {
         int m = INT_MIN;
-        for (int k = threadIdx.x; k < n; k += blockDim.x) m = max(m, pos[k]);
+        for (int k = tid; k < n; k += ET) m = max(m, __ldg(pos + k));
         m = __reduce_max_sync(kAll, m);
-        if ((threadIdx.x & 31) == 0) atomicMax(&sh_new, m);
+        if ((tid & 31) == 0) atomicMax(&sh_new, m);
         __syncthreads();
         newest = sh_new;
     }
     const long long old = (long long)newest - a.recent;
     auto key_of = [&](int k) -> unsigned {
-        const int p = pos ? pos[k] : k;
-        return p < a.first || p > old ? kAll : weight_key(acc[k]);
+        const int p = pos ? __ldg(pos + k) : k;
+        return p < a.first || p > old ? kAll : weight_key(__ldg(acc + k));
     };
     unsigned prefix = 0, mask = 0;
     int need = keep;
-    for (int d = 0; d < 3; d++) {
+    bool whole = false;   // every key of the prefix stays: no further digit matters
+    for (int d = 0; d < 3 && !whole; d++) {
         const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-        for (int i = threadIdx.x; i < EV_BINS; i += blockDim.x) hist[i] = 0;
-        __syncthreads();
-        for (int k = threadIdx.x; k < n; k += blockDim.x) {
-            const unsigned x = key_of(k);
-            if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & ((1u << bits) - 1)], 1);
+        int *hs = d & 1 ? hist2 : hist, *other = d & 1 ? hist : hist2;
+        for (int k0 = 0; k0 < n; k0 += ET) {
+            const int k = k0 + tid;
+            const unsigned x = k < n ? key_of(k) : 0u;
+            hist_add(hs, (x >> shift) & ((1u << bits) - 1), k < n && (x & mask) == prefix);
         }
         __syncthreads();
-        // thread i: bins 2047 - 2i and 2046 - 2i, from the top
-        const int b0 = EV_BINS - 1 - 2 * (int)threadIdx.x;
-        const int v0 = hist[b0], v1 = hist[b0 - 1];
-        int total;
-        const int incl = block_scan_incl(v0 + v1, scan, &total);
-        const int above = incl - v0 - v1;
-        if (above < need && incl >= need) {
-            const bool second = above + v0 < need;
-            sh_digit = second ? b0 - 1 : b0;
-            sh_above = second ? above + v0 : above;
-            sh_in = second ? v1 : v0;
-        }
-        __syncthreads();
-        need -= sh_above;
-        prefix |= (unsigned)sh_digit << shift;
+        pick_bin(hs, need, scan, got);
+        need -= got[1];
+        prefix |= (unsigned)got[0] << shift;
         mask |= ((1u << bits) - 1) << shift;
-        const bool whole = sh_in == need;
-        __syncthreads();
-        if (whole) break;
+        whole = got[2] == need;
+        if (d < 2)
+            for (int i = tid; i < 2 * ET; i += ET) other[i] = 0;
+        __syncthreads();   // got is read, the next histogram clear
     }
-    int eq_base = 0, out_base = 0;
-    for (int k0 = 0; k0 < keep; k0 += blockDim.x) {
-        const int k = k0 + threadIdx.x;
-        const bool in = k < keep;
-        const unsigned x = in ? key_of(k) & mask : 0u;
-        const bool eq = in && x == prefix;
-        int total_eq, total;
-        const int eq_rank = block_scan_incl(eq, scan, &total_eq) + eq_base;
-        const bool hole = in && !(x > prefix || (eq && eq_rank <= need));
-        const int at = block_scan_incl(hole, scan, &total) + out_base;
-        if (in) src[k] = -1;
-        if (hole) holes[at - 1] = k;
-        eq_base += total_eq;
-        out_base += total;
+    // EIPT slots in a row per thread; with `whole` every key equal to the prefix stays and their order does not matter
+    int eq_base = 0, holes_n = 0, moved = 0;
+    for (int phase = 0; phase < 2; phase++) {
+        const int from = phase ? keep : 0, to = phase ? n : keep;
+        for (int k0 = from; k0 < to; k0 += ET * EIPT) {
+            const int k1 = k0 + tid * EIPT;
+            unsigned eq = 0, gt = 0;
+#pragma unroll
+            for (int j = 0; j < EIPT; j++) {
+                const unsigned x = k1 + j < to ? key_of(k1 + j) & mask : 0u;
+                if (k1 + j < to && x == prefix) eq |= 1u << j;
+                if (k1 + j < to && x > prefix) gt |= 1u << j;
+            }
+            unsigned stay = gt | eq;
+            if (!whole) {   // of the equal ones only the first `need`
+                int total;
+                int before = block_scan_incl(__popc(eq), scan, &total) - __popc(eq) + eq_base;
+                eq_base += total;
+                stay = gt;
+                for (unsigned e = eq; e && before < need; e &= e - 1, before++) stay |= e & -e;
+            }
+            const unsigned in = k1 < to ? (to - k1 >= EIPT ? (1u << EIPT) - 1 : (1u << (to - k1)) - 1) : 0u;
+            const unsigned hit = phase ? stay & in : ~stay & in;
+            int total;
+            int at = block_scan_incl(__popc(hit), scan, &total) - __popc(hit);
+            if (phase == 0) {
+                at += holes_n;
+                holes_n += total;
+#pragma unroll
+                for (int j = 0; j < EIPT; j++) {
+                    if (!(in >> j & 1)) continue;
+                    src[k1 + j] = -1;
+                    if (hit >> j & 1) {
+                        holes[at++] = k1 + j;
+                        flag[page_quot(c.div, k1 + j)] = 1;
+                    }
+                }
+            } else {
+                at += moved;
+                moved += total;
+                for (unsigned e = hit; e; e &= e - 1, at++)
+                    if (at < holes_n) src[holes[at]] = k1 + __ffs(e) - 1;
+            }
+        }
+        __syncthreads();   // the list of holes is written
     }
-    __syncthreads();   // the list of holes is written
-    int in_base = 0;
-    for (int k0 = keep; k0 < n; k0 += blockDim.x) {
-        const int k = k0 + threadIdx.x;
-        const bool in = k < n;
-        const unsigned x = in ? key_of(k) & mask : 0u;
-        const bool eq = in && x == prefix;
-        int total_eq, total;
-        const int eq_rank = block_scan_incl(eq, scan, &total_eq) + eq_base;
-        const bool stay = in && (x > prefix || (eq && eq_rank <= need));
-        const int at = block_scan_incl(stay, scan, &total) + in_base;
-        if (stay && at <= out_base) src[holes[at - 1]] = k;
-        eq_base += total_eq;
-        in_base += total;
+    // the pages that change: those with holes, and the one that held slots on both sides of keep
+    int base = 0;
+    for (int i0 = 0; i0 < a.pages; i0 += ET) {
+        const int i = i0 + tid;
+        const bool hit = i < a.pages && (flag[i] || (i == a.pages - 1 && keep % c.page));
+        int total;
+        const int at = block_scan_incl(hit, scan, &total) + base;
+        if (hit) a.todo[(long long)row * a.pages + at - 1] = i;
+        base += total;
     }
+    if (tid == 0) a.used[2 * row + 1] = base;
 }
 
-// The moves: one warp per (page below keep, row). lpr lanes carry a row, 16 bytes each; the bounds of a page that got or
-// lost rows are taken over the rows it now holds, the movers' from their sources.
-__global__ void __launch_bounds__(256) kv_move_k(EvictArgs a, int pages, int lpr) {
-    pdl_next();
-    pdl_wait();
+// The rows of one page (page id of the pool, its first `rows` slots; src: their sources or -1), by one warp.
+__device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int id, int rows, const int *src, int lpr) {
     const KvDev &c = a.c;
     const int lane = threadIdx.x & 31;
-    const long long w = blockIdx.x * 8LL + (threadIdx.x >> 5);
-    const long long row = w / pages;
-    if (row >= (long long)c.ns * c.HKV) return;
-    const int place = (int)(w % pages), s = (int)(row / c.HKV), g = (int)(row % c.HKV);
-    const int n = a.used[row], keep = a.keep;
-    if (place == 0 && g == 0 && lane == 0) a.len_out[s] = min(n, keep);
-    if (n <= keep) return;
-    const int k0 = place * c.page, rows = min(c.page, keep - k0);
-    if (rows <= 0) return;
-    const int *src = a.src + row * keep + k0;
-    bool any = false;
-    for (int i = lane; i < rows; i += 32) any = any || src[i] >= 0;
-    any = __any_sync(kAll, any);
-    const bool cut = rows < c.page;   // the page held slots at and above keep
-    if (!any && !cut) return;
-    const int id = page_id(c.table, c.ts, s, place, c.mp, c.n_pages);
-    if (any) {
-        float *acc = a.acc + s * a.ms + g * a.mh;
-        int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
-        for (int i = lane; i < rows; i += 32) {
-            const int k = src[i];
-            if (k < 0) continue;
-            acc[k0 + i] = acc[k];
-            if (pos) pos[k0 + i] = pos[k];
-        }
-    }
-    if (id < 0) return;
     const int rpw = 32 / lpr, sub = lane / lpr, ch = lane - sub * lpr;
     const bool live = ch * 8 < c.D;
     const bool bounds = c.bounds != nullptr;
@@ -669,11 +919,49 @@ __global__ void __launch_bounds__(256) kv_move_k(EvictArgs a, int pages, int lpr
     *reinterpret_cast<uint4 *>(b + c.D) = make_uint4(as_u(mx[0]), as_u(mx[1]), as_u(mx[2]), as_u(mx[3]));
 }
 
+// The moves: the warps of `ctas` CTAs per row take the row's changed pages in turn. lpr lanes carry a row, 16 bytes each; the
+// bounds of a page are taken over the rows it now holds, the movers' from their sources. Every source lies at or above keep
+// and every target below, so that the order of the moves does not matter. Bound by memory: rows in and out.
+__global__ void __launch_bounds__(256) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
+    pdl_next();
+    pdl_wait();
+    const KvDev &c = a.c;
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x / ctas, part = blockIdx.x - row * ctas;
+    const int s = row / c.HKV, g = row - s * c.HKV, keep = a.keep;
+    if (part == 0 && g == 0 && threadIdx.x == 0) a.len_out[s] = min(a.used[2 * row], keep);
+    const int todo = a.used[2 * row + 1];
+    for (int w = part * 8 + (threadIdx.x >> 5); w < todo; w += ctas * 8) {
+        const int place = a.todo[(long long)row * a.pages + w];
+        const int k0 = place * c.page, rows = min(c.page, keep - k0);
+        const int *src = a.src + (long long)row * keep + k0;
+        const int id = page_id(c.table, c.ts, s, place, c.mp, c.n_pages);
+        float *acc = a.acc + s * a.ms + g * a.mh;
+        int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
+        for (int i = lane; i < rows; i += 32) {
+            const int k = src[i];
+            if (k < 0) continue;
+            acc[k0 + i] = acc[k];
+            if (pos) pos[k0 + i] = pos[k];
+        }
+        if (id >= 0) move_page(a, s, g, id, rows, src, lpr);
+    }
+}
+
 // bytes that the acc or pos rows of all heads and streams span
 size_t marks_bytes(const KvDev &c, int64_t ms, int64_t mh) {
     return ((size_t)std::max(c.ns - 1, 0) * (size_t)std::max<int64_t>(ms, 0) + (size_t)(c.HKV - 1) * (size_t)std::max<int64_t>(mh, 0) +
             (size_t)c.cap) * 4;
 }
+template <int DP>
+int score_launch(const SelectArgs &a, const KvCall &call, dim3 grid) {
+    using C = ScoreCfg<DP>;
+    static bool attr[kMaxDevices] = {};
+    G9_CU(smem_limit_once(kv_score_k<DP>, C::smem(C::TG), attr));
+    G9_CU(launch_pdl(kv_score_k<DP>, grid, dim3(SW * 32), C::smem(a.tg), call.st, a));
+    return launched("kv_score");
+}
+
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 }  // namespace
@@ -778,7 +1066,8 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     if (int e = kv_begin(c, H, sync, who, &a.c, &call)) return e;
     if (c->ns == 0 || nq <= 0 || nsel == 0) return 0;
     const long long rows = (long long)c->ns * nq * c->HKV;
-    if (rows > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows (stream, token, head) in one call", who, rows);
+    if (rows > INT_MAX || c->ns * (long long)c->HKV > 65535)
+        return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows (stream, token, head) in one call", who, rows);
     G9_TRY(kv_operand(call, Q, who, "Q"));
     G9_TRY(kv_operand(call, vis, who, "vis"));
     G9_TRY(kv_operand(call, sel, who, "sel"));
@@ -795,20 +1084,36 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     a.qs = qs;
     a.vis = vis;
     a.sel = sel;
+    a.hg = (a.G + 7) / 8;
+    const long long tiles = (long long)nq * a.hg;
+    const int dp = c->D <= 64 ? 64 : c->D <= 128 ? 128 : 256;
+    // a CTA reads its pages once for as many row tiles as its shared memory holds
+    const long long tg = std::min<long long>(tiles, dp == 64 ? ScoreCfg<64>::TG : dp == 128 ? ScoreCfg<128>::TG : ScoreCfg<256>::TG);
+    const long long zt = a.hg > tg ? a.hg : tg / a.hg * a.hg, zs = (tiles + zt - 1) / zt;
+    if (zs > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %d tokens of %d heads in one call", who, nq, H);
+    a.tiles = (int)tiles;
+    a.tg = (int)std::min(tg, zt);
+    a.zt = (int)zt;
+    // steps of a warp: about eight CTAs per SM over all (stream, head) rows, at most 8 steps, which amortise the queries
+    const long long all = (c->mp + SPAGES - 1) / SPAGES, sg = (long long)c->ns * c->HKV * zs;
+    a.steps = (int)std::min<long long>(8, std::max<long long>(1, all * sg / (8LL * SW * call.d->sm_count)));
+    const int ctas = (int)std::max<long long>(1, (all + SW * a.steps - 1) / (SW * a.steps));
+    const size_t score = up256((size_t)rows * c->mp * 4), key = up256((size_t)rows * c->mp * 8),
+                 l1 = up256((size_t)c->ns * nq * H * 4), peak = up256((size_t)sg * ctas * SW * 4);
     void *buf = nullptr;
     unsigned *cnt = nullptr;
-    G9_TRY(kv_workspace(ws, call, who, std::max<size_t>((size_t)rows * c->mp * 8, 256), 0, &buf, &cnt));
-    a.key = (unsigned long long *)buf;
-    const size_t smem = (size_t)a.G * c->D * 8 + (size_t)SEL_PAGES * (4 * c->D + 16) + SEL_PAGES * 8;
-    if (smem > 227 * 1024) return GEN9BLAS_DECLINED;
-    static bool attr[kMaxDevices] = {};
-    G9_CU(smem_limit_once(kv_score_k, 227 * 1024, attr));
+    G9_TRY(kv_workspace(ws, call, who, score + key + l1 + peak, 0, &buf, &cnt));
+    a.score = (float *)buf;
+    a.key = (unsigned long long *)((char *)buf + score);
+    a.l1 = (float *)((char *)buf + score + key);
+    a.peak = (float *)((char *)buf + score + key + l1);
     if (c->mp > 0) {
-        G9_CU(launch_pdl(kv_score_k, dim3((unsigned)((c->mp + SEL_PAGES - 1) / SEL_PAGES), (unsigned)rows), dim3(128), smem,
-                         call.st, a));
-        G9_TRY(launched("kv_score"));
+        const dim3 grid((unsigned)ctas, (unsigned)(c->ns * c->HKV), (unsigned)zs);
+        if (dp == 64) G9_TRY(score_launch<64>(a, call, grid));
+        else if (dp == 128) G9_TRY(score_launch<128>(a, call, grid));
+        else G9_TRY(score_launch<256>(a, call, grid));
     }
-    G9_CU(launch_pdl(kv_choose_k, dim3((unsigned)rows), dim3(512), 0, call.st, a));
+    G9_CU(launch_pdl(kv_choose_k, dim3((unsigned)rows), dim3(CT), 0, call.st, a, ctas));
     G9_TRY(launched("kv_choose"));
     const KvWrite w[1] = {{sel, (size_t)rows * nsel * 4}};
     return kv_finish(call, sync, w, 1);
@@ -840,18 +1145,21 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     a.len_out = len_out;
     void *buf = nullptr;
     unsigned *cnt = nullptr;
-    const size_t list = up256((size_t)rows * a.keep * 4);
-    G9_TRY(kv_workspace(ws, call, who, 2 * list + up256((size_t)rows * 4), 0, &buf, &cnt));
+    a.pages = (a.keep - 1) / c->page + 1;
+    const size_t list = up256((size_t)rows * a.keep * 4), pages = up256((size_t)rows * a.pages * 4);
+    G9_TRY(kv_workspace(ws, call, who, 2 * list + 2 * pages + up256((size_t)rows * 8), 0, &buf, &cnt));
     a.src = (int *)buf;
     a.holes = (int *)((char *)buf + list);
-    a.used = (int *)((char *)buf + 2 * list);
-    G9_CU(launch_pdl(kv_rank_k, dim3((unsigned)rows), dim3(1024), 0, call.st, a));
+    a.flag = (int *)((char *)buf + 2 * list);
+    a.todo = (int *)((char *)buf + 2 * list + pages);
+    a.used = (int *)((char *)buf + 2 * list + 2 * pages);
+    G9_CU(launch_pdl(kv_rank_k, dim3((unsigned)rows), dim3(ET), 0, call.st, a));
     G9_TRY(launched("kv_rank"));
-    const int pages = (a.keep + c->page - 1) / c->page;
+    // a page per warp where the rows are few, up to about 16 CTAs per SM in all
+    const long long most = (a.pages + 7) / 8, ctas = std::max<long long>(1, std::min(most, 16LL * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
-    const long long warps = rows * pages;
-    if ((warps + 7) / 8 > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld pages in one call", who, warps);
-    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, call.st, a, pages, lpr));
+    if (rows * ctas > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows in one call", who, rows);
+    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(256), 0, call.st, a, (int)ctas, lpr));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
     const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};

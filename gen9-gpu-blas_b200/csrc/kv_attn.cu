@@ -34,7 +34,6 @@ struct PagedArgs {
     float *O, *lse;
     float *part;              // partial results, slot (CTA + unit)
     unsigned *cnt;            // arrivals per unit, zero before and after each launch
-    int parts;                // few units: cut into parts, one CTA a part
     float *score;             // scores in base 2 [(s, t, h)][score_row], NULL without weights
     long long score_row;
     float *lse2;              // log2 of the sum of 2^score, [(s, t, h)], with weights
@@ -57,6 +56,7 @@ struct PagedCfg {
     static constexpr int ROWOFF = AW * AKEYS * 16;
     static constexpr int SMEM = RING + QF + KIDX + ROWOFF + ROWS * 4;
     static constexpr int CTAS = DP == 256 ? 1 : 2;
+    static constexpr int COST = DP == 64 ? 32 : 16;             // steps that a CTA reads in the time of a segment's latencies
 };
 
 // Steps of one outer index: its slots [k0, k1) from the first visible one on, held to a multiple of a step; at least one,
@@ -111,50 +111,42 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- this CTA's work. Every warp finds it for itself: T steps in all; the outer index `outer` that holds the CTA's
-    // first step (or part), `pre` steps (parts) before it.
-    // Few units (at most half the CTAs): each is cut into parts of about `chunk` steps, one CTA a part; with chunk at least
-    // T / (CTAs - units) there are never more parts than CTAs. Otherwise CTA b takes the steps [b·chunk, (b + 1)·chunk) of
-    // all units in a row, a segment of a unit at a time: a segment costs a CTA about 6 µs of latencies besides its steps,
-    // so that 8 heads of one stream of 1000 keys take 10.4 µs in parts and 15.1 µs in segments.
-    int T = 0, pre = 0, outer = 0, n0 = 0;   // n0: steps of outer index `lane`
+    // ---- this CTA's work. Every warp finds it for itself. All units' steps in a row are cut into equal runs of `chunk`, one
+    // a CTA, a segment of a unit at a time. A segment costs a CTA about 6 µs of latencies besides its steps (row data, first
+    // copies, merge), so that each unit is counted COST steps longer than it is, at its start: a CTA that begins a unit in
+    // the middle of its run gets that much less to read, and short units begin a run of their own. (Equal runs without it took
+    // 32.4 µs at 8 streams of 4096 keys, a whole number of CTAs per unit 27.7; 14.1 and 10.4 at one stream of 1000.)
+    int T = 0, pre = 0, outer = 0, n0 = 0;   // steps in all; before outer index `outer`; of outer index `lane`
     if (a.sel) {
-        T = a.outer * a.inner * a.sel_steps;
+        T = a.outer * a.inner * (a.sel_steps + C::COST);
     } else {
         for (int o = lane; o < a.outer; o += 32) {
             int k0, k1;
-            const int n = outer_steps(a, o, k0, k1);
+            const int n = outer_steps(a, o, k0, k1) + C::COST;
             if (o == lane) n0 = n;
             T += n * a.inner;
         }
         T = __reduce_add_sync(kAll, T);
     }
-    const int b = blockIdx.x, units = a.outer * a.inner;
-    const bool parts = a.parts;
-    const unsigned over = parts ? gridDim.x - units : gridDim.x;
-    const int chunk = (int)(((unsigned)T + over - 1) / over + AW - 1) / AW * AW;
-    // ⌈2^32 / chunk⌉: n steps have (n + chunk - 1)·inv >> 32 parts, exact below 2^32 / chunk steps (the host keeps T there)
-    const unsigned inv_chunk = 0xffffffffu / (unsigned)chunk + 1u;
-    auto per_unit = [&](int n) { return parts ? (int)__umulhi((unsigned)(n + chunk - 1), inv_chunk) : n; };
-    if (!parts && (long long)b * chunk >= T) return;
-    const int lo = parts ? b : b * chunk, hi = parts ? b + 1 : min(lo + chunk, T);
+    const int b = blockIdx.x;
+    const int chunk = (int)(((unsigned)T + gridDim.x - 1) / gridDim.x + AW - 1) / AW * AW;
+    if ((long long)b * chunk >= T) return;
+    const int lo = b * chunk, hi = min(lo + chunk, T);
     if (a.sel) {
-        const int per = a.inner * per_unit(a.sel_steps);
+        const int per = a.inner * (a.sel_steps + C::COST);
         outer = lo / per;
         pre = outer * per;
-        if (outer >= a.outer) return;   // more CTAs than parts
     } else {
         for (int o0 = 0;; o0 += 32) {
-            if (o0 >= a.outer) return;
             int k0, k1;
-            const int n = o0 + lane < a.outer ? per_unit(o0 ? outer_steps(a, o0 + lane, k0, k1) : n0) * a.inner : 0;
+            const int n = o0 + lane < a.outer ? (o0 ? outer_steps(a, o0 + lane, k0, k1) + C::COST : n0) * a.inner : 0;
             int x = n;
 #pragma unroll
             for (int i = 1; i < 32; i <<= 1) {
                 const int y = __shfl_up_sync(kAll, x, i);
                 if (lane >= i) x += y;
             }
-            const unsigned past = __ballot_sync(kAll, pre + x > lo);
+            const unsigned past = __ballot_sync(kAll, pre + x > lo);   // lo < T: found before the indices run out
             if (past) {
                 const int l = __ffs(past) - 1;
                 outer = o0 + l;
@@ -174,29 +166,18 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
 
     for (int at = lo; at < hi;) {
         int k0, k1;
-        const int n = outer_steps(a, outer, k0, k1), pu = per_unit(n), iu = (at - pre) / pu;
+        const int n = outer_steps(a, outer, k0, k1), nv = n + C::COST, iu = (at - pre) / nv;
         if (iu >= a.inner) {
-            pre += pu * a.inner;
+            pre += nv * a.inner;
             outer++;
             continue;
         }
-        const int u = outer * a.inner + iu, rs0 = pre + iu * pu;
-        // steps [sb, se) of the unit, kept in slot `slot`; the unit's nsl slots follow one another from `slot0` on in key order
-        int sb = at - rs0, se = min(hi - rs0, n), slot, slot0, nsl;
-        if (parts) {
-            const int even = ((n + pu - 1) / pu + AW - 1) / AW * AW;
-            slot0 = rs0;
-            slot = at;
-            nsl = pu;
-            sb = min(sb * even, n);
-            se = min(sb + even, n);
-            at++;
-        } else {
-            at = rs0 + se;
-            slot0 = rs0 / chunk + u;
-            slot = b + u;
-            nsl = (rs0 + n - 1) / chunk + u - slot0 + 1;
-        }
+        const int u = outer * a.inner + iu, us = pre + iu * nv, rs0 = us + C::COST;   // the unit's run, its first step in it
+        const int sb = max(at - rs0, 0), se = min(hi - rs0, n);
+        at = us + nv;
+        if (se <= 0) break;   // this CTA's run ends before the unit's first step
+        // the unit's nsl slots, one a CTA, follow one another from slot0 on in key order
+        const int slot = b + u, slot0 = rs0 / chunk + u, nsl = (rs0 + n - 1) / chunk + u - slot0 + 1;
         const int g = page_quot(a.by_tiles, iu), row0 = (iu - g * a.tiles) * ROWS;
         const int s = a.sel ? page_quot(a.by_nq, outer) : outer, t0 = a.sel ? outer - s * a.nq : 0;
         const int live_rows = min(ROWS, a.qn * a.G - row0);
@@ -608,34 +589,47 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
     }
 }
 
-// The softmax weight of score `at` of a row; a row whose scores are all -inf has none.
-__device__ __forceinline__ float weight(const PagedArgs &a, long long row, int at) {
-    const float l2 = __ldcg(a.lse2 + row);
-    return l2 == -INFINITY ? 0.0f : exp2f(__ldcg(a.score + row * a.score_row + at) - l2);
-}
+// The softmax weight of a score; a row whose scores are all -inf has none.
+__device__ __forceinline__ float weight(float score, float l2) { return l2 == -INFINITY ? 0.0f : exp2f(score - l2); }
 
 // acc[k] += Σ over tokens and the head's queries of 2^(score − lse2), in a fixed order. Without chosen pages a thread per
-// slot; with them one CTA per (stream, head) walks the tokens one after the other, because their choices overlap.
-__global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedArgs a, float *acc, long long ms, long long mh) {
+// four slots (a slot without a page has scores of -inf and gains 0); with them one CTA per (stream, head) walks the tokens
+// one after the other, because their choices overlap.
+__global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedArgs a, float *acc, long long ms, long long mh, int v4) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const KvDev &c = a.c;
-    const long long sg = blockIdx.y;
-    const int s = (int)(sg / c.HKV), g = (int)(sg % c.HKV);
+    const int sg = blockIdx.y, s = sg / c.HKV, g = sg - s * c.HKV;
     float *row = acc + s * ms + g * mh;
     const int vs = a.vis[s];
     if (!a.sel) {
-        const int k = blockIdx.x * 256 + threadIdx.x;
+        const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
         if (k >= seen_slots(vs, a.dvis, a.nq - 1, c.cap)) return;
-        if (page_id(c.table, c.ts, s, page_quot(c.div, k), c.mp, c.n_pages) < 0) return;
-        float sum = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int t = 0; t < a.nq; t++) {
-            const int see = seen_slots(vs, a.dvis, t, c.cap);
-            if (k >= see || k < first_slot(see, a.window)) continue;
+            const int see = seen_slots(vs, a.dvis, t, c.cap), from = first_slot(see, a.window);
+            if (k >= see || k + 3 < from) continue;
             const long long q = ((long long)s * a.nq + t) * a.H + g * a.G;
-            for (int h = 0; h < a.G; h++) sum += weight(a, q + h, k);
+#pragma unroll 4
+            for (int h = 0; h < a.G; h++) {
+                const float l2 = __ldcg(a.lse2 + q + h);
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.score + (q + h) * a.score_row + k));
+                // scores outside [from, see) were not written for this token where its whole step lies outside
+                if (k >= from) sum.x += weight(x.x, l2);
+                if (k + 1 >= from && k + 1 < see) sum.y += weight(x.y, l2);
+                if (k + 2 >= from && k + 2 < see) sum.z += weight(x.z, l2);
+                if (k + 3 >= from && k + 3 < see) sum.w += weight(x.w, l2);
+            }
         }
-        row[k] += sum;
+        if (v4 && k + 3 < c.cap) {
+            float4 w = *reinterpret_cast<const float4 *>(row + k);
+            *reinterpret_cast<float4 *>(row + k) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
+        } else {
+            row[k] += sum.x;
+            if (k + 1 < c.cap) row[k + 1] += sum.y;
+            if (k + 2 < c.cap) row[k + 2] += sum.z;
+            if (k + 3 < c.cap) row[k + 3] += sum.w;
+        }
         return;
     }
     const int n = a.nsel * c.page;
@@ -650,7 +644,7 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
             const int k = place * c.page + j - e * c.page;
             if (k >= see) continue;
             float sum = 0.0f;
-            for (int h = 0; h < a.G; h++) sum += weight(a, q + h, j);
+            for (int h = 0; h < a.G; h++) sum += weight(__ldcg(a.score + (q + h) * a.score_row + j), __ldcg(a.lse2 + q + h));
             row[k] += sum;
         }
         __syncthreads();   // the next token may choose the same pages
@@ -736,7 +730,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     const int nt = rows <= 8 ? 1 : rows <= 16 || dp == 256 ? 2 : 4;
     const long long tiles = (rows + 8 * nt - 1) / (8 * nt), outer = (long long)c->ns * (sel ? nq : 1);
     // never more steps than this; they and the (s, t, h) rows are counted in 32 bits
-    const long long per = sel ? a.sel_steps : (a.c.cap + AKEYS - 1) / AKEYS + 1;
+    const long long per = (sel ? a.sel_steps : (a.c.cap + AKEYS - 1) / AKEYS + 1) + (dp == 64 ? 32 : 16);
     if ((__int128)outer * tiles * c->HKV * per > INT_MAX / 2 || (__int128)c->ns * nq * H > INT_MAX)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld (stream, token) rows of up to %lld slots pass 2^30 steps in one call", who,
                     (long long)c->ns * nq, (long long)per * AKEYS);
@@ -752,11 +746,10 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     int ctas = 1;
     G9_TRY(paged(dp, nt, a, call, true, &ctas));
     // never more CTAs than steps there can be
-    ctas = (int)std::min<long long>(ctas, units + (units * per + AW - 1) / AW);
-    a.parts = 2 * units <= ctas && per < 65536 - 4;   // a part below 2^16 steps: the kernel's division is exact
+    ctas = (int)std::min<long long>(ctas, (units * per + AW - 1) / AW);
     const size_t part = up256((size_t)(ctas + units) * 8 * nt * (dp + 4) * 4);
     const long long heads = (long long)c->ns * nq * H;
-    a.score_row = sel ? (long long)a.nsel * c->page : a.c.cap;
+    a.score_row = ((sel ? (long long)a.nsel * c->page : a.c.cap) + 3) / 4 * 4;   // rows of whole float4
     const size_t lse2 = acc ? up256((size_t)heads * 4) : 0;
     if (acc && (__int128)heads * a.score_row * 4 > ((__int128)1 << 46))
         return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s: weights of %lld rows of %lld slots", who, heads, a.score_row);
@@ -772,8 +765,9 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     if (acc && a.score_row > 0) {
         const long long sg = (long long)c->ns * c->HKV;
         if (sg > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: weights of %lld (stream, head) rows in one call", who, sg);
-        const dim3 grid(sel ? 1u : (unsigned)((a.c.cap + 255) / 256), (unsigned)sg);
-        G9_CU(launch_pdl(kv_weigh_k, grid, dim3(256), 0, call.st, a, acc, (long long)ms, (long long)mh));
+        const dim3 grid(sel ? 1u : (unsigned)((a.c.cap + 1023) / 1024), (unsigned)sg);
+        const int v4 = ((uintptr_t)acc & 15) == 0 && ((ms | mh) & 3) == 0;
+        G9_CU(launch_pdl(kv_weigh_k, grid, dim3(256), 0, call.st, a, acc, (long long)ms, (long long)mh, v4));
         G9_TRY(launched("kv_weigh"));
     }
     const size_t marks = ((size_t)(c->ns - 1) * (size_t)std::max<int64_t>(ms, 0) +

@@ -52,6 +52,11 @@ for _name, (_args, _res) in _SIGNATURES.items():
 _append, _attend, _select, _evict = (_fn[n] for n in ("kv_append", "attn_paged", "kv_select", "kv_evict"))
 _set_stream, _get_stream, _get_device = _fn["set_stream"], _fn["get_stream"], _fn["get_device"]
 _LEGACY = 1   # cudaStreamLegacy: torch's default stream (a null stream would mean the library's own)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # torch's accessor without the Stream object, 1.2 us less
+if _raw_stream is None:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+_f32, _i32 = torch.float32, torch.int32
 
 
 def _check(status, what):
@@ -104,6 +109,7 @@ class PagedKV:
         self.device, self.streams, self.slots = K.device, table.shape[0], table.shape[1] * page
         self.heads, self.page, self.dim = heads, page, dim
         self._index = K.device.index
+        self._per_stream = torch.Size([self.streams])
         self._ws = workspace.handle if workspace is not None else None
 
         def span(x):
@@ -112,6 +118,7 @@ class PagedKV:
         self._c = _Cache(dim, heads, page, pages, K.data_ptr(), ks[0], ks[2], ks[1], span(K), V.data_ptr(), vs[0], vs[2],
                          vs[1], span(V), bounds.data_ptr() if bounds is not None else None, table.data_ptr(),
                          table.stride(0), table.shape[1], table.shape[0])
+        self._ref = ctypes.byref(self._c)
         if _fn["init"]():
             raise RuntimeError(_fn["error"]().decode(errors="replace"))
 
@@ -120,9 +127,9 @@ class PagedKV:
         stream, device = _get_stream(), _get_device()
         if device != self._index:
             _check(_fn["set_device"](self._index), what)
-        _set_stream(torch.cuda.current_stream(self._index).cuda_stream or _LEGACY)
+        _set_stream(_raw_stream(self._index) or _LEGACY)
         try:
-            status = fn(self._c, *args)
+            status = fn(self._ref, *args)
         finally:
             if device != self._index:
                 _fn["set_device"](device)
@@ -130,43 +137,58 @@ class PagedKV:
         if status:
             _check(status, what)
 
+    # The checks run in every call, so their messages are put together only when one fails.
     def _rows(self, name, x, heads):
-        _need(x.dtype == torch.float32 and x.dim() == 4 and x.device == self.device and x.shape[0] == self.streams and
-              x.shape[3] == self.dim and (heads is None or x.shape[2] == heads) and (x.stride(3) == 1 or self.dim == 1),
-              f"{name}: float32 [{self.streams}, tokens, heads, {self.dim}] on {self.device}, unit stride last")
+        n, st = x.shape, x.stride()
+        if not (x.dtype is _f32 and len(n) == 4 and x.get_device() == self._index and n[0] == self.streams and n[3] == self.dim
+                and (heads is None or n[2] == heads) and st[3] == 1):
+            raise ValueError(f"{name}: float32 [{self.streams}, tokens, {heads or 'heads'}, {self.dim}] on {self.device}, unit "
+                             f"stride last; got {x.dtype} {list(n)} on {x.device}")
+        return n, st
 
     def _ints(self, name, x):
-        _need(x.dtype == torch.int32 and x.dim() == 1 and x.shape[0] == self.streams and x.device == self.device and
-              (x.stride(0) == 1 or self.streams <= 1), f"{name}: contiguous int32 [{self.streams}] on {self.device}")
+        if not (x.dtype is _i32 and x.shape == self._per_stream and x.get_device() == self._index and x.is_contiguous()):
+            raise ValueError(f"{name}: contiguous int32 [{self.streams}] on {self.device}; got {x.dtype} {list(x.shape)} on "
+                             f"{x.device}")
         return x.data_ptr()
 
     def _marks(self, acc, pos):
-        ms = mh = 0
-        for name, x, dt in (("acc", acc, torch.float32), ("pos", pos, torch.int32)):
+        st = None
+        for name, x, dt in (("acc", acc, _f32), ("pos", pos, _i32)):
             if x is None:
                 continue
-            _need(x.dtype == dt and x.dim() == 3 and x.shape[0] == self.streams and x.shape[1] == self.heads and
-                  x.shape[2] >= self.slots and x.device == self.device and (x.stride(2) == 1 or x.shape[2] <= 1),
-                  f"{name}: {dt} [{self.streams}, {self.heads}, at least {self.slots}] on {self.device}, unit stride last")
-            ms, mh = x.stride(0), x.stride(1)
-        _need(acc is None or pos is None or acc.stride() == pos.stride(), "acc and pos differ in their strides")
-        return acc.data_ptr() if acc is not None else None, pos.data_ptr() if pos is not None else None, ms, mh
+            n = x.shape
+            if not (x.dtype is dt and len(n) == 3 and n[0] == self.streams and n[1] == self.heads and n[2] >= self.slots and
+                    x.get_device() == self._index and (x.stride(2) == 1 or n[2] <= 1)):
+                raise ValueError(f"{name}: {dt} [{self.streams}, {self.heads}, at least {self.slots}] on {self.device}, unit "
+                                 f"stride last; got {x.dtype} {list(n)} on {x.device}")
+            if st is not None and st != x.stride():
+                raise ValueError("acc and pos differ in their strides")
+            st = x.stride()
+        return (None if acc is None else acc.data_ptr(), None if pos is None else pos.data_ptr(),
+                *((0, 0) if st is None else st[:2]))
+
+    def _like(self, q, n):
+        """A contiguous float32 tensor of q's shape."""
+        return torch.empty_like(q) if q.is_contiguous() else q.new_empty(n)
+
+    def _given(self, x, shape, dtype):
+        if not (x.dtype is dtype and tuple(x.shape) == shape and x.is_contiguous() and x.get_device() == self._index):
+            raise ValueError(f"out: contiguous {dtype} {list(shape)} on {self.device}; got {x.dtype} {list(x.shape)} on {x.device}")
 
     def append(self, k, v, length, count=None, acc=None, pos=None, pos0=None, wait=False):
         """Writes the tokens k, v [streams, tokens, kv heads, dim] behind each stream's `length` slots, of stream s the
         first count[s] (all without count); bounds follow. acc and pos [streams, kv heads, slots]: set to 0 and
         pos0[s] + t (the slot's number without pos0). With wait, returns whether every token found a page."""
-        self._rows("k", k, self.heads)
-        self._rows("v", v, self.heads)
-        _need(k.shape == v.shape, "k and v differ in shape")
-        a, p, ms, mh = self._marks(acc, pos)
-        n = self._ints("length", length)
-        cn = self._ints("count", count) if count is not None else None
-        p0 = self._ints("pos0", pos0) if pos0 is not None else None
-        bad = _I(0)
-        ks, vs = k.stride(), v.stride()
-        self._run("append", _append, k.shape[1], k.data_ptr(), ks[1], ks[2], ks[0], v.data_ptr(), vs[1], vs[2], vs[0], n, cn, a, p,
-                       ms, mh, p0, int(wait), ctypes.addressof(bad))
+        n, ks = self._rows("k", k, self.heads)
+        m, vs = self._rows("v", v, self.heads)
+        if n != m:
+            raise ValueError(f"k {list(n)} and v {list(m)} differ in shape")
+        a, p, ms, mh = self._marks(acc, pos) if acc is not None or pos is not None else (None, None, 0, 0)
+        bad = _I(0) if wait else None
+        self._run("append", _append, n[1], k.data_ptr(), ks[1], ks[2], ks[0], v.data_ptr(), vs[1], vs[2], vs[0],
+                  self._ints("length", length), None if count is None else self._ints("count", count), a, p, ms, mh,
+                  None if pos0 is None else self._ints("pos0", pos0), 1 if wait else 0, ctypes.addressof(bad) if wait else None)
         return not bad.value if wait else None
 
     def attend(self, q, visible, step=1, scale=None, window=0, sel=None, acc=None, out=None, lse=False):
@@ -174,42 +196,37 @@ class PagedKV:
         (the last `window` of them, if given; those of the pages sel[s, t, g], if given). acc gains the weights each slot
         received. Returns out (float32, as q), and with lse=True also the logarithms of the softmax sums
         [streams, tokens, heads]."""
-        self._rows("q", q, None)
-        ns, nq, h, d = q.shape
+        n, qs = self._rows("q", q, None)
+        ns, nq, h, d = n
         see = self._ints("visible", visible)
-        a, _, ms, mh = self._marks(acc, None)
-        nsel = sp = None
+        a, _, ms, mh = self._marks(acc, None) if acc is not None else (None, None, 0, 0)
+        nsel = 0
+        sp = None
         if sel is not None:
-            _need(sel.dtype == torch.int32 and sel.dim() == 4 and sel.shape[:3] == (ns, nq, self.heads) and
-                  sel.is_contiguous() and sel.device == self.device,
-                  f"sel: contiguous int32 [{ns}, {nq}, {self.heads}, pages] on {self.device}")
+            if not (sel.dtype is _i32 and sel.dim() == 4 and sel.shape[:3] == (ns, nq, self.heads) and sel.is_contiguous() and
+                    sel.get_device() == self._index):
+                raise ValueError(f"sel: contiguous int32 [{ns}, {nq}, {self.heads}, pages] on {self.device}; got {sel.dtype} "
+                                 f"{list(sel.shape)} on {sel.device}")
             nsel, sp = sel.shape[3], sel.data_ptr() or see   # no pages at all: the list is there, and nothing is read
         if out is None:
-            out = torch.empty((ns, nq, h, d), device=self.device, dtype=torch.float32)
+            out = self._like(q, n)
         else:
-            _need(out.dtype == torch.float32 and out.shape == q.shape and out.is_contiguous() and out.device == self.device,
-                  "out: contiguous float32 of q's shape")
-        logs = torch.empty((ns, nq, h), device=self.device, dtype=torch.float32) if lse else None
-        qs = q.stride()
-        self._run("attend", _attend, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, window, sp, nsel or 0,
-                       d ** -0.5 if scale is None else scale, out.data_ptr(), logs.data_ptr() if lse else None, a, ms, mh,
-                  self._ws, 0)
+            self._given(out, tuple(n), _f32)
+        logs = q.new_empty((ns, nq, h)) if lse else None
+        self._run("attend", _attend, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, window, sp, nsel,
+                  d ** -0.5 if scale is None else scale, out.data_ptr(), logs.data_ptr() if lse else None, a, ms, mh, self._ws, 0)
         return (out, logs) if lse else out
 
     def select(self, q, visible, pages, step=1, first=1, last=1, out=None):
         """The `pages` pages that each token and kv head attends to: the first and the last ones it sees, then those whose
         bounds allow the largest q·k. int32 [streams, tokens, kv heads, pages], ascending, -1 behind."""
-        self._rows("q", q, None)
-        ns, nq, h, _ = q.shape
-        see = self._ints("visible", visible)
+        n, qs = self._rows("q", q, None)
         if out is None:
-            out = torch.empty((ns, nq, self.heads, pages), device=self.device, dtype=torch.int32)
+            out = q.new_empty((n[0], n[1], self.heads, pages), dtype=_i32)
         else:
-            _need(out.dtype == torch.int32 and tuple(out.shape) == (ns, nq, self.heads, pages) and out.is_contiguous() and
-                  out.device == self.device, "out: contiguous int32 [streams, tokens, kv heads, pages]")
-        qs = q.stride()
-        self._run("select", _select, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, first, last, pages, out.data_ptr(),
-                  self._ws, 0)
+            self._given(out, (n[0], n[1], self.heads, pages), _i32)
+        self._run("select", _select, n[2], n[1], q.data_ptr(), qs[1], qs[2], qs[0], self._ints("visible", visible), step, first,
+                  last, pages, out.data_ptr(), self._ws, 0)
         return out
 
     def evict(self, length, keep, acc, pos=None, first=0, recent=0, out=None):

@@ -309,7 +309,9 @@ def test_streams_that_share_pages(kv):
 # ------------------------------------------------------------------------------------------------ selection
 @pytest.mark.parametrize("lens,page,heads,group,D,nq,m,first,last", [
     ([400, 17, 0, 1], 16, 2, 4, 128, 1, 8, 1, 1), ([1000, 999], 8, 1, 1, 64, 3, 20, 2, 3), ([300], 5, 2, 7, 80, 2, 1, 0, 0),
-    ([3000], 4, 1, 2, 256, 1, 100, 0, 1), ([90], 16, 3, 8, 8, 1, 3, 5, 5), ([64 * 130], 64, 1, 4, 128, 1, 64, 1, 1)])
+    ([3000], 4, 1, 2, 256, 1, 100, 0, 1), ([90], 16, 3, 8, 8, 1, 3, 5, 5), ([64 * 130], 64, 1, 4, 128, 1, 64, 1, 1),
+    ([200], 8, 1, 72, 64, 2, 5, 1, 1), ([333, 20], 16, 1, 16, 256, 2, 7, 1, 1), ([500], 16, 2, 4, 128, 7, 9, 1, 1),
+    ([700, 701], 16, 1, 12, 128, 5, 4, 0, 0), ([9000], 8, 1, 4, 128, 1, 600, 1, 1)])
 def test_select(kv, lens, page, heads, group, D, nq, m, first, last):
     rng = np.random.default_rng(D + page)
     host, K, V, table, bounds = make(rng, [n + nq - 1 if n else 0 for n in lens], page, heads, D)
@@ -350,6 +352,27 @@ def test_select_near_ties_follow_the_exact_order(kv):
     got = kv.PagedKV(K, K, table, bounds=torch.from_numpy(bounds).cuda()).select(torch.from_numpy(q).cuda(), ints([n]), 10, first=0,
                                                                                 last=0)
     assert np.array_equal(got.cpu().numpy(), kv_ref.select(host, q, [n], 10, first=0, last=0))
+
+
+@pytest.mark.parametrize("n,m", [(3000, 700), (600, 30)])
+def test_select_many_equal_pages(kv, n, m):
+    """Hundreds of pages with the same bounds, some infinite or missing: the lowest places of the equal ones."""
+    rng = np.random.default_rng(22)
+    K = torch.zeros(n, 2, 1, 64, dtype=torch.float16, device="cuda")
+    kinds = rng.standard_normal((3, 2, 2, 64)).astype(np.float16)
+    kinds.sort(axis=2)
+    bounds = kinds[rng.integers(0, 3, n)]
+    table = np.arange(n, dtype=np.int32)[None].copy()
+    q = rng.standard_normal((1, 1, 4, 64)).astype(np.float32)
+    for step in range(3):
+        if step == 1:
+            table[0, ::17] = -1
+        if step == 2:
+            bounds[5::31, :, 1, 3] = np.inf
+            bounds[6::31, :, :, 3] = np.nan
+        host = {"K": K.cpu().numpy(), "V": K.cpu().numpy(), "bounds": bounds, "table": table}
+        got = kv.PagedKV(K, K, ints(table), bounds=torch.from_numpy(bounds).cuda()).select(torch.from_numpy(q).cuda(), ints([n]), m)
+        assert np.array_equal(got.cpu().numpy(), kv_ref.select(host, q, [n], m)), step
 
 
 # ------------------------------------------------------------------------------------------------ eviction
