@@ -192,11 +192,6 @@ namespace {
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void cp16(unsigned dst, const void *src, int bytes) {   // bytes 16, or 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void pdl_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------------------------- cache writes
@@ -329,6 +324,7 @@ struct SelectArgs {
     float *peak;                // [(s, g)][CTA][warp]: largest |bound| seen; infinity where a score is not finite
     unsigned long long *key;    // [row][mp]: 64-bit keys of pages decided by hand, where they are many
     int *sel;
+    unsigned *err;              // the device's error word
 };
 
 __device__ __forceinline__ int pages_seen(const SelectArgs &a, int s, int t) {
@@ -336,14 +332,23 @@ __device__ __forceinline__ int pages_seen(const SelectArgs &a, int s, int t) {
     return n / a.c.page + (n % a.c.page != 0);
 }
 
+__device__ __forceinline__ void bulk_row(void *dst, const void *src, unsigned bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                     sm100::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar))
+                 : "memory");
+}
+constexpr uint64_t SWAIT_NS = 2000000000ull;   // a row that has not landed after 2 s is an error
 constexpr int SW = 4, SPAGES = 16, SNST = 3;   // warps of a CTA, pages of a step, stages of a warp's ring
 template <int DP>
 struct ScoreCfg {
-    static constexpr int STAGE = SPAGES * DP * 2 * 2;               // lower and upper rows of 16 pages
+    static constexpr int PITCH = DP * 2 * 2 + 16;                   // a page's lower and upper row; 16 bytes more spread the banks
+    static constexpr int STAGE = SPAGES * PITCH;
     static constexpr int RING = SW * SNST * STAGE;
     static constexpr int QF = 2 * (DP / 16) * 32 * 16;              // fragments of one row tile: q < 0 and q > 0
     static constexpr int TG = DP == 256 ? 1 : DP == 128 ? 4 : 8;    // row tiles a CTA holds at most
-    static constexpr int smem(int tg) { return RING + tg * (QF + 8 * 4); }
+    static constexpr int BARS = SW * SNST * 8;
+    static constexpr int smem(int tg) { return RING + BARS + tg * (QF + 8 * 4); }
 };
 
 // Score of (page, query head): Σ_d max(q_d·lo_d, q_d·hi_d) = Σ min(q, 0)·lo + Σ max(q, 0)·hi, a product of the bounds (A, 16
@@ -355,44 +360,57 @@ struct ScoreCfg {
 template <int DP>
 __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ SelectArgs a) {
     using C = ScoreCfg<DP>;
-    constexpr int KT = DP / 16, PITCH = DP * 2, CH = DP / 8;
+    constexpr int KT = DP / 16, PITCH = C::PITCH;
     extern __shared__ __align__(128) uint8_t ss[];
-    uint4 *qf = reinterpret_cast<uint4 *>(ss + C::RING);                       // [tile][half][kt][lane]
-    float *qinv = reinterpret_cast<float *>(ss + C::RING + a.tg * C::QF);      // [tile][8]
-    pdl_next();
-    pdl_wait();
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ss + C::RING);
+    uint4 *qf = reinterpret_cast<uint4 *>(ss + C::RING + C::BARS);                       // [tile][half][kt][lane]
+    float *qinv = reinterpret_cast<float *>(ss + C::RING + C::BARS + a.tg * C::QF);      // [tile][8]
+    __shared__ int quit;
     const KvDev &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
+    uint8_t *wring = ss + warp * SNST * C::STAGE;
+    uint64_t *bar = bars + warp * SNST;
+    if (lane < SNST) sm100::mbar_init(bar + lane, 1);
+    sm100::fence_barrier_init();
+    if (tid == 0) quit = 0;
+    // what lies behind a row shorter than the tiles is multiplied by zeros: it has to be finite
+    for (int i = lane; i < SNST * SPAGES; i += 32)
+        for (int e = c.D * 4; e < PITCH; e += 16) *reinterpret_cast<uint4 *>(wring + i * PITCH + e) = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+    pdl_next();
+    pdl_wait();
     const int sg = blockIdx.y, s = sg / c.HKV, g = sg - s * c.HKV;
     const int z0 = blockIdx.z * a.zt, z1 = min(z0 + a.zt, a.tiles);
     const int have = pages_seen(a, s, (z1 - 1) / a.hg);
     const int step0 = blockIdx.x * SW * a.steps, all = (have + SPAGES - 1) / SPAGES;
     if (step0 >= all) return;
-    const int my = min(a.steps, max(0, (all - step0 - warp + SW - 1) / SW));
-    uint8_t *wring = ss + warp * SNST * C::STAGE;
+    const int my = min(a.steps, max(0, (all - step0 - warp + SW - 1) / SW)), kts = (c.D + 15) / 16;
     const unsigned wbase = sm100::smem_u32(wring);
+    unsigned copied = 0;   // copies of this warp so far: copy n goes to stage n % SNST, in the barrier's phase n / SNST
     auto id_of = [&](int i) {
         const int p = (step0 + warp + SW * i) * SPAGES + (lane & 15);
         return i < my && p < have ? page_id(c.table, c.ts, s, p, c.mp, c.n_pages) : -1;
     };
+    // one bulk copy per page, both rows (lane l < 16: page l); a page that is missing keeps what its place held before
     auto copy = [&](int i, int id) {
-        if (i < my) {
-            const unsigned at = wbase + (i % SNST) * C::STAGE;
-#pragma unroll
-            for (int j = 0; j < SPAGES * 2 * CH / 32; j++) {
-                const int e = j * 32 + lane, pg = e / (2 * CH), half = e / CH & 1, ch = e % CH;
-                const int pid = __shfl_sync(kAll, id, pg);
-                const int bytes = pid >= 0 && ch * 8 < c.D ? 16 : 0;
-                const __half *src = c.bounds + (((long long)max(pid, 0) * c.HKV + g) * 2 + half) * c.D + ch * 8;
-                cp16(at + half * SPAGES * PITCH + pg * PITCH + ((ch ^ (pg & 7)) << 4), bytes ? src : c.bounds, bytes);
-            }
-        }
-        cp_commit();
+        if (i >= my) return;
+        const int st = copied % SNST;
+        const unsigned here = __ballot_sync(kAll, lane < SPAGES && id >= 0);
+        if (lane == 0) sm100::mbar_arrive_expect_tx(bar + st, __popc(here) * c.D * 4);
+        __syncwarp();
+        if (here >> lane & 1u)
+            bulk_row(wring + st * C::STAGE + lane * PITCH, c.bounds + ((long long)id * c.HKV + g) * 2 * c.D, c.D * 4, bar + st);
+        copied++;
     };
     const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = lane >> 4;
     __half2 peak = __half2half2(__ushort_as_half(0));
-    bool wild = false;
-    for (int tile0 = z0; tile0 < z1; tile0 += a.tg) {
+    bool wild = false, ok = true;
+    unsigned used = 0;   // copies of this warp that it has waited for
+    auto wait = [&]() {
+        ok = ok && sm100::mbar_wait(bar + used % SNST, used / SNST & 1, &quit, SWAIT_NS);
+        used++;
+    };
+    for (int tile0 = z0; tile0 < z1 && ok; tile0 += a.tg) {
         const int ntile = min(a.tg, z1 - tile0);
         if (tile0 > z0) __syncthreads();   // every warp has left the last tiles' fragments
         int ids[SNST - 1];
@@ -445,27 +463,34 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
         }
         __syncthreads();
         for (int i = 0; i < my; i++) {
-            cp_wait<SNST - 2>();
-            __syncwarp();
-            copy(i + SNST - 1, next);
-            const unsigned lo = wbase + (i % SNST) * C::STAGE, hi = lo + SPAGES * PITCH;
+            const unsigned lo = wbase + used % SNST * C::STAGE, hi = lo + c.D * 2;
+            wait();
+            if (!__all_sync(kAll, ok)) {
+                ok = false;
+                break;
+            }
+            copy(i + SNST - 1, next);   // into the stage before this one, which every lane has left
             const int p = (step0 + warp + SW * i) * SPAGES + gq;
             const bool in0 = __shfl_sync(kAll, now, gq) >= 0, in1 = __shfl_sync(kAll, now, gq + 8) >= 0;
             float top[2] = {-INFINITY, -INFINITY};
+            __half2 pk0 = __half2half2(__ushort_as_half(0)), pk1 = pk0;
             for (int tile = 0; tile < ntile; tile++) {
                 float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
                 const uint4 *q0 = qf + tile * 2 * KT * 32 + lane, *q1 = q0 + KT * 32;
 #pragma unroll
                 for (int kt = 0; kt < KT; kt++) {
-                    const unsigned off = arow * PITCH + (((2 * kt + acol) ^ (arow & 7)) << 4);
+                    if (kt >= kts) break;
+                    const unsigned off = arow * PITCH + kt * 32 + acol * 16;
                     unsigned l4[4], u4[4];
                     at_ldsm(lo + off, l4);
                     at_ldsm(hi + off, u4);
-                    if (tile == 0) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) peak = __hmax2(peak, __hmax2(__habs2(as_h2(l4[e])), __habs2(as_h2(u4[e]))));
+                    if (tile == 0) {   // registers 0 and 2: page gq, 1 and 3: page gq + 8
+                        pk0 = __hmax2(__hmax2(pk0, __hmax2(__habs2(as_h2(l4[0])), __habs2(as_h2(l4[2])))),
+                                      __hmax2(__habs2(as_h2(u4[0])), __habs2(as_h2(u4[2]))));
+                        pk1 = __hmax2(__hmax2(pk1, __hmax2(__habs2(as_h2(l4[1])), __habs2(as_h2(l4[3])))),
+                                      __hmax2(__habs2(as_h2(u4[1])), __habs2(as_h2(u4[3]))));
                     }
-                    const uint4 f = q0[kt * 32], h = q1[kt * 32];
+                const uint4 f = q0[kt * 32], h = q1[kt * 32];
                     at_mma(sc[0], l4, f.x, f.y);
                     at_mma(sc[1], u4, h.x, h.y);
                     at_mma(sc[0], l4, f.z, f.w);
@@ -495,11 +520,21 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
                 }
                 top[0] = top[1] = -INFINITY;
             }
+            if (in0) peak = __hmax2(peak, pk0);
+            if (in1) peak = __hmax2(peak, pk1);
             now = after;
             after = next;
             next = id_of(i + SNST);
+            __syncwarp();   // every lane has read this stage
         }
-        cp_wait<0>();
+    }
+    if (!ok) {   // a copy that has not landed: what is in flight is waited for, again with a limit
+        ok = true;
+        while (used < copied) wait();
+        if (lane == 0) {
+            quit = 1;
+            *(volatile unsigned *)a.err = kDevErrWaitTimeout;
+        }
     }
     float pk = fmaxf(__low2float(peak), __high2float(peak));
     for (int i = 16; i > 0; i >>= 1) pk = fmaxf(pk, __shfl_xor_sync(kAll, pk, i));
@@ -529,7 +564,135 @@ __device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   /
     return x + (w ? before : 0);
 }
 
-// Adds one to hist[bin] for the lanes with in: lanes of a warp with the same bin together (keys crowd in few bins).
+constexpr int NLIST = 64;
+struct NthKey {   // shared memory of nth_key
+    int counts[2][3][32];
+    uint32_t list[NLIST];
+    int n;
+};
+// The m-th largest of n 32-bit keys (n >= m >= 1) of a CTA, and how many are larger. Two bits a round from the top: the counts
+// of keys at least as large as each of three candidates, added up in the warps and through shared memory, one barrier a
+// round, until at most NLIST keys share the bits found; those are ranked directly. Thread t holds the keys t, t + NT, ... in
+// reg (0 past the end); keys beyond R·NT come from `more` in every round. (Radix selection with shared-memory histograms took
+// 3 to 4 µs a digit here, for the crowding of keys in few bins, its scans and four barriers each.)
+template <int NT, int R, typename More>
+__device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int m, NthKey &sh, More more, int *larger) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint32_t v = 0;
+    int above = 0, in = n, shift = 32;   // keys above the range [v, v + 2^shift), keys in it
+    if (threadIdx.x == 0) sh.n = 0;
+    for (int round = 0; round < 16 && in > NLIST; round++) {
+        shift -= 2;
+        int c1 = 0, c2 = 0, c3 = 0;
+        const uint32_t a1 = v | 1u << shift, a2 = v | 2u << shift, a3 = v | 3u << shift;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            c1 += reg[i] >= a1;
+            c2 += reg[i] >= a2;
+            c3 += reg[i] >= a3;
+        }
+        for (int i = R * NT + threadIdx.x; i < n; i += NT) {
+            const uint32_t k = more(i);
+            c1 += k >= a1;
+            c2 += k >= a2;
+            c3 += k >= a3;
+        }
+        c1 = __reduce_add_sync(kAll, c1);
+        c2 = __reduce_add_sync(kAll, c2);
+        c3 = __reduce_add_sync(kAll, c3);
+        int (&buf)[3][32] = sh.counts[round & 1];
+        if (lane == 0) {
+            buf[0][w] = c1;
+            buf[1][w] = c2;
+            buf[2][w] = c3;
+        }
+        __syncthreads();
+        c1 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[0][lane] : 0);
+        c2 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[1][lane] : 0);
+        c3 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[2][lane] : 0);
+        if (c3 >= m) {
+            v = a3;
+            in = c3 - above;
+        } else if (c2 >= m) {
+            v = a2;
+            in = c2 - c3;
+            above = c3;
+        } else if (c1 >= m) {
+            v = a1;
+            in = c1 - c2;
+            above = c2;
+        } else {
+            in = in + above - c1;
+            above = c1;
+        }
+    }
+    *larger = above;
+    if (in > NLIST || shift == 0) return v;   // equal keys to the last bit
+    __syncthreads();   // sh.n is set
+    auto put = [&](uint32_t k) {
+        if (shift == 32 || k >> shift == v >> shift) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < NLIST) sh.list[at] = k;   // never more
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < R; i++)
+        if ((int)threadIdx.x + i * NT < n) put(reg[i]);
+    for (int i = R * NT + threadIdx.x; i < n; i += NT) put(more(i));
+    __syncthreads();
+    // lane: the keys lane and lane + 32 of the list
+    const uint32_t k0 = lane < in ? sh.list[lane] : 0u, k1 = lane + 32 < in ? sh.list[lane + 32] : 0u;
+    int g0 = 0, g1 = 0, e0 = 0, e1 = 0;   // keys larger than each, and as large
+    for (int i = 0; i < in; i++) {
+        const uint32_t k = sh.list[i];
+        g0 += k > k0;
+        g1 += k > k1;
+        e0 += k >= k0;
+        e1 += k >= k1;
+    }
+    const int r = m - above;   // the r-th of the list: fewer than r are larger, at least r as large
+    const unsigned hit0 = __ballot_sync(kAll, lane < in && g0 < r && e0 >= r), hit1 = __ballot_sync(kAll, lane + 32 < in && g1 < r && e1 >= r);
+    const int l = __ffs(hit0 ? hit0 : hit1) - 1;
+    const uint32_t x0 = __shfl_sync(kAll, k0, l), x1 = __shfl_sync(kAll, k1, l);
+    const int y0 = __shfl_sync(kAll, g0, l), y1 = __shfl_sync(kAll, g1, l);
+    *larger = above + (hit0 ? y0 : y1);
+    return hit0 ? x0 : x1;
+}
+
+// Places of the hits of a CTA's items in order of their index (item i·NT + thread): sum of the earlier counts of the (round,
+// warp) pairs. cnt holds the counts of R·NT / 32 pairs; on return the exclusive sums, and the total.
+template <int NT, int R>
+__device__ __forceinline__ int scan_counts(int *cnt, int *total) {
+    __syncthreads();   // the counts are written
+    constexpr int N = R * NT / 32, PER = (N + 31) / 32;
+    if (threadIdx.x < 32) {
+        int v[PER], sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = threadIdx.x * PER + j;
+            v[j] = i < N ? cnt[i] : 0;
+            sum += v[j];
+        }
+        int x = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(kAll, x, o);
+            if ((int)threadIdx.x >= o) x += y;
+        }
+        if (threadIdx.x == 31) *total = x;
+        x -= sum;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = threadIdx.x * PER + j;
+            if (i < N) cnt[i] = x;
+            x += v[j];
+        }
+    }
+    __syncthreads();
+    return *total;
+}
+
+// Adds one to hist[bin] for the lanes with in: lanes of a warp with the same bin together.
 __device__ __forceinline__ void hist_add(int *hist, int bin, bool in) {
     const unsigned live = __ballot_sync(kAll, in);
     if (!in) return;
@@ -551,8 +714,8 @@ __device__ __forceinline__ void pick_bin(const int *hist, int need, int *scan, i
     __syncthreads();
 }
 
-// A page's score in 64 bits, by one warp: the key of the largest over the heads.
-__device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int s, int t, int g, int place) {
+// A page's score in 64 bits, by one warp: the key of the largest over the heads h0 .. h1 - 1 (0: NaN, or no page).
+__device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int s, int t, int g, int place, int h0, int h1) {
     const KvDev &c = a.c;
     const int lane = threadIdx.x & 31;
     const int id = page_id(c.table, c.ts, s, place, c.mp, c.n_pages);
@@ -560,9 +723,10 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int
     const __half *lo = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D, *hi = lo + c.D;
     double best = -INFINITY;
     bool nan = false;
-    for (int h = 0; h < a.G; h++) {
+    for (int h = h0; h < h1; h++) {
         const float *q = a.Q + s * a.qs + t * a.qt + (long long)(g * a.G + h) * a.qh;
         double x = 0.0;
+#pragma unroll 4
         for (int d = lane; d < c.D; d += 32) {
             const float v = q[d];
             x = fma((double)v, (double)__half2float(v >= 0.0f ? hi[d] : lo[d]), x);
@@ -574,16 +738,18 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int
     return nan ? 0ull : score_key(best);
 }
 
-constexpr int CT = 512, CLIST = 512;
-// One CTA per row (s, t, g). Keys are the FP32 scores' order-preserving bits (pages that are always taken above all); the
-// nsel-th largest, tau, by radix selection over digits of 10, 11 and 11 bits. With E the bound of a score's error, a page above
-// tau + 2E is taken, one below tau - 2E is not: nsel pages have scores of at least tau - E, and fewer than nsel more than tau + E.
-// The pages between are ranked by their 64-bit scores.
+constexpr int CT = 256, CR = 16, CLIST = 512;   // threads, scores a thread holds, pages decided by hand in shared memory
+// One CTA per row (s, t, g). Keys are the FP32 scores' order-preserving bits (pages that are always taken above all); tau is
+// the nsel-th largest. With E the bound of a score's error, a page above tau + 2E is taken, one below tau - 2E is not: nsel pages
+// have scores of at least tau - E, and fewer than nsel more than tau + E. The pages between are ranked by their 64-bit scores.
 __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ SelectArgs a, int score_ctas) {
-    __shared__ int hist[2 * CT], hist2[2 * CT], scan[32], got[3];
-    __shared__ float red[CT / 32];
+    __shared__ NthKey nth;
+    __shared__ int hist[2 * CT], scan[32], got[3];
+    __shared__ int order[CR * CT / 32], order_n;
+    __shared__ float red[2][CT / 32];
     __shared__ int list[CLIST];
     __shared__ unsigned long long lkey[CLIST];
+    __shared__ unsigned char lnan[CLIST];
     __shared__ int sure, nlist;
     pdl_next();
     pdl_wait();
@@ -599,14 +765,17 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     }
     float *score = a.score + (long long)row * c.mp;
     auto always = [&](int p) { return p < a.first || p >= have - a.last; };
-    auto key_of = [&](int p) { return always(p) ? kAll : weight_key(__ldcg(score + p)); };
+    auto key_of = [&](int p, float x) { return always(p) ? kAll : weight_key(x); };
+    float x[CR];
+#pragma unroll
+    for (int i = 0; i < CR; i++) x[i] = tid + i * CT < have ? __ldcg(score + tid + i * CT) : 0.0f;
     // ---- E = 2^-14 · max |q|_1 · max |bound| (2^-13 for D > 128): each of the 4·D/16 tensor-core steps adds 17 numbers, each cut
     // off at worst 2^-23 below the largest, which is at most |q|_1·|bound|, 2^-18.9 in all; 32 steps at D = 128 make 2^-13.9
     // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21
     float big = 0.0f, l1 = 0.0f;
     {
         const int sg = s * c.HKV + g, z = t * a.hg / a.zt;
-        const int used = ((pages_seen(a, s, t) + SPAGES - 1) / SPAGES + SW * a.steps - 1) / (SW * a.steps);   // CTAs with pages
+        const int used = ((have + SPAGES - 1) / SPAGES + SW * a.steps - 1) / (SW * a.steps);   // CTAs with pages
         for (int i = tid; i < used * SW; i += CT)
             big = fmaxf(big, __ldcg(a.peak + ((long long)z * c.ns * c.HKV + sg) * score_ctas * SW + i));
         for (int h = tid; h < a.G; h += CT) l1 = fmaxf(l1, __ldcg(a.l1 + (long long)st * a.H + g * a.G + h));
@@ -615,67 +784,66 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
             l1 = fmaxf(l1, __shfl_xor_sync(kAll, l1, o));
         }
         if (tid == 0) nlist = sure = 0;
-        // l1 lives in the first warps only when G is small: both maxima go through shared memory
         if (lane == 0) {
-            red[warp] = big;
-            scan[warp] = __float_as_int(l1);
+            red[0][warp] = big;
+            red[1][warp] = l1;
         }
-        for (int i = tid; i < 2 * CT; i += CT) hist[i] = hist2[i] = 0;
-        __syncthreads();
-        for (int w = 0; w < CT / 32; w++) {
-            big = fmaxf(big, red[w]);
-            l1 = fmaxf(l1, __int_as_float(scan[w]));
-        }
-        __syncthreads();
+    }
+    // ---- tau
+    uint32_t key[CR];
+#pragma unroll
+    for (int i = 0; i < CR; i++) key[i] = tid + i * CT < have ? key_of(tid + i * CT, x[i]) : 0u;
+    int larger;
+    const uint32_t at = nth_key<CT, CR>(key, have, m, nth, [&](int i) { return key_of(i, __ldcg(score + i)); }, &larger);
+    for (int w = 0; w < CT / 32; w++) {
+        big = fmaxf(big, red[0][w]);
+        l1 = fmaxf(l1, red[1][w]);
     }
     const float E = (c.D > 128 ? 0x1p-13f : 0x1p-14f) * l1 * big;
-    // ---- tau: the m-th largest key
-    unsigned prefix = 0, mask = 0;
-    int need = m;
-    for (int d = 0; d < 4; d++) {
-        const int shift = d == 0 ? 22 : d == 1 ? 12 : d == 2 ? 2 : 0, bits = d == 3 ? 2 : 10;
-        int *hs = d & 1 ? hist2 : hist, *other = d & 1 ? hist : hist2;
-        for (int i = tid; i < (have + CT - 1) / CT * CT; i += CT) {
-            const unsigned k = i < have ? key_of(i) : 0u;
-            hist_add(hs, (k >> shift) & ((1u << bits) - 1), i < have && (k & mask) == prefix);
-        }
-        __syncthreads();
-        pick_bin(hs, need, scan, got);
-        need -= got[1];
-        prefix |= (unsigned)got[0] << shift;
-        mask |= ((1u << bits) - 1) << shift;
-        if (d < 3) {
-            for (int i = tid; i < 2 * CT; i += CT) other[i] = 0;
-            __syncthreads();   // got is read, the next histogram clear
-        }
-    }
-    const bool full = prefix == kAll;   // enough pages that are always taken: the lowest of them
-    const unsigned tb = prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix;
-    const float tau = __uint_as_float(tb);
-    const bool know = E < INFINITY && prefix != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
+    const bool full = at == kAll;   // enough pages that are always taken: the lowest of them
+    const float tau = __uint_as_float(at & 0x80000000u ? at & 0x7fffffffu : ~at);
+    const bool know = E < INFINITY && at != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
     const float above = know ? tau + 2.0f * E : 3.4e38f, below = know ? tau - 2.0f * E : -INFINITY;
+    // 1: taken for sure, 0: not, -1: between
+    auto side = [&](int i, float y) { return always(i) || (know && y > above) ? 1 : !know || y >= below ? -1 : 0; };
     if (!full) {
-        for (int i = tid; i < have; i += CT) {
-            if (always(i)) {
-                atomicAdd(&sure, 1);
-                continue;
+        int mine = 0;
+        auto look = [&](int i, float y) {
+            const int w = side(i, y);
+            mine += w > 0;
+            if (w < 0) {
+                const int slot = atomicAdd(&nlist, 1);
+                if (slot < CLIST) list[slot] = i;
             }
-            const float x = __ldcg(score + i);
-            if (know && x > above) atomicAdd(&sure, 1);
-            else if (!know || x >= below) {
-                const int at = atomicAdd(&nlist, 1);
-                if (at < CLIST) list[at] = i;
-            }
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < CR; i++)
+            if (tid + i * CT < have) look(tid + i * CT, x[i]);
+        for (int i = CR * CT + tid; i < have; i += CT) look(i, __ldcg(score + i));
+        mine = __reduce_add_sync(kAll, mine);
+        if (lane == 0) atomicAdd(&sure, mine);
         __syncthreads();
         const int r = m - sure, nb = nlist;   // r >= 1 of the nb pages between are taken
         if (nb <= CLIST) {
-            if (nb > r)
-                for (int i = warp; i < nb; i += CT / 32) {
-                    const unsigned long long k = exact_key(a, s, t, g, list[i]);
-                    if (lane == 0) lkey[i] = k;
+            if (nb > r) {   // a warp per (page, query head)
+                for (int i = tid; i < nb; i += CT) {
+                    lkey[i] = 0ull;
+                    lnan[i] = 0;
                 }
-            __syncthreads();
+                __syncthreads();
+                for (int i = warp; i < nb * a.G; i += CT / 32) {
+                    const int e = i / a.G;
+                    const unsigned long long k = exact_key(a, s, t, g, list[e], i - e * a.G, i - e * a.G + 1);
+                    if (lane == 0) {
+                        if (k) atomicMax(&lkey[e], k);
+                        else lnan[e] = 1;
+                    }
+                }
+                __syncthreads();
+                for (int i = tid; i < nb; i += CT)
+                    if (lnan[i]) lkey[i] = 0ull;
+                __syncthreads();
+            }
             for (int i = tid; i < nb; i += CT) {
                 int better = 0;
                 if (nb > r)
@@ -684,23 +852,22 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
                 score[list[i]] = better < r ? INFINITY : -INFINITY;
             }
         } else {   // very many: 64-bit keys of all of them, and radix selection over these
-            unsigned long long *key = a.key + (long long)row * c.mp;
+            unsigned long long *wide = a.key + (long long)row * c.mp;
             for (int i = warp; i < have; i += CT / 32) {
-                const float x = __ldcg(score + i);
-                const bool in = !always(i) && !(know && x > above) && (!know || x >= below);
-                const unsigned long long k = in ? exact_key(a, s, t, g, i) : 0ull;
+                const bool in = side(i, __ldcg(score + i)) < 0;
+                const unsigned long long k = in ? exact_key(a, s, t, g, i, 0, a.G) : 0ull;
                 // a page of the list has a key of at least 1, so that 0 marks the others; NaN and missing pages get 1
-                if (lane == 0) key[i] = in ? max(k, 1ull) : 0ull;
+                if (lane == 0) wide[i] = in ? max(k, 1ull) : 0ull;
             }
             __syncthreads();
             unsigned long long pre = 0, msk = 0;
             int left = r;
-            for (int shift = 54; shift >= -6; shift -= 10) {
-                const int sh = max(shift, 0), bits = shift < 0 ? 4 : 10;
+            for (int shift = 55; shift >= -8; shift -= 9) {   // 2·CT bins
+                const int sh = max(shift, 0), bits = shift < 0 ? 1 : 9;
                 for (int i = tid; i < 2 * CT; i += CT) hist[i] = 0;
                 __syncthreads();
                 for (int i = tid; i < (have + CT - 1) / CT * CT; i += CT) {
-                    const unsigned long long k = i < have ? key[i] : 0ull;
+                    const unsigned long long k = i < have ? wide[i] : 0ull;
                     hist_add(hist, (int)(k >> sh) & ((1 << bits) - 1), k != 0ull && (k & msk) == pre);
                 }
                 __syncthreads();
@@ -713,7 +880,7 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
             int eq0 = 0;
             for (int i0 = 0; i0 < have; i0 += CT) {   // ties: the lowest places
                 const int i = i0 + tid;
-                const unsigned long long k = i < have ? key[i] : 0ull;
+                const unsigned long long k = i < have ? wide[i] : 0ull;
                 int total;
                 const int rank = block_scan_incl(k != 0ull && k == pre, scan, &total) + eq0;
                 if (k != 0ull) score[i] = k > pre || (k == pre && rank <= left) ? INFINITY : -INFINITY;
@@ -722,14 +889,25 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
         }
         __syncthreads();   // the decided scores are written
     }
+    // ---- the taken pages in order, CR·CT at a time
     int base = 0;
-    for (int i0 = 0; i0 < have && base < m; i0 += CT) {
-        const int i = i0 + tid;
-        const bool take = i < have && (always(i) || (!full && __ldcg(score + i) > above));
-        int total;
-        const int at = block_scan_incl(take, scan, &total) + base;
-        if (take && at <= m) out[at - 1] = i;
+    for (int i0 = 0; i0 < have && base < m; i0 += CR * CT) {
+        unsigned hit[CR];
+#pragma unroll
+        for (int i = 0; i < CR; i++) {
+            const int p = i0 + i * CT + tid;
+            const bool take = p < have && (always(p) || (!full && __ldcg(score + p) > above));
+            hit[i] = __ballot_sync(kAll, take);
+            if (lane == 0) order[i * (CT / 32) + warp] = __popc(hit[i]);
+        }
+        const int total = scan_counts<CT, CR>(order, &order_n);
+#pragma unroll
+        for (int i = 0; i < CR; i++) {
+            const int slot = base + order[i * (CT / 32) + warp] + __popc(hit[i] & ((1u << lane) - 1u));
+            if ((hit[i] >> lane & 1u) && slot < m) out[slot] = i0 + i * CT + tid;
+        }
         base += total;
+        __syncthreads();   // the sums are read before the next counts land on them
     }
 }
 
@@ -749,18 +927,20 @@ struct EvictArgs {
     int *len_out;
 };
 
-constexpr int ET = 1024, EIPT = 8;   // threads, slots a thread takes in a row in the ordered passes
-// Which slots stay, and where the movers go: one CTA per row (s, g). The threshold key (the keep-th largest) by radix
-// selection over digits of 11, 11 and 10 bits, warps adding equal digits together; then one ordered pass: below `keep` the
-// given-up slots are listed and their pages marked, from there on the j-th staying slot becomes the source of the j-th of
-// them. acc and pos come from L1 after the first pass.
+constexpr int ER = 16;   // slots a thread holds
+// Which slots stay, and where the movers go: one CTA per row (s, g). The threshold is the keep-th largest key; then one
+// ordered pass over the slots, ER·ET at a time: below `keep` the given-up slots are listed and their pages marked, from
+// there on the j-th staying slot becomes the source of the j-th of them. ET = 256 threads hold 4096 slots, 1024 threads 16384:
+// the smaller where the table has no more (256 rows of 2064 slots: 61 µs with 1024 threads, most of them idle).
+template <int ET>
 __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArgs a) {
-    __shared__ int hist[2 * ET], hist2[2 * ET];
-    __shared__ int scan[32], got[3], sh_new;
+    __shared__ NthKey nth;
+    __shared__ int order[ER * ET / 32], eqs[ER * ET / 32], order_n, eqs_n, sh_new;
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const int row = blockIdx.x, s = row / c.HKV, g = row - s * c.HKV, tid = threadIdx.x;
+    const int row = blockIdx.x, s = row / c.HKV, g = row - s * c.HKV;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = min(max(a.len[s], 0), c.cap), keep = a.keep;
     if (tid == 0) {
         a.used[2 * row] = n;
@@ -772,98 +952,102 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
     const int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
     int *src = a.src + (long long)row * keep, *holes = a.holes + (long long)row * keep, *flag = a.flag + (long long)row * a.pages;
     for (int i = tid; i < a.pages; i += ET) flag[i] = 0;
-    for (int i = tid; i < 2 * ET; i += ET) hist[i] = hist2[i] = 0;
-    __syncthreads();
+    uint32_t key[ER];   // the weight's key, then that with the sure ones on top
     int newest = n - 1;
     if (pos) {
-        int m = INT_MIN;
-        for (int k = tid; k < n; k += ET) m = max(m, __ldg(pos + k));
+        int p[ER], m = INT_MIN;
+#pragma unroll
+        for (int i = 0; i < ER; i++) p[i] = tid + i * ET < n ? __ldg(pos + tid + i * ET) : INT_MIN;
+#pragma unroll
+        for (int i = 0; i < ER; i++) key[i] = tid + i * ET < n ? weight_key(__ldg(acc + tid + i * ET)) : 0u;
+#pragma unroll
+        for (int i = 0; i < ER; i++) m = max(m, p[i]);
+        for (int k = ER * ET + tid; k < n; k += ET) m = max(m, __ldg(pos + k));
         m = __reduce_max_sync(kAll, m);
-        if ((tid & 31) == 0) atomicMax(&sh_new, m);
+        __syncthreads();   // sh_new is set
+        if (lane == 0) atomicMax(&sh_new, m);
         __syncthreads();
         newest = sh_new;
+#pragma unroll
+        for (int i = 0; i < ER; i++)
+            if (tid + i * ET < n && (p[i] < a.first || p[i] > (long long)newest - a.recent)) key[i] = kAll;
+    } else {
+#pragma unroll
+        for (int i = 0; i < ER; i++) {
+            const int k = tid + i * ET;
+            key[i] = k >= n ? 0u : k < a.first || k > (long long)newest - a.recent ? kAll : weight_key(__ldg(acc + k));
+        }
     }
     const long long old = (long long)newest - a.recent;
-    auto key_of = [&](int k) -> unsigned {
+    auto key_of = [&](int k) -> uint32_t {
         const int p = pos ? __ldg(pos + k) : k;
         return p < a.first || p > old ? kAll : weight_key(__ldg(acc + k));
     };
-    unsigned prefix = 0, mask = 0;
-    int need = keep;
-    bool whole = false;   // every key of the prefix stays: no further digit matters
-    for (int d = 0; d < 3 && !whole; d++) {
-        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-        int *hs = d & 1 ? hist2 : hist, *other = d & 1 ? hist : hist2;
-        for (int k0 = 0; k0 < n; k0 += ET) {
-            const int k = k0 + tid;
-            const unsigned x = k < n ? key_of(k) : 0u;
-            hist_add(hs, (x >> shift) & ((1u << bits) - 1), k < n && (x & mask) == prefix);
-        }
-        __syncthreads();
-        pick_bin(hs, need, scan, got);
-        need -= got[1];
-        prefix |= (unsigned)got[0] << shift;
-        mask |= ((1u << bits) - 1) << shift;
-        whole = got[2] == need;
-        if (d < 2)
-            for (int i = tid; i < 2 * ET; i += ET) other[i] = 0;
-        __syncthreads();   // got is read, the next histogram clear
-    }
-    // EIPT slots in a row per thread; with `whole` every key equal to the prefix stays and their order does not matter
+    int larger;
+    const uint32_t last = nth_key<ET, ER>(key, n, keep, nth, key_of, &larger);
+    const int need = keep - larger;   // of the keys equal to the threshold the first `need` stay
     int eq_base = 0, holes_n = 0, moved = 0;
-    for (int phase = 0; phase < 2; phase++) {
-        const int from = phase ? keep : 0, to = phase ? n : keep;
-        for (int k0 = from; k0 < to; k0 += ET * EIPT) {
-            const int k1 = k0 + tid * EIPT;
-            unsigned eq = 0, gt = 0;
+    for (int i0 = 0; i0 < n; i0 += ER * ET) {
+        unsigned eq[ER], hole[ER], mover[ER];   // ballots of the warps
 #pragma unroll
-            for (int j = 0; j < EIPT; j++) {
-                const unsigned x = k1 + j < to ? key_of(k1 + j) & mask : 0u;
-                if (k1 + j < to && x == prefix) eq |= 1u << j;
-                if (k1 + j < to && x > prefix) gt |= 1u << j;
-            }
-            unsigned stay = gt | eq;
-            if (!whole) {   // of the equal ones only the first `need`
-                int total;
-                int before = block_scan_incl(__popc(eq), scan, &total) - __popc(eq) + eq_base;
-                eq_base += total;
-                stay = gt;
-                for (unsigned e = eq; e && before < need; e &= e - 1, before++) stay |= e & -e;
-            }
-            const unsigned in = k1 < to ? (to - k1 >= EIPT ? (1u << EIPT) - 1 : (1u << (to - k1)) - 1) : 0u;
-            const unsigned hit = phase ? stay & in : ~stay & in;
-            int total;
-            int at = block_scan_incl(__popc(hit), scan, &total) - __popc(hit);
-            if (phase == 0) {
-                at += holes_n;
-                holes_n += total;
+        for (int i = 0; i < ER; i++) {
+            const int k = i0 + i * ET + tid;
+            if (i0 > 0) key[i] = k < n ? key_of(k) : 0u;
+            eq[i] = __ballot_sync(kAll, k < n && key[i] == last);
+            if (lane == 0) eqs[i * (ET / 32) + warp] = __popc(eq[i]);
+        }
+        const int eq_total = scan_counts<ET, ER>(eqs, &eqs_n);
 #pragma unroll
-                for (int j = 0; j < EIPT; j++) {
-                    if (!(in >> j & 1)) continue;
-                    src[k1 + j] = -1;
-                    if (hit >> j & 1) {
-                        holes[at++] = k1 + j;
-                        flag[page_quot(c.div, k1 + j)] = 1;
-                    }
-                }
-            } else {
-                at += moved;
-                moved += total;
-                for (unsigned e = hit; e; e &= e - 1, at++)
-                    if (at < holes_n) src[holes[at]] = k1 + __ffs(e) - 1;
+        for (int i = 0; i < ER; i++) {
+            const int k = i0 + i * ET + tid;
+            const int rank = eq_base + eqs[i * (ET / 32) + warp] + __popc(eq[i] & ((1u << lane) - 1u));
+            const bool stay = k < n && (key[i] > last || (key[i] == last && rank < need));
+            hole[i] = __ballot_sync(kAll, k < keep && !stay);
+            mover[i] = __ballot_sync(kAll, k >= keep && stay);
+            // holes lie below keep, movers behind: their counts share a word (at most 2^14 of each at once)
+            if (lane == 0) order[i * (ET / 32) + warp] = __popc(hole[i]) | __popc(mover[i]) << 16;
+            if (k < keep) src[k] = -1;
+        }
+        const int total = scan_counts<ET, ER>(order, &order_n);
+#pragma unroll
+        for (int i = 0; i < ER; i++) {
+            const int k = i0 + i * ET + tid, before = order[i * (ET / 32) + warp];
+            if (hole[i] >> lane & 1u) {
+                holes[holes_n + (before & 0xffff) + __popc(hole[i] & ((1u << lane) - 1u))] = k;
+                flag[page_quot(c.div, k)] = 1;
             }
         }
-        __syncthreads();   // the list of holes is written
+        __syncthreads();   // the holes so far are listed: the movers of these slots fill the first of them
+#pragma unroll
+        for (int i = 0; i < ER; i++) {
+            const int k = i0 + i * ET + tid, before = order[i * (ET / 32) + warp];
+            if (mover[i] >> lane & 1u) {
+                const int at = moved + (before >> 16) + __popc(mover[i] & ((1u << lane) - 1u));
+                if (at < keep) src[holes[at]] = k;
+            }
+        }
+        eq_base += eq_total;
+        holes_n += total & 0xffff;
+        moved += total >> 16;
+        __syncthreads();   // the sums are read before the next counts land on them
     }
     // the pages that change: those with holes, and the one that held slots on both sides of keep
     int base = 0;
-    for (int i0 = 0; i0 < a.pages; i0 += ET) {
-        const int i = i0 + tid;
-        const bool hit = i < a.pages && (flag[i] || (i == a.pages - 1 && keep % c.page));
-        int total;
-        const int at = block_scan_incl(hit, scan, &total) + base;
-        if (hit) a.todo[(long long)row * a.pages + at - 1] = i;
+    for (int i0 = 0; i0 < a.pages; i0 += ER * ET) {
+        unsigned hit[ER];
+#pragma unroll
+        for (int i = 0; i < ER; i++) {
+            const int p = i0 + i * ET + tid;
+            hit[i] = __ballot_sync(kAll, p < a.pages && (flag[p] || (p == a.pages - 1 && keep % c.page)));
+            if (lane == 0) order[i * (ET / 32) + warp] = __popc(hit[i]);
+        }
+        const int total = scan_counts<ET, ER>(order, &order_n);
+#pragma unroll
+        for (int i = 0; i < ER; i++)
+            if (hit[i] >> lane & 1u)
+                a.todo[(long long)row * a.pages + base + order[i * (ET / 32) + warp] + __popc(hit[i] & ((1u << lane) - 1u))] = i0 + i * ET + tid;
         base += total;
+        __syncthreads();
     }
     if (tid == 0) a.used[2 * row + 1] = base;
 }
@@ -881,29 +1065,42 @@ __device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int 
         mn[j] = __half2half2(__ushort_as_half(0x7c00));
         mx[j] = __half2half2(__ushort_as_half(0xfc00));
     }
-#pragma unroll 4
-    for (int i = sub; i < rows; i += rpw) {
-        const int k = src[i];
-        int from = -1, slot = i;
-        if (k >= 0) {
-            const int pl = page_quot(c.div, k);
-            from = page_id(c.table, c.ts, s, pl, c.mp, c.n_pages);
-            slot = k - pl * c.page;
-        }
-        if (!live || (!bounds && from < 0)) continue;
-        const int rid = from >= 0 ? from : id;
-        if (from < 0) slot = i;
-        const uint4 kv = *reinterpret_cast<const uint4 *>(c.K + row_at(rid, slot, g, c.kp, c.kk, c.kh) + ch * 8);
-        if (from >= 0) {
-            const uint4 vv = *reinterpret_cast<const uint4 *>(c.V + row_at(rid, slot, g, c.vp, c.vk, c.vh) + ch * 8);
-            *reinterpret_cast<uint4 *>(c.K + row_at(id, i, g, c.kp, c.kk, c.kh) + ch * 8) = kv;
-            *reinterpret_cast<uint4 *>(c.V + row_at(id, i, g, c.vp, c.vk, c.vh) + ch * 8) = vv;
-        }
-        const unsigned x[4] = {kv.x, kv.y, kv.z, kv.w};
+    constexpr int U = 4;   // rows in flight per lane: all their loads come before the first store
+    for (int i0 = sub; i0 < rows; i0 += U * rpw) {
+        int from[U], slot[U], k[U];
+        uint4 kv[U], vv[U];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            mn[j] = __hmin2(mn[j], as_h2(x[j]));
-            mx[j] = __hmax2(mx[j], as_h2(x[j]));
+        for (int j = 0; j < U; j++) k[j] = i0 + j * rpw < rows ? __ldg(src + i0 + j * rpw) : -1;
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int pl = page_quot(c.div, max(k[j], 0));
+            from[j] = k[j] >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
+            slot[j] = from[j] >= 0 ? k[j] - pl * c.page : i0 + j * rpw;
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const bool row = live && i0 + j * rpw < rows;
+            const int rid = from[j] >= 0 ? from[j] : id;
+            if (row && (bounds || from[j] >= 0))
+                kv[j] = __ldcg(reinterpret_cast<const uint4 *>(c.K + row_at(rid, slot[j], g, c.kp, c.kk, c.kh) + ch * 8));
+            if (row && from[j] >= 0)
+                vv[j] = __ldcg(reinterpret_cast<const uint4 *>(c.V + row_at(rid, slot[j], g, c.vp, c.vk, c.vh) + ch * 8));
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int i = i0 + j * rpw;
+            if (!live || i >= rows) continue;
+            if (from[j] >= 0) {
+                *reinterpret_cast<uint4 *>(c.K + row_at(id, i, g, c.kp, c.kk, c.kh) + ch * 8) = kv[j];
+                *reinterpret_cast<uint4 *>(c.V + row_at(id, i, g, c.vp, c.vk, c.vh) + ch * 8) = vv[j];
+            }
+            if (!bounds) continue;
+            const unsigned x[4] = {kv[j].x, kv[j].y, kv[j].z, kv[j].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                mn[e] = __hmin2(mn[e], as_h2(x[e]));
+                mx[e] = __hmax2(mx[e], as_h2(x[e]));
+            }
         }
     }
     if (!bounds) return;
@@ -922,7 +1119,8 @@ __device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int 
 // The moves: the warps of `ctas` CTAs per row take the row's changed pages in turn. lpr lanes carry a row, 16 bytes each; the
 // bounds of a page are taken over the rows it now holds, the movers' from their sources. Every source lies at or above keep
 // and every target below, so that the order of the moves does not matter. Bound by memory: rows in and out.
-__global__ void __launch_bounds__(256) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
+constexpr int MT = 128;
+__global__ void __launch_bounds__(MT, 6) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
@@ -931,7 +1129,7 @@ __global__ void __launch_bounds__(256) kv_move_k(const __grid_constant__ EvictAr
     const int s = row / c.HKV, g = row - s * c.HKV, keep = a.keep;
     if (part == 0 && g == 0 && threadIdx.x == 0) a.len_out[s] = min(a.used[2 * row], keep);
     const int todo = a.used[2 * row + 1];
-    for (int w = part * 8 + (threadIdx.x >> 5); w < todo; w += ctas * 8) {
+    for (int w = part * (MT / 32) + (threadIdx.x >> 5); w < todo; w += ctas * (MT / 32)) {
         const int place = a.todo[(long long)row * a.pages + w];
         const int k0 = place * c.page, rows = min(c.page, keep - k0);
         const int *src = a.src + (long long)row * keep + k0;
@@ -1094,9 +1292,9 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     a.tiles = (int)tiles;
     a.tg = (int)std::min(tg, zt);
     a.zt = (int)zt;
-    // steps of a warp: about eight CTAs per SM over all (stream, head) rows, at most 8 steps, which amortise the queries
+    // steps of a warp: about four CTAs per SM over all (stream, head) rows, which amortises the queries
     const long long all = (c->mp + SPAGES - 1) / SPAGES, sg = (long long)c->ns * c->HKV * zs;
-    a.steps = (int)std::min<long long>(8, std::max<long long>(1, all * sg / (8LL * SW * call.d->sm_count)));
+    a.steps = (int)std::max<long long>(1, all * sg / (4LL * SW * call.d->sm_count));
     const int ctas = (int)std::max<long long>(1, (all + SW * a.steps - 1) / (SW * a.steps));
     const size_t score = up256((size_t)rows * c->mp * 4), key = up256((size_t)rows * c->mp * 8),
                  l1 = up256((size_t)c->ns * nq * H * 4), peak = up256((size_t)sg * ctas * SW * 4);
@@ -1104,6 +1302,7 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     unsigned *cnt = nullptr;
     G9_TRY(kv_workspace(ws, call, who, score + key + l1 + peak, 0, &buf, &cnt));
     a.score = (float *)buf;
+    a.err = call.d->err_dev;
     a.key = (unsigned long long *)((char *)buf + score);
     a.l1 = (float *)((char *)buf + score + key);
     a.peak = (float *)((char *)buf + score + key + l1);
@@ -1153,13 +1352,14 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     a.flag = (int *)((char *)buf + 2 * list);
     a.todo = (int *)((char *)buf + 2 * list + pages);
     a.used = (int *)((char *)buf + 2 * list + 2 * pages);
-    G9_CU(launch_pdl(kv_rank_k, dim3((unsigned)rows), dim3(ET), 0, call.st, a));
+    if (a.c.cap <= 256 * ER) G9_CU(launch_pdl(kv_rank_k<256>, dim3((unsigned)rows), dim3(256), 0, call.st, a));
+    else G9_CU(launch_pdl(kv_rank_k<1024>, dim3((unsigned)rows), dim3(1024), 0, call.st, a));
     G9_TRY(launched("kv_rank"));
-    // a page per warp where the rows are few, up to about 16 CTAs per SM in all
-    const long long most = (a.pages + 7) / 8, ctas = std::max<long long>(1, std::min(most, 16LL * call.d->sm_count / rows));
+    // a page per warp where the rows are few, else one wave of CTAs in all
+    const long long most = (a.pages + MT / 32 - 1) / (MT / 32), ctas = std::max<long long>(1, std::min(most, 6LL * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
     if (rows * ctas > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows in one call", who, rows);
-    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(256), 0, call.st, a, (int)ctas, lpr));
+    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
     const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};
