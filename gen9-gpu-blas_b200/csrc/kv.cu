@@ -3,6 +3,7 @@
 // reference, whose attention (lib/gen9blas_ml.h:122-149) reads one contiguous cache per stream.
 #include "kv.h"
 #include "common.cuh"
+#include "kv_plan.cuh"
 #include "mma_sync.cuh"
 #include "sm100.cuh"
 #include <algorithm>
@@ -220,7 +221,7 @@ __device__ __forceinline__ unsigned as_u(__half2 x) { return *reinterpret_cast<c
 
 // One CTA per (page that may be touched, head, stream); its warps take the page's new rows in turn, a lane four elements
 // (or two times four, D > 128) of each row, and keep the elements' least and largest value for the bounds.
-__global__ void __launch_bounds__(256) kv_append_k(AppendArgs a) {
+__global__ void __launch_bounds__(256, 4) kv_append_k(const __grid_constant__ AppendArgs a) {
     __shared__ uint2 red[8][2][2][32];   // [warp][least, largest][four-element group of the lane][lane]
     pdl_next();
     pdl_wait();
@@ -313,15 +314,16 @@ __global__ void __launch_bounds__(256) kv_append_k(AppendArgs a) {
 struct SelectArgs {
     KvDev c;
     int G, H, nq, dvis, first, last, nsel;
-    int hg, tiles, tg, zt, steps;   // 8-head groups of a token, row tiles (token, group) in all, at once in a CTA, and in all
-                                    // of a CTA (whole tokens; more than tg only where one token's groups are more); steps
-                                    // of a warp
+    int hg, tiles, tg, zt, zs;      // 8-head groups of a token, row tiles (token, group) in all, at once in a CTA, in all of a unit
+                                    // (whole tokens; more than tg only where one token's groups are more), units of a head
+    int unit_steps;                 // most steps of a unit: ⌈mp / 16⌉
+    PageDiv by_zs;
     const float *Q;
     long long qt, qh, qs;
     const int *vis;
     float *score;               // [row (s, t, g)][mp]: FP32 scores; kv_choose_k overwrites those that it decided by hand
     float *l1;                  // [(s, t, h)]: sum of |q|
-    float *peak;                // [(s, g)][CTA][warp]: largest |bound| seen; infinity where a score is not finite
+    float *peak;                // [(s, g, z)][unit_steps]: largest |bound| of a step; infinity where a score is not finite
     unsigned long long *key;    // [row][mp]: 64-bit keys of pages decided by hand, where they are many
     int *sel;
     unsigned *err;              // the device's error word
@@ -339,6 +341,7 @@ __device__ __forceinline__ void bulk_row(void *dst, const void *src, unsigned by
                  : "memory");
 }
 constexpr uint64_t SWAIT_NS = 2000000000ull;   // a row that has not landed after 2 s is an error
+constexpr int SCOST = 8;   // steps that a CTA reads in the time of a segment's latencies
 constexpr int SW = 4, SPAGES = 16, SNST = 3;   // warps of a CTA, pages of a step, stages of a warp's ring
 template <int DP>
 struct ScoreCfg {
@@ -353,10 +356,10 @@ struct ScoreCfg {
 
 // Score of (page, query head): Σ_d max(q_d·lo_d, q_d·hi_d) = Σ min(q, 0)·lo + Σ max(q, 0)·hi, a product of the bounds (A, 16
 // pages × 16 elements, FP16 as they are) with the two halves of the query (B, 8 heads) in two FP16 parts each, as in
-// attn_paged_k. A CTA's four warps take every fourth step of 16 pages of one (stream, head) through rings of their own,
-// for all its row tiles (token, 8 heads); a page's score is the largest over the heads of a token. Where a token has more
-// head groups than shared memory holds, the CTA reads its pages again for the next ones. Bound by the reading of the
-// bounds.
+// attn_paged_k. Units are (stream, head, tokens whose tiles of 8 heads shared memory holds at once); a CTA's run (kv_plan.cuh)
+// is a stretch of steps of 16 pages, of which its four warps take every fourth through rings of their own. A page's score is
+// the largest over the heads of a token; where one token has more tiles than fit, the CTA reads its pages again for the next
+// ones. Bound by the reading of the bounds.
 template <int DP>
 __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ SelectArgs a) {
     using C = ScoreCfg<DP>;
@@ -379,153 +382,175 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
     __syncwarp();
     pdl_next();
     pdl_wait();
-    const int sg = blockIdx.y, s = sg / c.HKV, g = sg - s * c.HKV;
-    const int z0 = blockIdx.z * a.zt, z1 = min(z0 + a.zt, a.tiles);
-    const int have = pages_seen(a, s, (z1 - 1) / a.hg);
-    const int step0 = blockIdx.x * SW * a.steps, all = (have + SPAGES - 1) / SPAGES;
-    if (step0 >= all) return;
-    const int my = min(a.steps, max(0, (all - step0 - warp + SW - 1) / SW)), kts = (c.D + 15) / 16;
+    const int kts = (c.D + 15) / 16, inner = c.HKV * a.zs;
     const unsigned wbase = sm100::smem_u32(wring);
-    unsigned copied = 0;   // copies of this warp so far: copy n goes to stage n % SNST, in the barrier's phase n / SNST
-    auto id_of = [&](int i) {
-        const int p = (step0 + warp + SW * i) * SPAGES + (lane & 15);
-        return i < my && p < have ? page_id(c.table, c.ts, s, p, c.mp, c.n_pages) : -1;
-    };
-    // one bulk copy per page, both rows (lane l < 16: page l); a page that is missing keeps what its place held before
-    auto copy = [&](int i, int id) {
-        if (i >= my) return;
-        const int st = copied % SNST;
-        const unsigned here = __ballot_sync(kAll, lane < SPAGES && id >= 0);
-        if (lane == 0) sm100::mbar_arrive_expect_tx(bar + st, __popc(here) * c.D * 4);
-        __syncwarp();
-        if (here >> lane & 1u)
-            bulk_row(wring + st * C::STAGE + lane * PITCH, c.bounds + ((long long)id * c.HKV + g) * 2 * c.D, c.D * 4, bar + st);
-        copied++;
-    };
+    unsigned copied = 0, used = 0;   // copies of this warp so far, and those it has waited for: copy n goes to stage n % SNST,
+                                     // in the barrier's phase n / SNST
     const int arow = (lane & 7) + ((lane >> 3) & 1) * 8, acol = lane >> 4;
-    __half2 peak = __half2half2(__ushort_as_half(0));
-    bool wild = false, ok = true;
-    unsigned used = 0;   // copies of this warp that it has waited for
+    bool ok = true;
     auto wait = [&]() {
         ok = ok && sm100::mbar_wait(bar + used % SNST, used / SNST & 1, &quit, SWAIT_NS);
         used++;
     };
-    for (int tile0 = z0; tile0 < z1 && ok; tile0 += a.tg) {
-        const int ntile = min(a.tg, z1 - tile0);
-        if (tile0 > z0) __syncthreads();   // every warp has left the last tiles' fragments
-        int ids[SNST - 1];
-#pragma unroll
-        for (int i = 0; i < SNST - 1; i++) ids[i] = id_of(i);
-#pragma unroll
-        for (int i = 0; i < SNST - 1; i++) copy(i, ids[i]);
-        int next = id_of(SNST - 1), now = ids[0], after = ids[1];
-        // ---- query fragments: a warp prepares every fourth row of the tiles
-        for (int r = warp; r < ntile * 8; r += SW) {
-            const int tile = tile0 + (r >> 3), t = tile / a.hg, h = (tile - t * a.hg) * 8 + (r & 7);
-            const bool live = h < a.G;
-            const float *qp = a.Q + s * a.qs + t * a.qt + (long long)(g * a.G + (live ? h : 0)) * a.qh;
-            float x[DP / 32], big = 0.0f, l1 = 0.0f;
-#pragma unroll
-            for (int i = 0; i < DP / 64; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int d = 64 * i + 2 * lane + j;
-                    const float v = live && d < c.D ? qp[d] : 0.0f;
-                    x[2 * i + j] = v;
-                    big = fmaxf(big, fabsf(v));
-                    l1 += fabsf(v);
-                }
-            for (int i = 16; i > 0; i >>= 1) {
-                big = fmaxf(big, __shfl_xor_sync(kAll, big, i));
-                l1 += __shfl_xor_sync(kAll, l1, i);
-            }
-            int ex = 0;
-            if (big > 0.0f) ex = min(max(140 - (int)((__float_as_uint(big) >> 23) & 0xffu), -126), 126);
-            const float up = at_pow2(ex);
-            if (lane == 0) {
-                qinv[r] = at_pow2(-ex);
-                if (live && blockIdx.x == 0) a.l1[((long long)s * a.nq + t) * a.H + g * a.G + h] = l1;
-            }
-#pragma unroll
-            for (int i = 0; i < DP / 64; i++)
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
-                    y0 = half ? fmaxf(y0, 0.0f) : fminf(y0, 0.0f);
-                    y1 = half ? fmaxf(y1, 0.0f) : fminf(y1, 0.0f);
-                    unsigned h2, l2;
-                    at_split(y0, y1, h2, l2);
-                    const int d = 64 * i + 2 * lane, kt = d >> 4, dd = d & 15;
-                    unsigned *f = reinterpret_cast<unsigned *>(qf + (((r >> 3) * 2 + half) * KT + kt) * 32 + (r & 7) * 4 + ((dd & 7) >> 1));
-                    f[dd >> 3] = h2;
-                    f[2 + (dd >> 3)] = l2;
-                }
+    auto unit_steps = [&](int s) { return max(1, (pages_seen(a, s, a.nq - 1) + SPAGES - 1) / SPAGES); };
+    const Run run = find_run(c.ns, inner, SCOST, SW, unit_steps);
+    int s = run.outer, pre = run.pre;
+    for (int at = run.lo; at < run.hi && ok;) {
+        const int nv = unit_steps(s) + SCOST, iu = (at - pre) / nv;
+        if (iu >= inner) {
+            pre += nv * inner;
+            s++;
+            continue;
         }
-        __syncthreads();
-        for (int i = 0; i < my; i++) {
-            const unsigned lo = wbase + used % SNST * C::STAGE, hi = lo + c.D * 2;
-            wait();
-            if (!__all_sync(kAll, ok)) {
-                ok = false;
-                break;
-            }
-            copy(i + SNST - 1, next);   // into the stage before this one, which every lane has left
-            const int p = (step0 + warp + SW * i) * SPAGES + gq;
-            const bool in0 = __shfl_sync(kAll, now, gq) >= 0, in1 = __shfl_sync(kAll, now, gq + 8) >= 0;
-            float top[2] = {-INFINITY, -INFINITY};
-            __half2 pk0 = __half2half2(__ushort_as_half(0)), pk1 = pk0;
-            for (int tile = 0; tile < ntile; tile++) {
-                float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-                const uint4 *q0 = qf + tile * 2 * KT * 32 + lane, *q1 = q0 + KT * 32;
+        const int us = pre + iu * nv, sb = max(at - us - SCOST, 0), se = min(run.hi - us, nv) - SCOST;
+        at = us + nv;
+        if (se <= 0) break;   // the run ends before the unit's first step
+        const int g = page_quot(a.by_zs, iu), z = iu - g * a.zs;
+        const int z0 = z * a.zt, z1 = min(z0 + a.zt, a.tiles);
+        const int have = pages_seen(a, s, (z1 - 1) / a.hg);   // of the unit's last token; steps go by the call's last
+        float *peaks = a.peak + (((long long)s * c.HKV + g) * a.zs + z) * a.unit_steps;
+        const int my = se > sb + warp ? (se - sb - warp + SW - 1) / SW : 0;
+        auto id_of = [&](int i) {
+            const int p = (sb + warp + SW * i) * SPAGES + (lane & 15);
+            return i < my && p < have ? page_id(c.table, c.ts, s, p, c.mp, c.n_pages) : -1;
+        };
+        // one bulk copy per page, both rows (lane l < 16: page l); a page that is missing keeps what its place held before
+        auto copy = [&](int i, int id) {
+            if (i >= my) return;
+            const int st = copied % SNST;
+            const unsigned here = __ballot_sync(kAll, lane < SPAGES && id >= 0);
+            if (lane == 0) sm100::mbar_arrive_expect_tx(bar + st, __popc(here) * c.D * 4);
+            __syncwarp();
+            if (here >> lane & 1u)
+                bulk_row(wring + st * C::STAGE + lane * PITCH, c.bounds + ((long long)id * c.HKV + g) * 2 * c.D, c.D * 4, bar + st);
+            copied++;
+        };
+        __syncthreads();   // every warp has left the last unit's fragments
+        for (int tile0 = z0; tile0 < z1 && ok; tile0 += a.tg) {
+            const int ntile = min(a.tg, z1 - tile0);
+            if (tile0 > z0) __syncthreads();   // every warp has left the last tiles' fragments
+            int ids[SNST - 1];
 #pragma unroll
-                for (int kt = 0; kt < KT; kt++) {
-                    if (kt >= kts) break;
-                    const unsigned off = arow * PITCH + kt * 32 + acol * 16;
-                    unsigned l4[4], u4[4];
-                    at_ldsm(lo + off, l4);
-                    at_ldsm(hi + off, u4);
-                    if (tile == 0) {   // registers 0 and 2: page gq, 1 and 3: page gq + 8
-                        pk0 = __hmax2(__hmax2(pk0, __hmax2(__habs2(as_h2(l4[0])), __habs2(as_h2(l4[2])))),
-                                      __hmax2(__habs2(as_h2(u4[0])), __habs2(as_h2(u4[2]))));
-                        pk1 = __hmax2(__hmax2(pk1, __hmax2(__habs2(as_h2(l4[1])), __habs2(as_h2(l4[3])))),
-                                      __hmax2(__habs2(as_h2(u4[1])), __habs2(as_h2(u4[3]))));
+            for (int i = 0; i < SNST - 1; i++) ids[i] = id_of(i);
+#pragma unroll
+            for (int i = 0; i < SNST - 1; i++) copy(i, ids[i]);
+            int next = id_of(SNST - 1), now = ids[0], after = ids[1];
+            // ---- query fragments: a warp prepares every fourth row of the tiles
+            for (int r = warp; r < ntile * 8; r += SW) {
+                const int tile = tile0 + (r >> 3), t = tile / a.hg, h = (tile - t * a.hg) * 8 + (r & 7);
+                const bool live = h < a.G;
+                const float *qp = a.Q + s * a.qs + t * a.qt + (long long)(g * a.G + (live ? h : 0)) * a.qh;
+                float x[DP / 32], big = 0.0f, l1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < DP / 64; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int d = 64 * i + 2 * lane + j;
+                        const float v = live && d < c.D ? qp[d] : 0.0f;
+                        x[2 * i + j] = v;
+                        big = fmaxf(big, fabsf(v));
+                        l1 += fabsf(v);
                     }
-                const uint4 f = q0[kt * 32], h = q1[kt * 32];
-                    at_mma(sc[0], l4, f.x, f.y);
-                    at_mma(sc[1], u4, h.x, h.y);
-                    at_mma(sc[0], l4, f.z, f.w);
-                    at_mma(sc[1], u4, h.z, h.w);
+                for (int i = 16; i > 0; i >>= 1) {
+                    big = fmaxf(big, __shfl_xor_sync(kAll, big, i));
+                    l1 += __shfl_xor_sync(kAll, l1, i);
                 }
-                const int t = (tile0 + tile) / a.hg, hb = (tile0 + tile - t * a.hg) * 8;
+                int ex = 0;
+                if (big > 0.0f) ex = min(max(140 - (int)((__float_as_uint(big) >> 23) & 0xffu), -126), 126);
+                const float up = at_pow2(ex);
+                if (lane == 0) {
+                    qinv[r] = at_pow2(-ex);
+                    if (live && sb == 0) a.l1[((long long)s * a.nq + t) * a.H + g * a.G + h] = l1;
+                }
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (hb + 2 * tq + j >= a.G) continue;
-                    const float inv = qinv[tile * 8 + 2 * tq + j];
-                    const float x0 = (sc[0][j] + sc[1][j]) * inv, x1 = (sc[0][2 + j] + sc[1][2 + j]) * inv;
-                    wild = wild || (in0 && !(fabsf(x0) < INFINITY)) || (in1 && !(fabsf(x1) < INFINITY));
-                    top[0] = fmaxf(top[0], x0);
-                    top[1] = fmaxf(top[1], x1);
-                }
-                if ((tile0 + tile) % a.hg != a.hg - 1 && tile != ntile - 1) continue;   // more heads of this token follow
+                for (int i = 0; i < DP / 64; i++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 1));
-                    top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 2));
-                }
-                if (tq == 0) {
-                    float *out = a.score + (((long long)s * a.nq + t) * c.HKV + g) * c.mp;
-                    const bool more = tile0 > z0;   // the token's earlier groups have left their largest
-                    if (p < have) out[p] = in0 ? (more ? fmaxf(out[p], top[0]) : top[0]) : -INFINITY;
-                    if (p + 8 < have) out[p + 8] = in1 ? (more ? fmaxf(out[p + 8], top[1]) : top[1]) : -INFINITY;
-                }
-                top[0] = top[1] = -INFINITY;
+                    for (int half = 0; half < 2; half++) {
+                        float y0 = x[2 * i] * up, y1 = x[2 * i + 1] * up;
+                        y0 = half ? fmaxf(y0, 0.0f) : fminf(y0, 0.0f);
+                        y1 = half ? fmaxf(y1, 0.0f) : fminf(y1, 0.0f);
+                        unsigned h2, l2;
+                        at_split(y0, y1, h2, l2);
+                        const int d = 64 * i + 2 * lane, kt = d >> 4, dd = d & 15;
+                        unsigned *f = reinterpret_cast<unsigned *>(qf + (((r >> 3) * 2 + half) * KT + kt) * 32 + (r & 7) * 4 + ((dd & 7) >> 1));
+                        f[dd >> 3] = h2;
+                        f[2 + (dd >> 3)] = l2;
+                    }
             }
-            if (in0) peak = __hmax2(peak, pk0);
-            if (in1) peak = __hmax2(peak, pk1);
-            now = after;
-            after = next;
-            next = id_of(i + SNST);
-            __syncwarp();   // every lane has read this stage
+            __syncthreads();
+            for (int i = 0; i < my; i++) {
+                const unsigned lo = wbase + used % SNST * C::STAGE, hi = lo + c.D * 2;
+                wait();
+                if (!__all_sync(kAll, ok)) {
+                    ok = false;
+                    break;
+                }
+                copy(i + SNST - 1, next);   // into the stage before this one, which every lane has left
+                const int step = sb + warp + SW * i, p = step * SPAGES + gq;
+                const bool in0 = __shfl_sync(kAll, now, gq) >= 0, in1 = __shfl_sync(kAll, now, gq + 8) >= 0;
+                float top[2] = {-INFINITY, -INFINITY};
+                __half2 pk0 = __half2half2(__ushort_as_half(0)), pk1 = pk0;
+                bool wild = false;
+                for (int tile = 0; tile < ntile; tile++) {
+                    float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                    const uint4 *q0 = qf + tile * 2 * KT * 32 + lane, *q1 = q0 + KT * 32;
+#pragma unroll
+                    for (int kt = 0; kt < KT; kt++) {
+                        if (kt >= kts) break;
+                        const unsigned off = arow * PITCH + kt * 32 + acol * 16;
+                        unsigned l4[4], u4[4];
+                        at_ldsm(lo + off, l4);
+                        at_ldsm(hi + off, u4);
+                        if (tile == 0) {   // registers 0 and 2: page gq, 1 and 3: page gq + 8
+                            pk0 = __hmax2(__hmax2(pk0, __hmax2(__habs2(as_h2(l4[0])), __habs2(as_h2(l4[2])))),
+                                          __hmax2(__habs2(as_h2(u4[0])), __habs2(as_h2(u4[2]))));
+                            pk1 = __hmax2(__hmax2(pk1, __hmax2(__habs2(as_h2(l4[1])), __habs2(as_h2(l4[3])))),
+                                          __hmax2(__habs2(as_h2(u4[1])), __habs2(as_h2(u4[3]))));
+                        }
+                    const uint4 f = q0[kt * 32], h = q1[kt * 32];
+                        at_mma(sc[0], l4, f.x, f.y);
+                        at_mma(sc[1], u4, h.x, h.y);
+                        at_mma(sc[0], l4, f.z, f.w);
+                        at_mma(sc[1], u4, h.z, h.w);
+                    }
+                    const int t = (tile0 + tile) / a.hg, hb = (tile0 + tile - t * a.hg) * 8;
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        if (hb + 2 * tq + j >= a.G) continue;
+                        const float inv = qinv[tile * 8 + 2 * tq + j];
+                        const float x0 = (sc[0][j] + sc[1][j]) * inv, x1 = (sc[0][2 + j] + sc[1][2 + j]) * inv;
+                        wild = wild || (in0 && !(fabsf(x0) < INFINITY)) || (in1 && !(fabsf(x1) < INFINITY));
+                        top[0] = fmaxf(top[0], x0);
+                        top[1] = fmaxf(top[1], x1);
+                    }
+                    if ((tile0 + tile) % a.hg != a.hg - 1 && tile != ntile - 1) continue;   // more heads of this token follow
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 1));
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(kAll, top[e], 2));
+                    }
+                    if (tq == 0) {
+                        float *out = a.score + (((long long)s * a.nq + t) * c.HKV + g) * c.mp;
+                        const bool more = tile0 > z0;   // the token's earlier groups have left their largest
+                        if (p < have) out[p] = in0 ? (more ? fmaxf(out[p], top[0]) : top[0]) : -INFINITY;
+                        if (p + 8 < have) out[p + 8] = in1 ? (more ? fmaxf(out[p + 8], top[1]) : top[1]) : -INFINITY;
+                    }
+                    top[0] = top[1] = -INFINITY;
+                }
+                if (!in0) pk0 = __half2half2(__ushort_as_half(0));
+                if (in1) pk0 = __hmax2(pk0, pk1);
+                // FP16 bits of positive numbers keep their order
+                const unsigned top16 = __reduce_max_sync(kAll, max(as_u(pk0) & 0xffffu, as_u(pk0) >> 16));
+                wild = __any_sync(kAll, wild);
+                if (lane == 0) {
+                    const float pk = wild ? INFINITY : __half2float(__ushort_as_half((unsigned short)top16));
+                    peaks[step] = tile0 > z0 ? fmaxf(peaks[step], pk) : pk;
+                }
+                now = after;
+                after = next;
+                next = id_of(i + SNST);
+                __syncwarp();   // every lane has read this stage
+            }
         }
     }
     if (!ok) {   // a copy that has not landed: what is in flight is waited for, again with a limit
@@ -536,10 +561,6 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
             *(volatile unsigned *)a.err = kDevErrWaitTimeout;
         }
     }
-    float pk = fmaxf(__low2float(peak), __high2float(peak));
-    for (int i = 16; i > 0; i >>= 1) pk = fmaxf(pk, __shfl_xor_sync(kAll, pk, i));
-    if (__any_sync(kAll, wild)) pk = INFINITY;
-    if (lane == 0) a.peak[(((long long)blockIdx.z * gridDim.y + sg) * gridDim.x + blockIdx.x) * SW + warp] = pk;
 }
 
 __device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   // whole CTA, at most 1024 threads
@@ -566,30 +587,60 @@ __device__ __forceinline__ int block_scan_incl(int v, int *sh, int *total) {   /
 
 constexpr int NLIST = 64;
 struct NthKey {   // shared memory of nth_key
-    int counts[2][3][32];
+    uint32_t buf[2][4][32];
     uint32_t list[NLIST];
-    int n;
+    int n, found[3];
 };
-// The m-th largest of n 32-bit keys (n >= m >= 1) of a CTA, and how many are larger. Two bits a round from the top: the counts
-// of keys at least as large as each of three candidates, added up in the warps and through shared memory, one barrier a
-// round, until at most NLIST keys share the bits found; those are ranked directly. Thread t holds the keys t, t + NT, ... in
-// reg (0 past the end); keys beyond R·NT come from `more` in every round. (Radix selection with shared-memory histograms took
-// 3 to 4 µs a digit here, for the crowding of keys in few bins, its scans and four barriers each.)
+// The m-th largest of n keys (n >= m >= 1) of a CTA, how many are larger and how many as large. A range of keys is cut into
+// four a round, by the counts of the keys at least as large as each of three borders (added up in the warps and through
+// shared memory, one barrier a round), from the least and the largest key on, until at most NLIST keys lie in it; those are
+// ranked directly. Keys of all ones stand above the range. Thread t holds the keys t, t + NT, ... in reg (anything past the
+// end); keys beyond R·NT come from `more` in every round. Scores and weights fill their range evenly enough for about three
+// rounds; it takes 16 at most. (Radix selection with shared-memory histograms took 3 to 4 µs a digit here, for the crowding
+// of keys in few bins, its scans and four barriers each; cutting from the top bit on 0.7 µs a round, eight rounds.)
 template <int NT, int R, typename More>
-__device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int m, NthKey &sh, More more, int *larger) {
+__device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int m, NthKey &sh, More more, int *larger, int *equal) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    uint32_t v = 0;
-    int above = 0, in = n, shift = 32;   // keys above the range [v, v + 2^shift), keys in it
+    constexpr int W = NT / 32;
+    uint32_t lo = kAll, hi = 0;
+    int top = 0;
+    auto range = [&](uint32_t k) {
+        top += k == kAll;
+        lo = min(lo, k);
+        hi = k == kAll ? hi : max(hi, k);
+    };
+#pragma unroll
+    for (int i = 0; i < R; i++)
+        if ((int)threadIdx.x + i * NT < n) range(reg[i]);
+    for (int i = R * NT + threadIdx.x; i < n; i += NT) range(more(i));
+    lo = __reduce_min_sync(kAll, lo);
+    hi = __reduce_max_sync(kAll, hi);
+    top = __reduce_add_sync(kAll, top);
+    if (lane == 0) {
+        sh.buf[0][0][w] = lo;
+        sh.buf[0][1][w] = hi;
+        sh.buf[0][2][w] = top;
+    }
     if (threadIdx.x == 0) sh.n = 0;
-    for (int round = 0; round < 16 && in > NLIST; round++) {
-        shift -= 2;
-        int c1 = 0, c2 = 0, c3 = 0;
-        const uint32_t a1 = v | 1u << shift, a2 = v | 2u << shift, a3 = v | 3u << shift;
+    __syncthreads();
+    lo = __reduce_min_sync(kAll, lane < W ? sh.buf[0][0][lane] : kAll);
+    hi = __reduce_max_sync(kAll, lane < W ? sh.buf[0][1][lane] : 0u);
+    top = __reduce_add_sync(kAll, lane < W ? (int)sh.buf[0][2][lane] : 0);
+    if (top >= m) {
+        *larger = 0;
+        *equal = top;
+        return kAll;
+    }
+    int above = top, in = n - top;   // keys above hi, keys in [lo, hi]
+    for (int round = 1; in > NLIST && lo < hi; round++) {
+        const uint32_t d = hi - lo, a1 = lo + (d >> 2) + 1, a2 = lo + (d >> 1) + 1, a3 = lo + (d >> 1) + (d >> 2) + 1;
+        uint32_t c1 = 0, c2 = 0, c3 = 0;
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            c1 += reg[i] >= a1;
-            c2 += reg[i] >= a2;
-            c3 += reg[i] >= a3;
+            const uint32_t k = (int)threadIdx.x + i * NT < n ? reg[i] : 0u;   // a1 > 0
+            c1 += k >= a1;
+            c2 += k >= a2;
+            c3 += k >= a3;
         }
         for (int i = R * NT + threadIdx.x; i < n; i += NT) {
             const uint32_t k = more(i);
@@ -597,40 +648,46 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
             c2 += k >= a2;
             c3 += k >= a3;
         }
+        uint32_t (&buf)[4][32] = sh.buf[round & 1];
         c1 = __reduce_add_sync(kAll, c1);
         c2 = __reduce_add_sync(kAll, c2);
         c3 = __reduce_add_sync(kAll, c3);
-        int (&buf)[3][32] = sh.counts[round & 1];
         if (lane == 0) {
             buf[0][w] = c1;
             buf[1][w] = c2;
             buf[2][w] = c3;
         }
         __syncthreads();
-        c1 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[0][lane] : 0);
-        c2 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[1][lane] : 0);
-        c3 = __reduce_add_sync(kAll, lane < NT / 32 ? buf[2][lane] : 0);
-        if (c3 >= m) {
-            v = a3;
-            in = c3 - above;
-        } else if (c2 >= m) {
-            v = a2;
-            in = c2 - c3;
-            above = c3;
-        } else if (c1 >= m) {
-            v = a1;
-            in = c1 - c2;
-            above = c2;
+        c1 = __reduce_add_sync(kAll, lane < W ? buf[0][lane] : 0u);
+        c2 = __reduce_add_sync(kAll, lane < W ? buf[1][lane] : 0u);
+        c3 = __reduce_add_sync(kAll, lane < W ? buf[2][lane] : 0u);
+        const int all = in + above;   // keys of at least lo
+        if ((int)c3 >= m) {
+            lo = a3;
+            in = (int)c3 - above;
+        } else if ((int)c2 >= m) {
+            lo = a2;
+            hi = a3 - 1;
+            in = (int)(c2 - c3);
+            above = (int)c3;
+        } else if ((int)c1 >= m) {
+            lo = a1;
+            hi = a2 - 1;
+            in = (int)(c1 - c2);
+            above = (int)c2;
         } else {
-            in = in + above - c1;
-            above = c1;
+            hi = a1 - 1;
+            in = all - (int)c1;
+            above = (int)c1;
         }
     }
-    *larger = above;
-    if (in > NLIST || shift == 0) return v;   // equal keys to the last bit
-    __syncthreads();   // sh.n is set
+    if (in > NLIST) {   // equal keys
+        *larger = above;
+        *equal = in;
+        return lo;
+    }
     auto put = [&](uint32_t k) {
-        if (shift == 32 || k >> shift == v >> shift) {
+        if (k >= lo && k <= hi) {
             const int at = atomicAdd(&sh.n, 1);
             if (at < NLIST) sh.list[at] = k;   // never more
         }
@@ -640,56 +697,44 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
         if ((int)threadIdx.x + i * NT < n) put(reg[i]);
     for (int i = R * NT + threadIdx.x; i < n; i += NT) put(more(i));
     __syncthreads();
-    // lane: the keys lane and lane + 32 of the list
-    const uint32_t k0 = lane < in ? sh.list[lane] : 0u, k1 = lane + 32 < in ? sh.list[lane + 32] : 0u;
-    int g0 = 0, g1 = 0, e0 = 0, e1 = 0;   // keys larger than each, and as large
-    for (int i = 0; i < in; i++) {
-        const uint32_t k = sh.list[i];
-        g0 += k > k0;
-        g1 += k > k1;
-        e0 += k >= k0;
-        e1 += k >= k1;
-    }
-    const int r = m - above;   // the r-th of the list: fewer than r are larger, at least r as large
-    const unsigned hit0 = __ballot_sync(kAll, lane < in && g0 < r && e0 >= r), hit1 = __ballot_sync(kAll, lane + 32 < in && g1 < r && e1 >= r);
-    const int l = __ffs(hit0 ? hit0 : hit1) - 1;
-    const uint32_t x0 = __shfl_sync(kAll, k0, l), x1 = __shfl_sync(kAll, k1, l);
-    const int y0 = __shfl_sync(kAll, g0, l), y1 = __shfl_sync(kAll, g1, l);
-    *larger = above + (hit0 ? y0 : y1);
-    return hit0 ? x0 : x1;
-}
-
-// Places of the hits of a CTA's items in order of their index (item i·NT + thread): sum of the earlier counts of the (round,
-// warp) pairs. cnt holds the counts of R·NT / 32 pairs; on return the exclusive sums, and the total.
-template <int NT, int R>
-__device__ __forceinline__ int scan_counts(int *cnt, int *total) {
-    __syncthreads();   // the counts are written
-    constexpr int N = R * NT / 32, PER = (N + 31) / 32;
-    if (threadIdx.x < 32) {
-        int v[PER], sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = threadIdx.x * PER + j;
-            v[j] = i < N ? cnt[i] : 0;
-            sum += v[j];
+    // four threads a key of the list: how many are larger, how many at least as large; the r-th is where fewer than r are
+    // larger and at least r as large
+    const int r = m - above, i = threadIdx.x >> 2;
+    if (threadIdx.x < 4 * NLIST) {
+        const uint32_t k = i < in ? sh.list[i] : 0u;
+        int g = 0, e = 0;
+#pragma unroll 4
+        for (int j = threadIdx.x & 3; j < in; j += 4) {
+            g += sh.list[j] > k;
+            e += sh.list[j] >= k;
         }
-        int x = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(kAll, x, o);
-            if ((int)threadIdx.x >= o) x += y;
-        }
-        if (threadIdx.x == 31) *total = x;
-        x -= sum;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = threadIdx.x * PER + j;
-            if (i < N) cnt[i] = x;
-            x += v[j];
+        g += __shfl_xor_sync(kAll, g, 1);
+        e += __shfl_xor_sync(kAll, e, 1);
+        g += __shfl_xor_sync(kAll, g, 2);
+        e += __shfl_xor_sync(kAll, e, 2);
+        if ((threadIdx.x & 3) == 0 && i < in && g < r && e >= r) {   // equal keys write the same
+            sh.found[0] = (int)k;
+            sh.found[1] = g;
+            sh.found[2] = e;
         }
     }
     __syncthreads();
-    return *total;
+    *larger = above + sh.found[1];
+    *equal = sh.found[2] - sh.found[1];
+    return (uint32_t)sh.found[0];
+}
+
+// Places of the hits of a CTA's items in order of their index (item i·NT + thread): exclusive sums, in place, of the counts of
+// the (round, warp) pairs in cnt, N <= blockDim.x of them. Returns the total.
+template <int N>
+__device__ __forceinline__ int scan_counts(int *cnt, int *scan) {
+    __syncthreads();   // the counts are written
+    const int v = (int)threadIdx.x < N ? cnt[threadIdx.x] : 0;
+    int total;
+    const int x = block_scan_incl(v, scan, &total) - v;
+    if ((int)threadIdx.x < N) cnt[threadIdx.x] = x;
+    __syncthreads();
+    return total;
 }
 
 // Adds one to hist[bin] for the lanes with in: lanes of a warp with the same bin together.
@@ -738,14 +783,17 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int
     return nan ? 0ull : score_key(best);
 }
 
-constexpr int CT = 256, CR = 16, CLIST = 512;   // threads, scores a thread holds, pages decided by hand in shared memory
+constexpr int CT = 256, CLIST = 512;   // threads, pages decided by hand in shared memory
 // One CTA per row (s, t, g). Keys are the FP32 scores' order-preserving bits (pages that are always taken above all); tau is
 // the nsel-th largest. With E the bound of a score's error, a page above tau + 2E is taken, one below tau - 2E is not: nsel pages
 // have scores of at least tau - E, and fewer than nsel more than tau + E. The pages between are ranked by their 64-bit scores.
-__global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ SelectArgs a, int score_ctas) {
+// CR: scores a thread holds in registers, as many as the table's pages need (more are read again where they are used).
+template <int CR>
+__global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ SelectArgs a) {
     __shared__ NthKey nth;
     __shared__ int hist[2 * CT], scan[32], got[3];
-    __shared__ int order[CR * CT / 32], order_n;
+    __shared__ int order[CR * CT / 32];
+    __shared__ unsigned taken[CR * CT / 32];   // pages decided by hand, of those that registers hold
     __shared__ float red[2][CT / 32];
     __shared__ int list[CLIST];
     __shared__ unsigned long long lkey[CLIST];
@@ -774,10 +822,8 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21
     float big = 0.0f, l1 = 0.0f;
     {
-        const int sg = s * c.HKV + g, z = t * a.hg / a.zt;
-        const int used = ((have + SPAGES - 1) / SPAGES + SW * a.steps - 1) / (SW * a.steps);   // CTAs with pages
-        for (int i = tid; i < used * SW; i += CT)
-            big = fmaxf(big, __ldcg(a.peak + ((long long)z * c.ns * c.HKV + sg) * score_ctas * SW + i));
+        const float *peak = a.peak + (((long long)s * c.HKV + g) * a.zs + t * a.hg / a.zt) * a.unit_steps;
+        for (int i = tid; i < (have + SPAGES - 1) / SPAGES; i += CT) big = fmaxf(big, __ldcg(peak + i));
         for (int h = tid; h < a.G; h += CT) l1 = fmaxf(l1, __ldcg(a.l1 + (long long)st * a.H + g * a.G + h));
         for (int o = 16; o > 0; o >>= 1) {
             big = fmaxf(big, __shfl_xor_sync(kAll, big, o));
@@ -793,8 +839,9 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     uint32_t key[CR];
 #pragma unroll
     for (int i = 0; i < CR; i++) key[i] = tid + i * CT < have ? key_of(tid + i * CT, x[i]) : 0u;
-    int larger;
-    const uint32_t at = nth_key<CT, CR>(key, have, m, nth, [&](int i) { return key_of(i, __ldcg(score + i)); }, &larger);
+    for (int i = tid; i < CR * CT / 32; i += CT) taken[i] = 0;
+    int larger, equal;
+    const uint32_t at = nth_key<CT, CR>(key, have, m, nth, [&](int i) { return key_of(i, __ldcg(score + i)); }, &larger, &equal);
     for (int w = 0; w < CT / 32; w++) {
         big = fmaxf(big, red[0][w]);
         l1 = fmaxf(l1, red[1][w]);
@@ -806,6 +853,10 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     const float above = know ? tau + 2.0f * E : 3.4e38f, below = know ? tau - 2.0f * E : -INFINITY;
     // 1: taken for sure, 0: not, -1: between
     auto side = [&](int i, float y) { return always(i) || (know && y > above) ? 1 : !know || y >= below ? -1 : 0; };
+    auto decide = [&](int i, bool take) {
+        if (i >= CR * CT) score[i] = take ? INFINITY : -INFINITY;
+        else if (take) atomicOr(&taken[i >> 5], 1u << (i & 31));
+    };
     if (!full) {
         int mine = 0;
         auto look = [&](int i, float y) {
@@ -839,17 +890,15 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
                         else lnan[e] = 1;
                     }
                 }
-                __syncthreads();
-                for (int i = tid; i < nb; i += CT)
-                    if (lnan[i]) lkey[i] = 0ull;
-                __syncthreads();
             }
+            __syncthreads();
+            auto rank_key = [&](int i) { return lnan[i] ? 0ull : lkey[i]; };
             for (int i = tid; i < nb; i += CT) {
                 int better = 0;
                 if (nb > r)
                     for (int j = 0; j < nb; j++)
                         better += lkey[j] > lkey[i] || (lkey[j] == lkey[i] && list[j] < list[i]);
-                score[list[i]] = better < r ? INFINITY : -INFINITY;
+                decide(list[i], better < r);
             }
         } else {   // very many: 64-bit keys of all of them, and radix selection over these
             unsigned long long *wide = a.key + (long long)row * c.mp;
@@ -883,7 +932,7 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
                 const unsigned long long k = i < have ? wide[i] : 0ull;
                 int total;
                 const int rank = block_scan_incl(k != 0ull && k == pre, scan, &total) + eq0;
-                if (k != 0ull) score[i] = k > pre || (k == pre && rank <= left) ? INFINITY : -INFINITY;
+                if (k != 0ull) decide(i, k > pre || (k == pre && rank <= left));
                 eq0 += total;
             }
         }
@@ -896,11 +945,15 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
 #pragma unroll
         for (int i = 0; i < CR; i++) {
             const int p = i0 + i * CT + tid;
-            const bool take = p < have && (always(p) || (!full && __ldcg(score + p) > above));
+            bool take = p < have && always(p);
+            if (p < have && !full) {
+                if (i0 == 0) take = take || (know && x[i] > above) || (taken[p >> 5] >> (p & 31) & 1u);
+                else take = take || __ldcg(score + p) > above;
+            }
             hit[i] = __ballot_sync(kAll, take);
             if (lane == 0) order[i * (CT / 32) + warp] = __popc(hit[i]);
         }
-        const int total = scan_counts<CT, CR>(order, &order_n);
+        const int total = scan_counts<CR * CT / 32>(order, scan);
 #pragma unroll
         for (int i = 0; i < CR; i++) {
             const int slot = base + order[i * (CT / 32) + warp] + __popc(hit[i] & ((1u << lane) - 1u));
@@ -927,15 +980,15 @@ struct EvictArgs {
     int *len_out;
 };
 
-constexpr int ER = 16;   // slots a thread holds
 // Which slots stay, and where the movers go: one CTA per row (s, g). The threshold is the keep-th largest key; then one
 // ordered pass over the slots, ER·ET at a time: below `keep` the given-up slots are listed and their pages marked, from
-// there on the j-th staying slot becomes the source of the j-th of them. ET = 256 threads hold 4096 slots, 1024 threads 16384:
-// the smaller where the table has no more (256 rows of 2064 slots: 61 µs with 1024 threads, most of them idle).
-template <int ET>
+// there on the j-th staying slot becomes the source of the j-th of them. ET threads hold ER slots each: as few as the table's
+// slots need (256 rows of 2064 slots took 61 µs with 1024 threads of 16, most of it idle registers), at most 1024 of 16,
+// beyond which the weights are read again where they are used.
+template <int ET, int ER>
 __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArgs a) {
     __shared__ NthKey nth;
-    __shared__ int order[ER * ET / 32], eqs[ER * ET / 32], order_n, eqs_n, sh_new;
+    __shared__ int order[ER * ET / 32], scan[32], sh_new;
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
@@ -983,32 +1036,47 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
         const int p = pos ? __ldg(pos + k) : k;
         return p < a.first || p > old ? kAll : weight_key(__ldg(acc + k));
     };
-    int larger;
-    const uint32_t last = nth_key<ET, ER>(key, n, keep, nth, key_of, &larger);
-    const int need = keep - larger;   // of the keys equal to the threshold the first `need` stay
+    int larger, equal;
+    const uint32_t last = nth_key<ET, ER>(key, n, keep, nth, key_of, &larger, &equal);
+    const int need = keep - larger;   // of the `equal` keys at the threshold the first `need` stay
     int eq_base = 0, holes_n = 0, moved = 0;
     for (int i0 = 0; i0 < n; i0 += ER * ET) {
-        unsigned eq[ER], hole[ER], mover[ER];   // ballots of the warps
+        unsigned hole[ER], mover[ER];   // ballots of the warps
+        if (i0 > 0) {
 #pragma unroll
-        for (int i = 0; i < ER; i++) {
-            const int k = i0 + i * ET + tid;
-            if (i0 > 0) key[i] = k < n ? key_of(k) : 0u;
-            eq[i] = __ballot_sync(kAll, k < n && key[i] == last);
-            if (lane == 0) eqs[i * (ET / 32) + warp] = __popc(eq[i]);
+            for (int i = 0; i < ER; i++) key[i] = i0 + i * ET + tid < n ? key_of(i0 + i * ET + tid) : 0u;
         }
-        const int eq_total = scan_counts<ET, ER>(eqs, &eqs_n);
+        unsigned stays = 0;   // bit i: slot i0 + i·ET + tid
+        if (equal == need) {
+#pragma unroll
+            for (int i = 0; i < ER; i++) stays |= (unsigned)(key[i] >= last && i0 + i * ET + tid < n) << i;
+        } else {
+            unsigned eq[ER];
+#pragma unroll
+            for (int i = 0; i < ER; i++) {
+                eq[i] = __ballot_sync(kAll, i0 + i * ET + tid < n && key[i] == last);
+                if (lane == 0) order[i * (ET / 32) + warp] = __popc(eq[i]);
+            }
+            const int eq_total = scan_counts<ER * ET / 32>(order, scan);
+#pragma unroll
+            for (int i = 0; i < ER; i++) {
+                const int rank = eq_base + order[i * (ET / 32) + warp] + __popc(eq[i] & ((1u << lane) - 1u));
+                stays |= (unsigned)(i0 + i * ET + tid < n && (key[i] > last || (key[i] == last && rank < need))) << i;
+            }
+            eq_base += eq_total;
+            __syncthreads();   // the sums are read before the next counts land on them
+        }
 #pragma unroll
         for (int i = 0; i < ER; i++) {
             const int k = i0 + i * ET + tid;
-            const int rank = eq_base + eqs[i * (ET / 32) + warp] + __popc(eq[i] & ((1u << lane) - 1u));
-            const bool stay = k < n && (key[i] > last || (key[i] == last && rank < need));
+            const bool stay = stays >> i & 1u;
             hole[i] = __ballot_sync(kAll, k < keep && !stay);
             mover[i] = __ballot_sync(kAll, k >= keep && stay);
             // holes lie below keep, movers behind: their counts share a word (at most 2^14 of each at once)
             if (lane == 0) order[i * (ET / 32) + warp] = __popc(hole[i]) | __popc(mover[i]) << 16;
             if (k < keep) src[k] = -1;
         }
-        const int total = scan_counts<ET, ER>(order, &order_n);
+        const int total = scan_counts<ER * ET / 32>(order, scan);
 #pragma unroll
         for (int i = 0; i < ER; i++) {
             const int k = i0 + i * ET + tid, before = order[i * (ET / 32) + warp];
@@ -1026,7 +1094,6 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
                 if (at < keep) src[holes[at]] = k;
             }
         }
-        eq_base += eq_total;
         holes_n += total & 0xffff;
         moved += total >> 16;
         __syncthreads();   // the sums are read before the next counts land on them
@@ -1041,7 +1108,7 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
             hit[i] = __ballot_sync(kAll, p < a.pages && (flag[p] || (p == a.pages - 1 && keep % c.page)));
             if (lane == 0) order[i * (ET / 32) + warp] = __popc(hit[i]);
         }
-        const int total = scan_counts<ET, ER>(order, &order_n);
+        const int total = scan_counts<ER * ET / 32>(order, scan);
 #pragma unroll
         for (int i = 0; i < ER; i++)
             if (hit[i] >> lane & 1u)
@@ -1065,37 +1132,29 @@ __device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int 
         mn[j] = __half2half2(__ushort_as_half(0x7c00));
         mx[j] = __half2half2(__ushort_as_half(0xfc00));
     }
-    constexpr int U = 4;   // rows in flight per lane: all their loads come before the first store
-    for (int i0 = sub; i0 < rows; i0 += U * rpw) {
-        int from[U], slot[U], k[U];
-        uint4 kv[U], vv[U];
-#pragma unroll
-        for (int j = 0; j < U; j++) k[j] = i0 + j * rpw < rows ? __ldg(src + i0 + j * rpw) : -1;
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            const int pl = page_quot(c.div, max(k[j], 0));
-            from[j] = k[j] >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
-            slot[j] = from[j] >= 0 ? k[j] - pl * c.page : i0 + j * rpw;
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+        // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
+        long long ko = 0, vo = -1;
+        if (r0 + lane < rows) {
+            const int k = __ldg(src + r0 + lane), pl = page_quot(c.div, max(k, 0));
+            const int from = k >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
+            ko = from >= 0 ? row_at(from, k - pl * c.page, g, c.kp, c.kk, c.kh) : row_at(id, r0 + lane, g, c.kp, c.kk, c.kh);
+            if (from >= 0) vo = row_at(from, k - pl * c.page, g, c.vp, c.vk, c.vh);
         }
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            const bool row = live && i0 + j * rpw < rows;
-            const int rid = from[j] >= 0 ? from[j] : id;
-            if (row && (bounds || from[j] >= 0))
-                kv[j] = __ldcg(reinterpret_cast<const uint4 *>(c.K + row_at(rid, slot[j], g, c.kp, c.kk, c.kh) + ch * 8));
-            if (row && from[j] >= 0)
-                vv[j] = __ldcg(reinterpret_cast<const uint4 *>(c.V + row_at(rid, slot[j], g, c.vp, c.vk, c.vh) + ch * 8));
-        }
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            const int i = i0 + j * rpw;
-            if (!live || i >= rows) continue;
-            if (from[j] >= 0) {
-                *reinterpret_cast<uint4 *>(c.K + row_at(id, i, g, c.kp, c.kk, c.kh) + ch * 8) = kv[j];
-                *reinterpret_cast<uint4 *>(c.V + row_at(id, i, g, c.vp, c.vk, c.vh) + ch * 8) = vv[j];
+        __half *kd = c.K + row_at(id, r0, g, c.kp, c.kk, c.kh) + ch * 8, *vd = c.V + row_at(id, r0, g, c.vp, c.vk, c.vh) + ch * 8;
+        const int here = min(32, rows - r0);
+        for (int i0 = 0; i0 < here; i0 += rpw) {
+            const int i = i0 + sub;
+            const long long kr = __shfl_sync(kAll, ko, i & 31), vr = __shfl_sync(kAll, vo, i & 31);
+            if (i >= here || !live || (!bounds && vr < 0)) continue;
+            const uint4 kv = __ldcg(reinterpret_cast<const uint4 *>(c.K + kr + ch * 8));
+            if (vr >= 0) {
+                const uint4 vv = __ldcg(reinterpret_cast<const uint4 *>(c.V + vr + ch * 8));
+                *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
+                *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = vv;
             }
             if (!bounds) continue;
-            const unsigned x[4] = {kv[j].x, kv[j].y, kv[j].z, kv[j].w};
+            const unsigned x[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 mn[e] = __hmin2(mn[e], as_h2(x[e]));
@@ -1119,8 +1178,10 @@ __device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int 
 // The moves: the warps of `ctas` CTAs per row take the row's changed pages in turn. lpr lanes carry a row, 16 bytes each; the
 // bounds of a page are taken over the rows it now holds, the movers' from their sources. Every source lies at or above keep
 // and every target below, so that the order of the moves does not matter. Bound by memory: rows in and out.
-constexpr int MT = 128;
-__global__ void __launch_bounds__(MT, 6) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
+// Many warps with a row each in flight: 12 CTAs per SM took 63 µs for 8 × 8 heads, 16384 -> 8192 slots (335 MB), 6 CTAs with
+// four rows a lane 79 µs.
+constexpr int MT = 128, MCTAS = 12;
+__global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
@@ -1151,12 +1212,15 @@ size_t marks_bytes(const KvDev &c, int64_t ms, int64_t mh) {
     return ((size_t)std::max(c.ns - 1, 0) * (size_t)std::max<int64_t>(ms, 0) + (size_t)(c.HKV - 1) * (size_t)std::max<int64_t>(mh, 0) +
             (size_t)c.cap) * 4;
 }
+// One wave of CTAs, as many as shared memory lets an SM hold, and no more than there can be runs.
 template <int DP>
-int score_launch(const SelectArgs &a, const KvCall &call, dim3 grid) {
+int score_launch(const SelectArgs &a, const KvCall &call, long long most) {
     using C = ScoreCfg<DP>;
     static bool attr[kMaxDevices] = {};
+    const int smem = C::smem(a.tg), per = std::max(1, 227 * 1024 / (smem + 1024 + 64));
     G9_CU(smem_limit_once(kv_score_k<DP>, C::smem(C::TG), attr));
-    G9_CU(launch_pdl(kv_score_k<DP>, grid, dim3(SW * 32), C::smem(a.tg), call.st, a));
+    const unsigned ctas = (unsigned)std::min<long long>(most, (long long)std::min(per, 4) * call.d->sm_count);
+    G9_CU(launch_pdl(kv_score_k<DP>, dim3(ctas), dim3(SW * 32), smem, call.st, a));
     return launched("kv_score");
 }
 
@@ -1264,7 +1328,7 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     if (int e = kv_begin(c, H, sync, who, &a.c, &call)) return e;
     if (c->ns == 0 || nq <= 0 || nsel == 0) return 0;
     const long long rows = (long long)c->ns * nq * c->HKV;
-    if (rows > INT_MAX || c->ns * (long long)c->HKV > 65535)
+    if (rows > INT_MAX)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows (stream, token, head) in one call", who, rows);
     G9_TRY(kv_operand(call, Q, who, "Q"));
     G9_TRY(kv_operand(call, vis, who, "vis"));
@@ -1288,16 +1352,17 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     // a CTA reads its pages once for as many row tiles as its shared memory holds
     const long long tg = std::min<long long>(tiles, dp == 64 ? ScoreCfg<64>::TG : dp == 128 ? ScoreCfg<128>::TG : ScoreCfg<256>::TG);
     const long long zt = a.hg > tg ? a.hg : tg / a.hg * a.hg, zs = (tiles + zt - 1) / zt;
-    if (zs > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %d tokens of %d heads in one call", who, nq, H);
     a.tiles = (int)tiles;
     a.tg = (int)std::min(tg, zt);
     a.zt = (int)zt;
-    // steps of a warp: about four CTAs per SM over all (stream, head) rows, which amortises the queries
-    const long long all = (c->mp + SPAGES - 1) / SPAGES, sg = (long long)c->ns * c->HKV * zs;
-    a.steps = (int)std::max<long long>(1, all * sg / (4LL * SW * call.d->sm_count));
-    const int ctas = (int)std::max<long long>(1, (all + SW * a.steps - 1) / (SW * a.steps));
+    a.zs = (int)zs;
+    a.by_zs = page_div((int)zs);
+    a.unit_steps = std::max(1, (c->mp + SPAGES - 1) / SPAGES);
+    const long long units = (long long)c->ns * c->HKV * zs;
+    if (units * (a.unit_steps + SCOST) > INT_MAX / 2)
+        return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows of up to %d pages pass 2^30 steps in one call", who, rows, c->mp);
     const size_t score = up256((size_t)rows * c->mp * 4), key = up256((size_t)rows * c->mp * 8),
-                 l1 = up256((size_t)c->ns * nq * H * 4), peak = up256((size_t)sg * ctas * SW * 4);
+                 l1 = up256((size_t)c->ns * nq * H * 4), peak = up256((size_t)units * a.unit_steps * 4);
     void *buf = nullptr;
     unsigned *cnt = nullptr;
     G9_TRY(kv_workspace(ws, call, who, score + key + l1 + peak, 0, &buf, &cnt));
@@ -1307,12 +1372,15 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     a.l1 = (float *)((char *)buf + score + key);
     a.peak = (float *)((char *)buf + score + key + l1);
     if (c->mp > 0) {
-        const dim3 grid((unsigned)ctas, (unsigned)(c->ns * c->HKV), (unsigned)zs);
-        if (dp == 64) G9_TRY(score_launch<64>(a, call, grid));
-        else if (dp == 128) G9_TRY(score_launch<128>(a, call, grid));
-        else G9_TRY(score_launch<256>(a, call, grid));
+        const long long most = (units * (a.unit_steps + SCOST) + SW - 1) / SW;
+        if (dp == 64) G9_TRY(score_launch<64>(a, call, most));
+        else if (dp == 128) G9_TRY(score_launch<128>(a, call, most));
+        else G9_TRY(score_launch<256>(a, call, most));
     }
-    G9_CU(launch_pdl(kv_choose_k, dim3((unsigned)rows), dim3(CT), 0, call.st, a, ctas));
+    const dim3 grid((unsigned)rows);
+    if (c->mp <= 4 * CT) G9_CU(launch_pdl(kv_choose_k<4>, grid, dim3(CT), 0, call.st, a));
+    else if (c->mp <= 8 * CT) G9_CU(launch_pdl(kv_choose_k<8>, grid, dim3(CT), 0, call.st, a));
+    else G9_CU(launch_pdl(kv_choose_k<16>, grid, dim3(CT), 0, call.st, a));
     G9_TRY(launched("kv_choose"));
     const KvWrite w[1] = {{sel, (size_t)rows * nsel * 4}};
     return kv_finish(call, sync, w, 1);
@@ -1352,11 +1420,14 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     a.flag = (int *)((char *)buf + 2 * list);
     a.todo = (int *)((char *)buf + 2 * list + pages);
     a.used = (int *)((char *)buf + 2 * list + 2 * pages);
-    if (a.c.cap <= 256 * ER) G9_CU(launch_pdl(kv_rank_k<256>, dim3((unsigned)rows), dim3(256), 0, call.st, a));
-    else G9_CU(launch_pdl(kv_rank_k<1024>, dim3((unsigned)rows), dim3(1024), 0, call.st, a));
+    const dim3 grid((unsigned)rows);
+    if (a.c.cap <= 256 * 4) G9_CU(launch_pdl(kv_rank_k<256, 4>, grid, dim3(256), 0, call.st, a));
+    else if (a.c.cap <= 256 * 12) G9_CU(launch_pdl(kv_rank_k<256, 12>, grid, dim3(256), 0, call.st, a));
+    else if (a.c.cap <= 1024 * 8) G9_CU(launch_pdl(kv_rank_k<1024, 8>, grid, dim3(1024), 0, call.st, a));
+    else G9_CU(launch_pdl(kv_rank_k<1024, 16>, grid, dim3(1024), 0, call.st, a));
     G9_TRY(launched("kv_rank"));
     // a page per warp where the rows are few, else one wave of CTAs in all
-    const long long most = (a.pages + MT / 32 - 1) / (MT / 32), ctas = std::max<long long>(1, std::min(most, 6LL * call.d->sm_count / rows));
+    const long long most = (a.pages + MT / 32 - 1) / (MT / 32), ctas = std::max<long long>(1, std::min<long long>(most, (long long)MCTAS * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
     if (rows * ctas > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows in one call", who, rows);
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr));

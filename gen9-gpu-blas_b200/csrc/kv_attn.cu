@@ -1,6 +1,7 @@
 // kv_attn.cu -- attention over the paged key-value cache (gen9blas_attn_paged, include/gen9blas_kv.h): decoding and draft
 // tokens, the whole cache, a window of it or chosen pages, with the weights each slot receives on request.
 #include "kv.h"
+#include "kv_plan.cuh"
 #include "mma_sync.cuh"
 #include "sm100.cuh"
 #include <algorithm>
@@ -111,51 +112,14 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- this CTA's work. Every warp finds it for itself. All units' steps in a row are cut into equal runs of `chunk`, one
-    // a CTA, a segment of a unit at a time. A segment costs a CTA about 6 µs of latencies besides its steps (row data, first
-    // copies, merge), so that each unit is counted COST steps longer than it is, at its start: a CTA that begins a unit in
-    // the middle of its run gets that much less to read, and short units begin a run of their own. (Equal runs without it took
-    // 32.4 µs at 8 streams of 4096 keys, a whole number of CTAs per unit 27.7; 14.1 and 10.4 at one stream of 1000.)
-    int T = 0, pre = 0, outer = 0, n0 = 0;   // steps in all; before outer index `outer`; of outer index `lane`
-    if (a.sel) {
-        T = a.outer * a.inner * (a.sel_steps + C::COST);
-    } else {
-        for (int o = lane; o < a.outer; o += 32) {
-            int k0, k1;
-            const int n = outer_steps(a, o, k0, k1) + C::COST;
-            if (o == lane) n0 = n;
-            T += n * a.inner;
-        }
-        T = __reduce_add_sync(kAll, T);
-    }
-    const int b = blockIdx.x;
-    const int chunk = (int)(((unsigned)T + gridDim.x - 1) / gridDim.x + AW - 1) / AW * AW;
-    if ((long long)b * chunk >= T) return;
-    const int lo = b * chunk, hi = min(lo + chunk, T);
-    if (a.sel) {
-        const int per = a.inner * (a.sel_steps + C::COST);
-        outer = lo / per;
-        pre = outer * per;
-    } else {
-        for (int o0 = 0;; o0 += 32) {
-            int k0, k1;
-            const int n = o0 + lane < a.outer ? (o0 ? outer_steps(a, o0 + lane, k0, k1) + C::COST : n0) * a.inner : 0;
-            int x = n;
-#pragma unroll
-            for (int i = 1; i < 32; i <<= 1) {
-                const int y = __shfl_up_sync(kAll, x, i);
-                if (lane >= i) x += y;
-            }
-            const unsigned past = __ballot_sync(kAll, pre + x > lo);   // lo < T: found before the indices run out
-            if (past) {
-                const int l = __ffs(past) - 1;
-                outer = o0 + l;
-                pre += __shfl_sync(kAll, x - n, l);
-                break;
-            }
-            pre += __shfl_sync(kAll, x, 31);
-        }
-    }
+    // ---- this CTA's run of steps. Counting a segment's latencies in (about 6 µs, COST steps; see kv_plan.cuh) took 8 streams of
+    // 4096 keys from 32.4 to 26.3 µs and one stream of 1000 keys from 14.1 to 9.6.
+    const Run run = find_run(a.outer, a.inner, C::COST, AW, [&](int o) {
+        int k0, k1;
+        return outer_steps(a, o, k0, k1);
+    });
+    const int lo = run.lo, hi = run.hi, chunk = run.chunk, b = blockIdx.x;
+    int outer = run.outer, pre = run.pre;
 
     uint8_t *wring = ring + warp * NST * C::STAGE;
     const unsigned wbase = sm100::smem_u32(wring);
@@ -297,19 +261,30 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
             inv[0][0] = __shfl_sync(kAll, down, 8 * tq);
             inv[0][1] = __shfl_sync(kAll, down, 8 * tq + 4);
         } else {
-            for (int r = warp; r < ROWS; r += AW) {   // each warp prepares every fourth row
-                const bool live = r < live_rows;
-                const int src = live ? r : 0;
+            // each warp prepares every fourth row, all of them requested first
+            constexpr int RW = ROWS / AW;
+            float x[RW][DP / 32];
+#pragma unroll
+            for (int k = 0; k < RW; k++) {
+                const int r = warp + AW * k, src = r < live_rows ? r : 0;
                 const float *qp = a.Q + s * a.qs + __shfl_sync(kAll, my_t, src) * a.qt + __shfl_sync(kAll, my_h, src) * a.qh;
-                float x[DP / 32], big = 0.0f;
 #pragma unroll
                 for (int i = 0; i < DP / 64; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const int d = 64 * i + 2 * lane + j;
-                        x[2 * i + j] = live && d < c.D ? qp[d] * a.qscale : 0.0f;
-                        big = fmaxf(big, fabsf(x[2 * i + j]));
+                        x[k][2 * i + j] = r < live_rows && d < c.D ? __ldg(qp + d) : 0.0f;
                     }
+            }
+#pragma unroll
+            for (int k = 0; k < RW; k++) {
+                const int r = warp + AW * k;
+                float big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < DP / 32; i++) {
+                    x[k][i] *= a.qscale;
+                    big = fmaxf(big, fabsf(x[k][i]));
+                }
                 for (int i = 16; i > 0; i >>= 1) big = fmaxf(big, __shfl_xor_sync(kAll, big, i));
                 const int ex = up_of(big);
                 const float up = at_pow2(ex);
@@ -317,7 +292,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
 #pragma unroll
                 for (int i = 0; i < DP / 64; i++) {
                     unsigned h2, l2;
-                    at_split(x[2 * i] * up, x[2 * i + 1] * up, h2, l2);
+                    at_split(x[k][2 * i] * up, x[k][2 * i + 1] * up, h2, l2);
                     const int d = 64 * i + 2 * lane, kt = d >> 4, dd = d & 15;
                     unsigned *f = reinterpret_cast<unsigned *>(qf + (kt * NT + (r >> 3)) * 32 + (r & 7) * 4 + ((dd & 7) >> 1));
                     f[dd >> 3] = h2;
@@ -546,44 +521,60 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
         }
         __syncthreads();
         if (!sh_last) continue;
-        // The unit's last CTA adds up the slots in key order, SW at a time with their loads in flight together. (A kernel of
-        // its own for it was slower: 30.1 µs against 27.8 at 8 streams of 4096 keys, the wait between the kernels.)
+        // The unit's last CTA adds up the slots in key order, SW slots of RB rows a thread at a time with their loads in flight
+        // together. (A kernel of its own for it was slower: 30.1 µs against 27.8 at 8 streams of 4096 keys, the wait between
+        // the kernels.)
         const float *pb = a.part + (long long)slot0 * ROWS * PR;
-        constexpr int SW = 16;
-        for (int r0 = 0; r0 < live_rows; r0 += RS) {
-            const int r = min(r0 + tid / (DP / 4), ROWS - 1);
-            const long long q = __shfl_sync(kAll, my_q, r);
-            if (r >= live_rows) continue;
-            float M = -INFINITY, L = 0.0f;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int j0 = 0; j0 < nsl; j0 += SW) {
-                float2 ml[SW];
-                float4 y[SW];
+        constexpr int RB = NT == 1 ? 1 : 2, SW = 16 / RB;
+        for (int r0 = 0; r0 < live_rows; r0 += RS * RB) {
+            int r[RB];
+            long long q[RB];
+            float M[RB], L[RB];
+            float4 x[RB];
 #pragma unroll
-                for (int j = 0; j < SW; j++) {
-                    ml[j] = make_float2(-INFINITY, 0.0f);
-                    y[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (j0 + j < nsl) {
-                        const float *p = pb + ((j0 + j) * ROWS + r) * PR;
-                        ml[j] = __ldcg(reinterpret_cast<const float2 *>(p));
-                        y[j] = __ldcg(reinterpret_cast<const float4 *>(p + 4 + d));
+            for (int k = 0; k < RB; k++) {
+                r[k] = min(r0 + RS * k + tid / (DP / 4), ROWS - 1);
+                q[k] = __shfl_sync(kAll, my_q, r[k]);
+                M[k] = -INFINITY;
+                L[k] = 0.0f;
+                x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            for (int j0 = 0; j0 < nsl; j0 += SW) {
+                float2 ml[RB][SW];
+                float4 y[RB][SW];
+#pragma unroll
+                for (int k = 0; k < RB; k++)
+#pragma unroll
+                    for (int j = 0; j < SW; j++) {
+                        ml[k][j] = make_float2(-INFINITY, 0.0f);
+                        y[k][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (j0 + j < nsl && r[k] < live_rows) {
+                            const float *p = pb + ((j0 + j) * ROWS + r[k]) * PR;
+                            ml[k][j] = __ldcg(reinterpret_cast<const float2 *>(p));
+                            y[k][j] = __ldcg(reinterpret_cast<const float4 *>(p + 4 + d));
+                        }
+                    }
+#pragma unroll
+                for (int k = 0; k < RB; k++) {
+                    float mn = M[k];
+#pragma unroll
+                    for (int j = 0; j < SW; j++) mn = fmaxf(mn, ml[k][j].x);
+                    const float ref = mn == -INFINITY ? 0.0f : mn, al = exp2f(M[k] - ref);
+                    M[k] = mn;
+                    L[k] *= al;
+                    x[k] = make_float4(x[k].x * al, x[k].y * al, x[k].z * al, x[k].w * al);
+#pragma unroll
+                    for (int j = 0; j < SW; j++) {
+                        const float f = exp2f(ml[k][j].x - ref);
+                        L[k] = fmaf(ml[k][j].y, f, L[k]);
+                        x[k] = make_float4(fmaf(y[k][j].x, f, x[k].x), fmaf(y[k][j].y, f, x[k].y), fmaf(y[k][j].z, f, x[k].z),
+                                           fmaf(y[k][j].w, f, x[k].w));
                     }
                 }
-                float mn = M;
-#pragma unroll
-                for (int j = 0; j < SW; j++) mn = fmaxf(mn, ml[j].x);
-                const float ref = mn == -INFINITY ? 0.0f : mn, al = exp2f(M - ref);
-                M = mn;
-                L *= al;
-                x = make_float4(x.x * al, x.y * al, x.z * al, x.w * al);
-#pragma unroll
-                for (int j = 0; j < SW; j++) {
-                    const float f = exp2f(ml[j].x - ref);
-                    L = fmaf(ml[j].y, f, L);
-                    x = make_float4(fmaf(y[j].x, f, x.x), fmaf(y[j].y, f, x.y), fmaf(y[j].z, f, x.z), fmaf(y[j].w, f, x.w));
-                }
             }
-            paged_out(a, q, d, M, L, x);
+#pragma unroll
+            for (int k = 0; k < RB; k++)
+                if (r[k] < live_rows) paged_out(a, q[k], d, M[k], L[k], x[k]);
         }
         if (tid == 0) a.cnt[u] = 0u;   // the next call finds the counter at zero
     }
