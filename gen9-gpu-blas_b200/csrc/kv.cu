@@ -220,8 +220,10 @@ __device__ __forceinline__ __half2 as_h2(unsigned x) { return *reinterpret_cast<
 __device__ __forceinline__ unsigned as_u(__half2 x) { return *reinterpret_cast<const unsigned *>(&x); }
 
 // One CTA per (page that may be touched, head, stream); its warps take the page's new rows in turn, a lane four elements
-// (or two times four, D > 128) of each row, and keep the elements' least and largest value for the bounds.
-__global__ void __launch_bounds__(256, 4) kv_append_k(const __grid_constant__ AppendArgs a) {
+// (or two times four, D > 128) of each row, and keep the elements' least and largest value for the bounds. Bound by memory:
+// the rows read once in FP32 and written once in FP16. Two rows of a warp in flight at five CTAs per SM: 18.5 µs for 81 MB (four
+// rows at three CTAs 23.4, one row at six 19.7).
+__global__ void __launch_bounds__(256, 5) kv_append_k(const __grid_constant__ AppendArgs a) {
     __shared__ uint2 red[8][2][2][32];   // [warp][least, largest][four-element group of the lane][lane]
     pdl_next();
     pdl_wait();
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(256, 4) kv_append_k(const __grid_constant__ Ap
     for (int j = 0; j < 2; j++) {
         const int d = 4 * lane + 128 * j;
         if (d >= c.D) break;
-#pragma unroll 4
+#pragma unroll 2
         for (int r = warp; r < rows; r += nw) {
             const uint2 kv = half4(row4(ksrc + (t0 + r) * a.kt + d, a.v4)), vv = half4(row4(vsrc + (t0 + r) * a.vt + d, a.v4));
             *reinterpret_cast<uint2 *>(kd + (long long)(i0 + r) * c.kk + d) = kv;
@@ -342,7 +344,8 @@ __device__ __forceinline__ void bulk_row(void *dst, const void *src, unsigned by
 }
 constexpr uint64_t SWAIT_NS = 2000000000ull;   // a row that has not landed after 2 s is an error
 constexpr int SCOST = 8;   // steps that a CTA reads in the time of a segment's latencies
-constexpr int SW = 4, SPAGES = 16, SNST = 3;   // warps of a CTA, pages of a step, stages of a warp's ring
+constexpr int SW = 4, SPAGES = 16, SNST = 2;   // warps of a CTA, pages of a step, stages of a warp's ring: two, so that an SM
+// holds 12 warps (D = 128), because a step computes about as long as its copy takes (46.7 µs with three stages, 41.2 with two)
 template <int DP>
 struct ScoreCfg {
     static constexpr int PITCH = DP * 2 * 2 + 16;                   // a page's lower and upper row; 16 bytes more spread the banks
@@ -429,12 +432,11 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
         for (int tile0 = z0; tile0 < z1 && ok; tile0 += a.tg) {
             const int ntile = min(a.tg, z1 - tile0);
             if (tile0 > z0) __syncthreads();   // every warp has left the last tiles' fragments
-            int ids[SNST - 1];
+            int ids[SNST];   // page numbers of the steps i .. i + SNST - 1; the last is the next to be copied
 #pragma unroll
-            for (int i = 0; i < SNST - 1; i++) ids[i] = id_of(i);
+            for (int i = 0; i < SNST; i++) ids[i] = id_of(i);
 #pragma unroll
             for (int i = 0; i < SNST - 1; i++) copy(i, ids[i]);
-            int next = id_of(SNST - 1), now = ids[0], after = ids[1];
             // ---- query fragments: a warp prepares every fourth row of the tiles
             for (int r = warp; r < ntile * 8; r += SW) {
                 const int tile = tile0 + (r >> 3), t = tile / a.hg, h = (tile - t * a.hg) * 8 + (r & 7);
@@ -485,9 +487,9 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
                     ok = false;
                     break;
                 }
-                copy(i + SNST - 1, next);   // into the stage before this one, which every lane has left
+                copy(i + SNST - 1, ids[SNST - 1]);   // into the stage before this one, which every lane has left
                 const int step = sb + warp + SW * i, p = step * SPAGES + gq;
-                const bool in0 = __shfl_sync(kAll, now, gq) >= 0, in1 = __shfl_sync(kAll, now, gq + 8) >= 0;
+                const bool in0 = __shfl_sync(kAll, ids[0], gq) >= 0, in1 = __shfl_sync(kAll, ids[0], gq + 8) >= 0;
                 float top[2] = {-INFINITY, -INFINITY};
                 __half2 pk0 = __half2half2(__ushort_as_half(0)), pk1 = pk0;
                 bool wild = false;
@@ -546,9 +548,9 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
                     const float pk = wild ? INFINITY : __half2float(__ushort_as_half((unsigned short)top16));
                     peaks[step] = tile0 > z0 ? fmaxf(peaks[step], pk) : pk;
                 }
-                now = after;
-                after = next;
-                next = id_of(i + SNST);
+#pragma unroll
+                for (int k = 0; k + 1 < SNST; k++) ids[k] = ids[k + 1];
+                ids[SNST - 1] = id_of(i + SNST);
                 __syncwarp();   // every lane has read this stage
             }
         }
