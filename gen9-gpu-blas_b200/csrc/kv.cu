@@ -1121,91 +1121,103 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
     if (tid == 0) a.used[2 * row + 1] = base;
 }
 
-// The rows of one page (page id of the pool, its first `rows` slots; src: their sources or -1), by one warp.
-__device__ __forceinline__ void move_page(const EvictArgs &a, int s, int g, int id, int rows, const int *src, int lpr) {
-    const KvDev &c = a.c;
-    const int lane = threadIdx.x & 31;
-    const int rpw = 32 / lpr, sub = lane / lpr, ch = lane - sub * lpr;
-    const bool live = ch * 8 < c.D;
-    const bool bounds = c.bounds != nullptr;
-    __half2 mn[4], mx[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        mn[j] = __half2half2(__ushort_as_half(0x7c00));
-        mx[j] = __half2half2(__ushort_as_half(0xfc00));
-    }
-    for (int r0 = 0; r0 < rows; r0 += 32) {
-        // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
-        long long ko = 0, vo = -1;
-        if (r0 + lane < rows) {
-            const int k = __ldg(src + r0 + lane), pl = page_quot(c.div, max(k, 0));
-            const int from = k >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
-            ko = from >= 0 ? row_at(from, k - pl * c.page, g, c.kp, c.kk, c.kh) : row_at(id, r0 + lane, g, c.kp, c.kk, c.kh);
-            if (from >= 0) vo = row_at(from, k - pl * c.page, g, c.vp, c.vk, c.vh);
-        }
-        __half *kd = c.K + row_at(id, r0, g, c.kp, c.kk, c.kh) + ch * 8, *vd = c.V + row_at(id, r0, g, c.vp, c.vk, c.vh) + ch * 8;
-        const int here = min(32, rows - r0);
-        for (int i0 = 0; i0 < here; i0 += rpw) {
-            const int i = i0 + sub;
-            const long long kr = __shfl_sync(kAll, ko, i & 31), vr = __shfl_sync(kAll, vo, i & 31);
-            if (i >= here || !live || (!bounds && vr < 0)) continue;
-            const uint4 kv = __ldcg(reinterpret_cast<const uint4 *>(c.K + kr + ch * 8));
-            if (vr >= 0) {
-                const uint4 vv = __ldcg(reinterpret_cast<const uint4 *>(c.V + vr + ch * 8));
-                *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
-                *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = vv;
-            }
-            if (!bounds) continue;
-            const unsigned x[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                mn[e] = __hmin2(mn[e], as_h2(x[e]));
-                mx[e] = __hmax2(mx[e], as_h2(x[e]));
-            }
-        }
-    }
-    if (!bounds) return;
-    for (int o = lpr; o < 32; o <<= 1)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            mn[j] = __hmin2(mn[j], as_h2(__shfl_xor_sync(kAll, as_u(mn[j]), o)));
-            mx[j] = __hmax2(mx[j], as_h2(__shfl_xor_sync(kAll, as_u(mx[j]), o)));
-        }
-    if (sub || !live) return;
-    __half *b = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D + ch * 8;
-    *reinterpret_cast<uint4 *>(b) = make_uint4(as_u(mn[0]), as_u(mn[1]), as_u(mn[2]), as_u(mn[3]));
-    *reinterpret_cast<uint4 *>(b + c.D) = make_uint4(as_u(mx[0]), as_u(mx[1]), as_u(mx[2]), as_u(mx[3]));
-}
-
-// The moves: the warps of `ctas` CTAs per row take the row's changed pages in turn. lpr lanes carry a row, 16 bytes each; the
-// bounds of a page are taken over the rows it now holds, the movers' from their sources. Every source lies at or above keep
-// and every target below, so that the order of the moves does not matter. Bound by memory: rows in and out.
-// Many warps with a row each in flight: 12 CTAs per SM took 63 µs for 8 × 8 heads, 16384 -> 8192 slots (335 MB), 6 CTAs with
-// four rows a lane 79 µs.
+// The moves: the CTAs of a row (`ctas` of them) take its changed pages in turn, a page to `team` warps (1 or all four), which
+// take its rows 32 at a time; lpr lanes carry a row, 16 bytes each. The bounds of a page are taken over the rows it now holds, the
+// movers' from their sources. Every source lies at or above keep and every target below, so that the order of the moves does
+// not matter. Bound by memory, rows in and out: many warps with a row each in flight -- 12 CTAs per SM took 63 µs for 8 × 8
+// heads, 16384 -> 8192 slots in pages of 32 (335 MB), 6 CTAs with four rows a lane 79 µs, all warps on one page 82 µs. Pages
+// of more than 32 slots take the whole CTA, or 64 rows come one after the other.
 constexpr int MT = 128, MCTAS = 12;
-__global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr) {
+__global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr, int team) {
+    __shared__ uint4 red[MT / 32][2][32];   // [warp][least, largest][lane]
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const int lane = threadIdx.x & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row = blockIdx.x / ctas, part = blockIdx.x - row * ctas;
     const int s = row / c.HKV, g = row - s * c.HKV, keep = a.keep;
-    if (part == 0 && g == 0 && threadIdx.x == 0) a.len_out[s] = min(a.used[2 * row], keep);
-    const int todo = a.used[2 * row + 1];
-    for (int w = part * (MT / 32) + (threadIdx.x >> 5); w < todo; w += ctas * (MT / 32)) {
+    if (part == 0 && g == 0 && tid == 0) a.len_out[s] = min(a.used[2 * row], keep);
+    const int todo = a.used[2 * row + 1], teams = MT / 32 / team, mate = warp % team;
+    const int rpw = 32 / lpr, sub = lane / lpr, ch = lane - sub * lpr;   // rows of a warp at once, this lane's row, its 16 bytes
+    const bool live = ch * 8 < c.D, bounds = c.bounds != nullptr;
+    for (int w = part * teams + warp / team; w < todo; w += ctas * teams) {
         const int place = a.todo[(long long)row * a.pages + w];
         const int k0 = place * c.page, rows = min(c.page, keep - k0);
         const int *src = a.src + (long long)row * keep + k0;
         const int id = page_id(c.table, c.ts, s, place, c.mp, c.n_pages);
         float *acc = a.acc + s * a.ms + g * a.mh;
         int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
-        for (int i = lane; i < rows; i += 32) {
+        for (int i = mate * 32 + lane; i < rows; i += team * 32) {
             const int k = src[i];
             if (k < 0) continue;
             acc[k0 + i] = acc[k];
             if (pos) pos[k0 + i] = pos[k];
         }
-        if (id >= 0) move_page(a, s, g, id, rows, src, lpr);
+        if (id < 0) continue;
+        __half2 mn[4], mx[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            mn[j] = __half2half2(__ushort_as_half(0x7c00));
+            mx[j] = __half2half2(__ushort_as_half(0xfc00));
+        }
+        for (int r0 = mate * 32; r0 < rows; r0 += team * 32) {
+            // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
+            long long ko = 0, vo = -1;
+            if (r0 + lane < rows) {
+                const int k = __ldg(src + r0 + lane), pl = page_quot(c.div, max(k, 0));
+                const int from = k >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
+                ko = from >= 0 ? row_at(from, k - pl * c.page, g, c.kp, c.kk, c.kh) : row_at(id, r0 + lane, g, c.kp, c.kk, c.kh);
+                if (from >= 0) vo = row_at(from, k - pl * c.page, g, c.vp, c.vk, c.vh);
+            }
+            __half *kd = c.K + row_at(id, r0, g, c.kp, c.kk, c.kh) + ch * 8, *vd = c.V + row_at(id, r0, g, c.vp, c.vk, c.vh) + ch * 8;
+            const int here = min(32, rows - r0);
+            for (int i0 = 0; i0 < here; i0 += rpw) {
+                const int i = i0 + sub;
+                const long long kr = __shfl_sync(kAll, ko, i & 31), vr = __shfl_sync(kAll, vo, i & 31);
+                if (i >= here || !live || (!bounds && vr < 0)) continue;
+                const uint4 kv = __ldcg(reinterpret_cast<const uint4 *>(c.K + kr + ch * 8));
+                if (vr >= 0) {
+                    const uint4 vv = __ldcg(reinterpret_cast<const uint4 *>(c.V + vr + ch * 8));
+                    *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
+                    *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = vv;
+                }
+                if (!bounds) continue;
+                const unsigned x[4] = {kv.x, kv.y, kv.z, kv.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    mn[e] = __hmin2(mn[e], as_h2(x[e]));
+                    mx[e] = __hmax2(mx[e], as_h2(x[e]));
+                }
+            }
+        }
+        if (!bounds) continue;
+        for (int o = lpr; o < 32; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                mn[j] = __hmin2(mn[j], as_h2(__shfl_xor_sync(kAll, as_u(mn[j]), o)));
+                mx[j] = __hmax2(mx[j], as_h2(__shfl_xor_sync(kAll, as_u(mx[j]), o)));
+            }
+        uint4 lo = make_uint4(as_u(mn[0]), as_u(mn[1]), as_u(mn[2]), as_u(mn[3]));
+        uint4 hi = make_uint4(as_u(mx[0]), as_u(mx[1]), as_u(mx[2]), as_u(mx[3]));
+        if (team > 1) {   // the whole CTA: every warp is here
+            red[warp][0][lane] = lo;
+            red[warp][1][lane] = hi;
+            __syncthreads();
+            if (warp == 0)
+                for (int i = 1; i < team; i++) {
+                    const uint4 x = red[i][0][lane], y = red[i][1][lane];
+                    lo = make_uint4(as_u(__hmin2(as_h2(lo.x), as_h2(x.x))), as_u(__hmin2(as_h2(lo.y), as_h2(x.y))),
+                                    as_u(__hmin2(as_h2(lo.z), as_h2(x.z))), as_u(__hmin2(as_h2(lo.w), as_h2(x.w))));
+                    hi = make_uint4(as_u(__hmax2(as_h2(hi.x), as_h2(y.x))), as_u(__hmax2(as_h2(hi.y), as_h2(y.y))),
+                                    as_u(__hmax2(as_h2(hi.z), as_h2(y.z))), as_u(__hmax2(as_h2(hi.w), as_h2(y.w))));
+                }
+            __syncthreads();   // the partial bounds are read before the next page's land on them
+        }
+        if (mate == 0 && sub == 0 && live) {
+            __half *b = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D + ch * 8;
+            *reinterpret_cast<uint4 *>(b) = lo;
+            *reinterpret_cast<uint4 *>(b + c.D) = hi;
+        }
     }
 }
 
@@ -1428,11 +1440,12 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     else if (a.c.cap <= 1024 * 8) G9_CU(launch_pdl(kv_rank_k<1024, 8>, grid, dim3(1024), 0, call.st, a));
     else G9_CU(launch_pdl(kv_rank_k<1024, 16>, grid, dim3(1024), 0, call.st, a));
     G9_TRY(launched("kv_rank"));
-    // a page per warp where the rows are few, else one wave of CTAs in all
-    const long long most = (a.pages + MT / 32 - 1) / (MT / 32), ctas = std::max<long long>(1, std::min<long long>(most, (long long)MCTAS * call.d->sm_count / rows));
+    const int team = c->page > 32 ? MT / 32 : 1, teams = MT / 32 / team;
+    // a page per team where the rows are few, else one wave of CTAs in all
+    const long long ctas = std::max<long long>(1, std::min<long long>((a.pages + teams - 1) / teams, (long long)MCTAS * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
     if (rows * ctas > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows in one call", who, rows);
-    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr));
+    G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
     const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};

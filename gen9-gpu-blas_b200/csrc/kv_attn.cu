@@ -46,18 +46,23 @@ __device__ __forceinline__ void cp16(unsigned dst, const void *src, int bytes) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
-template <int DP, int NT>
+template <int DP, int NT, bool W>
 struct PagedCfg {
     static constexpr int ROWS = 8 * NT;                         // query rows of a unit
     static constexpr int STAGE = AKEYS * DP * 2 * 2;            // bytes of a warp's stage: K rows, V rows
-    static constexpr int NST = DP == 64 ? 6 : 3;
+    // resident CTAs of an SM, held to by registers and shared memory: as many warps as fit serve the latencies of a step better
+    // than deeper rings of fewer (one row tile, D 128: three CTAs of two stages against two of three 24.9 and 26.2 µs at 8
+    // streams of 4096 keys, 31.5 and 35.5 at 64 chosen pages of 16; D 64: four of three against two of six 79 and 107 µs at
+    // 2 streams of 131071 keys)
+    // W, with weights: the addresses of the scores take the registers of a third CTA (65 against 52 µs at 8 streams of 8192 keys).
+    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? (NT == 1 && !W ? 3 : 2) : NT == 1 ? 4 : NT == 2 ? 3 : 2;
+    static constexpr int NST = DP == 64 ? (NT == 1 ? 3 : NT == 2 ? 4 : 6) : CTAS == 3 ? 2 : 3;
     static constexpr int RING = AW * NST * STAGE;
     static constexpr int QF = NT == 1 ? 0 : DP / 16 * NT * 32 * 16;   // query fragments, hi and lo (NT = 1: registers)
     static constexpr int KIDX = AW * NST * AKEYS * 4;
     static constexpr int ROWOFF = AW * AKEYS * 16;
     static constexpr int SMEM = RING + QF + KIDX + ROWOFF + ROWS * 4;
-    static constexpr int CTAS = DP == 256 ? 1 : 2;
-    static constexpr int COST = DP == 64 ? 32 : 16;             // steps that a CTA reads in the time of a segment's latencies
+    static constexpr int COST = 16;                                          // steps that a CTA reads in the time of a segment's latencies
 };
 
 // Steps of one outer index: its slots [k0, k1) from the first visible one on, held to a multiple of a step; at least one,
@@ -96,9 +101,9 @@ __device__ __forceinline__ void paged_out(const PagedArgs &a, long long q, int d
     }
 }
 
-template <int DP, int NT>
-__global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(const __grid_constant__ PagedArgs a) {
-    using C = PagedCfg<DP, NT>;
+template <int DP, int NT, bool W>
+__global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged_k(const __grid_constant__ PagedArgs a) {
+    using C = PagedCfg<DP, NT, W>;
     constexpr int ROWS = C::ROWS, NST = C::NST, KT = DP / 16, PITCH = DP * 2;
     extern __shared__ __align__(128) uint8_t pa_sm[];
     __shared__ bool sh_last;
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT>::CTAS) attn_paged_k(
                 for (int j = 0; j < 2; j++) {
                     const float x0 = ka < see[nt][j] && ka >= from[nt][j] ? sc[nt][j] * inv[nt][j] : -INFINITY;
                     const float x1 = kc < see[nt][j] && kc >= from[nt][j] ? sc[nt][2 + j] * inv[nt][j] : -INFINITY;
-                    if (a.score) {
+                    if constexpr (W) {
                         const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
                         float *sr = a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
                         if (r < live_rows && at0 < k1) sr[at0] = x0;
@@ -642,35 +647,41 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
     }
 }
 
-template <int DP, int NT>
-int paged_either(const PagedArgs &a, const KvCall &call, bool plan, int *ctas) {
-    using C = PagedCfg<DP, NT>;
+template <int DP, int NT, bool W>
+int paged_one(const PagedArgs &a, const KvCall &call, bool plan, int *ctas) {
+    using C = PagedCfg<DP, NT, W>;
     static bool attr[kMaxDevices] = {};
     static int occ[kMaxDevices] = {};
     if (plan) {   // the resident CTAs of the device
-        G9_CU(smem_limit_once(attn_paged_k<DP, NT>, C::SMEM, attr));
+        G9_CU(smem_limit_once(attn_paged_k<DP, NT, W>, C::SMEM, attr));
         if (!occ[call.d->dev])
-            G9_CU(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ[call.d->dev], attn_paged_k<DP, NT>, AW * 32, C::SMEM));
+            G9_CU(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ[call.d->dev], attn_paged_k<DP, NT, W>, AW * 32, C::SMEM));
         *ctas = std::max(occ[call.d->dev], 1) * call.d->sm_count;
         return 0;
     }
-    G9_CU(launch_pdl(attn_paged_k<DP, NT>, dim3((unsigned)*ctas), dim3(AW * 32), C::SMEM, call.st, a));
+    G9_CU(launch_pdl(attn_paged_k<DP, NT, W>, dim3((unsigned)*ctas), dim3(AW * 32), C::SMEM, call.st, a));
     return launched("attn_paged");
 }
 
-int paged(int dp, int nt, const PagedArgs &a, const KvCall &call, bool plan, int *ctas) {
+template <int DP, int NT>
+int paged_either(const PagedArgs &a, const KvCall &call, bool weights, bool plan, int *ctas) {
+    return weights ? paged_one<DP, NT, true>(a, call, plan, ctas) : paged_one<DP, NT, false>(a, call, plan, ctas);
+}
+
+// The kernel of a padded head size and a number of 8-row tiles; plan: only its resident CTAs.
+int paged(int dp, int nt, const PagedArgs &a, const KvCall &call, bool weights, bool plan, int *ctas) {
     if (dp == 64) {
-        if (nt == 1) return paged_either<64, 1>(a, call, plan, ctas);
-        if (nt == 2) return paged_either<64, 2>(a, call, plan, ctas);
-        return paged_either<64, 4>(a, call, plan, ctas);
+        if (nt == 1) return paged_either<64, 1>(a, call, weights, plan, ctas);
+        if (nt == 2) return paged_either<64, 2>(a, call, weights, plan, ctas);
+        return paged_either<64, 4>(a, call, weights, plan, ctas);
     }
     if (dp == 128) {
-        if (nt == 1) return paged_either<128, 1>(a, call, plan, ctas);
-        if (nt == 2) return paged_either<128, 2>(a, call, plan, ctas);
-        return paged_either<128, 4>(a, call, plan, ctas);
+        if (nt == 1) return paged_either<128, 1>(a, call, weights, plan, ctas);
+        if (nt == 2) return paged_either<128, 2>(a, call, weights, plan, ctas);
+        return paged_either<128, 4>(a, call, weights, plan, ctas);
     }
-    if (nt == 1) return paged_either<256, 1>(a, call, plan, ctas);
-    return paged_either<256, 2>(a, call, plan, ctas);
+    if (nt == 1) return paged_either<256, 1>(a, call, weights, plan, ctas);
+    return paged_either<256, 2>(a, call, weights, plan, ctas);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -721,7 +732,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     const int nt = rows <= 8 ? 1 : rows <= 16 || dp == 256 ? 2 : 4;
     const long long tiles = (rows + 8 * nt - 1) / (8 * nt), outer = (long long)c->ns * (sel ? nq : 1);
     // never more steps than this; they and the (s, t, h) rows are counted in 32 bits
-    const long long per = (sel ? a.sel_steps : (a.c.cap + AKEYS - 1) / AKEYS + 1) + (dp == 64 ? 32 : 16);
+    const long long per = (sel ? a.sel_steps : (a.c.cap + AKEYS - 1) / AKEYS + 1) + PagedCfg<64, 1, false>::COST;
     if ((__int128)outer * tiles * c->HKV * per > INT_MAX / 2 || (__int128)c->ns * nq * H > INT_MAX)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld (stream, token) rows of up to %lld slots pass 2^30 steps in one call", who,
                     (long long)c->ns * nq, (long long)per * AKEYS);
@@ -735,7 +746,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     a.q2 = ((uintptr_t)Q & 7) == 0 && ((qt | qh | qs) & 1) == 0;
     const long long units = outer * a.inner;
     int ctas = 1;
-    G9_TRY(paged(dp, nt, a, call, true, &ctas));
+    G9_TRY(paged(dp, nt, a, call, acc != nullptr, true, &ctas));
     // never more CTAs than steps there can be
     ctas = (int)std::min<long long>(ctas, (units * per + AW - 1) / AW);
     const size_t part = up256((size_t)(ctas + units) * 8 * nt * (dp + 4) * 4);
@@ -752,7 +763,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
         a.lse2 = (float *)((char *)buf + part);
         a.score = (float *)((char *)buf + part + lse2);
     }
-    G9_TRY(paged(dp, nt, a, call, false, &ctas));
+    G9_TRY(paged(dp, nt, a, call, acc != nullptr, false, &ctas));
     if (acc && a.score_row > 0) {
         const long long sg = (long long)c->ns * c->HKV;
         if (sg > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: weights of %lld (stream, head) rows in one call", who, sg);
