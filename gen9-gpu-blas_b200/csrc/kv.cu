@@ -170,6 +170,8 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
     return 0;
 }
 
+int kv_too_large(const char *who) { return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s: the call's workspace passes 2^46 bytes", who); }
+
 int kv_finish(const KvCall &call, int sync, const KvWrite *w, int n) {
     if (call.capturing) {
         // a replay writes without passing here: later calls of this library treat any range as possibly being written
@@ -1375,6 +1377,7 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     const long long units = (long long)c->ns * c->HKV * zs;
     if (units * (a.unit_steps + SCOST) > INT_MAX / 2)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows of up to %d pages pass 2^30 steps in one call", who, rows, c->mp);
+    if ((__int128)rows * c->mp * 12 + (__int128)c->ns * nq * H * 4 > kKvMost) return kv_too_large(who);
     const size_t score = up256((size_t)rows * c->mp * 4), key = up256((size_t)rows * c->mp * 8),
                  l1 = up256((size_t)c->ns * nq * H * 4), peak = up256((size_t)units * a.unit_steps * 4);
     void *buf = nullptr;
@@ -1411,7 +1414,7 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     if (c->ns == 0) return 0;
     G9_TRY(kv_operand(call, len, who, "len"));
     G9_TRY(kv_operand(call, len_out, who, "len_out"));
-    G9_TRY(kv_operand(call, acc, who, "acc"));
+    if (a.c.cap > 0) G9_TRY(kv_operand(call, acc, who, "acc"));
     if (pos) G9_TRY(kv_operand(call, pos, who, "pos"));
     const long long rows = (long long)c->ns * c->HKV;
     const int keep_in = std::min(keep, a.c.cap);        // no stream holds more
@@ -1427,6 +1430,7 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     void *buf = nullptr;
     unsigned *cnt = nullptr;
     a.pages = (a.keep - 1) / c->page + 1;
+    if ((__int128)rows * (a.keep + a.pages) * 8 > kKvMost) return kv_too_large(who);
     const size_t list = up256((size_t)rows * a.keep * 4), pages = up256((size_t)rows * a.pages * 4);
     G9_TRY(kv_workspace(ws, call, who, 2 * list + 2 * pages + up256((size_t)rows * 8), 0, &buf, &cnt));
     a.src = (int *)buf;
@@ -1444,7 +1448,6 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     // a page per team where the rows are few, else one wave of CTAs in all
     const long long ctas = std::max<long long>(1, std::min<long long>((a.pages + teams - 1) / teams, (long long)MCTAS * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
-    if (rows * ctas > INT_MAX) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %lld rows in one call", who, rows);
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);

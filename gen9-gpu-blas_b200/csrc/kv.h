@@ -51,6 +51,9 @@ int kv_operand(const KvCall &call, const void *p, const char *who, const char *n
 // The workspace of a call: at least `bytes` (NULL allowed for 0) and `counters` zeroed words.
 int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t bytes, size_t counters, void **buf,
                  unsigned **cnt);
+// Workspaces past this are refused as out of memory, so that sizes do not overflow.
+constexpr long long kKvMost = 1LL << 46;
+int kv_too_large(const char *who);
 // Ends a call: waits if sync, else records what was written for the no-wait ledger.
 struct KvWrite {
     const void *p;

@@ -749,25 +749,26 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     G9_TRY(paged(dp, nt, a, call, acc != nullptr, true, &ctas));
     // never more CTAs than steps there can be
     ctas = (int)std::min<long long>(ctas, (units * per + AW - 1) / AW);
+    if (acc && (long long)c->ns * c->HKV > 65535)
+        return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: weights of %lld (stream, head) rows in one call", who, (long long)c->ns * c->HKV);
+    if (((__int128)ctas + units) * 8 * nt * (dp + 4) * 4 > kKvMost) return kv_too_large(who);
     const size_t part = up256((size_t)(ctas + units) * 8 * nt * (dp + 4) * 4);
     const long long heads = (long long)c->ns * nq * H;
     a.score_row = ((sel ? (long long)a.nsel * c->page : a.c.cap) + 3) / 4 * 4;   // rows of whole float4
     const size_t lse2 = acc ? up256((size_t)heads * 4) : 0;
-    if (acc && (__int128)heads * a.score_row * 4 > ((__int128)1 << 46))
-        return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s: weights of %lld rows of %lld slots", who, heads, a.score_row);
+    if (acc && (__int128)heads * a.score_row * 4 > kKvMost) return kv_too_large(who);
     const size_t score = acc ? (size_t)heads * a.score_row * 4 : 0;
     void *buf = nullptr;
     G9_TRY(kv_workspace(ws, call, who, part + lse2 + score, (size_t)units, &buf, &a.cnt));
     a.part = (float *)buf;
+    if (c->n_pages == 0) a.c.K = a.c.V = (__half *)buf;   // named by copies of no bytes
     if (acc) {
         a.lse2 = (float *)((char *)buf + part);
         a.score = (float *)((char *)buf + part + lse2);
     }
     G9_TRY(paged(dp, nt, a, call, acc != nullptr, false, &ctas));
     if (acc && a.score_row > 0) {
-        const long long sg = (long long)c->ns * c->HKV;
-        if (sg > 65535) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: weights of %lld (stream, head) rows in one call", who, sg);
-        const dim3 grid(sel ? 1u : (unsigned)((a.c.cap + 1023) / 1024), (unsigned)sg);
+        const dim3 grid(sel ? 1u : (unsigned)((a.c.cap + 1023) / 1024), (unsigned)(c->ns * c->HKV));
         const int v4 = ((uintptr_t)acc & 15) == 0 && ((ms | mh) & 3) == 0;
         G9_CU(launch_pdl(kv_weigh_k, grid, dim3(256), 0, call.st, a, acc, (long long)ms, (long long)mh, v4));
         G9_TRY(launched("kv_weigh"));

@@ -140,6 +140,10 @@ CASES = [   # lens, page, heads, group, D, tokens, window, layout
     ([64, 200], 48, 1, 5, 8, 13, 10, "phsd"),
     ([200] * 40, 16, 2, 4, 64, 1, 0, "phsd"),       # more units than CTAs split evenly over
     ([2000, 0, 0, 5, 0, 1999], 16, 4, 4, 128, 1, 0, "phsd"),
+    ([60], 16, 1, 80, 64, 1, 0, "phsd"),            # one key-value head under 80 query heads
+    ([300], 32, 2, 2, 64, 40, 0, "pshd"),           # a short prompt in one call
+    ([3 * i % 41 for i in range(100)], 8, 2, 4, 64, 1, 0, "phsd"),
+    ([70, 9, 33], 8, 1, 3, 200, 2, 12, "both"),
 ]
 
 
@@ -546,6 +550,44 @@ def test_calls_on_several_streams(kv):
     for q, got in zip(qs, outs):
         attend_close(got, kv_ref.attend(host, q.cpu().numpy(), [900, 700]), 64)
     assert kv._get_stream() is None
+
+
+def test_nothing_to_do(kv):
+    """No streams, no tokens, no pages, no pool: empty or zero results, nothing read."""
+    z = dict(device="cuda", dtype=torch.float16)
+    K = torch.zeros(0, 2, 16, 64, **z)
+    b = torch.zeros(0, 2, 2, 64, **z)
+    q = torch.randn(3, 2, 4, 64, device="cuda")
+    for table in (torch.full((3, 5), 7, dtype=torch.int32, device="cuda"), torch.zeros(3, 0, dtype=torch.int32, device="cuda")):
+        cache = kv.PagedKV(K, K, table, bounds=b)
+        acc = torch.ones(3, 2, cache.slots, device="cuda")
+        out, lse = cache.attend(q, ints([50, 0, 3]), lse=True, acc=acc)
+        assert not out.any() and torch.isneginf(lse).all() and (acc == 1).all()
+        got = cache.select(q, ints([50, 0, 3]), 3).cpu().numpy()
+        have = np.minimum([[50, 51], [0, 1], [3, 4]], cache.slots)
+        assert np.array_equal((got >= 0).sum(-1), np.minimum(-(-have // 16), 3)[:, :, None].repeat(2, 2))
+        assert cache.append(q[:, :, :2], q[:, :, :2], ints([0, 1, 2]), wait=True) is False
+        assert cache.evict(ints([60, 2, 9]), 8, acc).tolist() == [min(8, cache.slots), min(2, cache.slots), min(8, cache.slots)]
+    K = torch.randn(4, 2, 16, 64, **z)
+    none = kv.PagedKV(K, K, torch.zeros(0, 4, dtype=torch.int32, device="cuda"))
+    assert none.attend(q[:0], ints([])).shape == (0, 2, 4, 64)
+    one = kv.PagedKV(K, K, ints([[1, 2]]))
+    assert one.attend(q[:1, :0], ints([9])).shape == (1, 0, 4, 64)
+
+
+def test_workspace_of_its_own(kv):
+    """A workspace grows with the calls, serves several caches in turn and ends without its caches."""
+    rng = np.random.default_rng(44)
+    ws = kv.Workspace()
+    for n, D in ((50, 64), (4000, 128), (100, 256)):
+        host, K, V, table, _ = make(rng, [n, n // 2], 16, 2, D)
+        q = rng.standard_normal((2, 1, 8, D)).astype(np.float32)
+        acc = torch.zeros(2, 2, table.shape[1] * 16, device="cuda")
+        got = kv.PagedKV(K, V, table, workspace=ws).attend(torch.from_numpy(q).cuda(), ints([n, n // 2]), acc=acc, lse=True)
+        attend_close(got, kv_ref.attend(host, q, [n, n // 2]), D)
+    ws.free()
+    ws.free()
+    assert ws.handle is None
 
 
 def test_refusals_on_the_device(kv, gpu_lib):
