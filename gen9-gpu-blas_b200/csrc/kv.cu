@@ -72,7 +72,7 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     k->div = page_div(c->page);
     if (int e = begin_op()) return e;
     call->d = dev_state();
-    call->st = stream();
+    call->st = c->stream ? (cudaStream_t)c->stream : stream();
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     G9_CU(cudaStreamIsCapturing(call->st, &cs));
     call->capturing = cs != cudaStreamCaptureStatusNone;
@@ -1248,8 +1248,6 @@ size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 extern "C" {
 
 GEN9BLAS_API int gen9blas_kv_supported(int D, int H, int HKV) { return shape_ok(D, H, HKV) ? 1 : 0; }
-
-GEN9BLAS_API void *gen9blas_get_stream(void) { return G.user_stream_set ? (void *)G.user_stream : nullptr; }
 
 GEN9BLAS_API gen9blas_kv_ws *gen9blas_kv_ws_create(void) {
     if (begin_op()) return nullptr;

@@ -30,13 +30,12 @@ class _Cache(ctypes.Structure):   # gen9blas_kv_cache
     _fields_ = [("D", _I), ("HKV", _I), ("page", _I), ("n_pages", _I),
                 ("K", _P), ("kp", _L), ("kk", _L), ("kh", _L), ("k_bytes", ctypes.c_size_t),
                 ("V", _P), ("vp", _L), ("vk", _L), ("vh", _L), ("v_bytes", ctypes.c_size_t),
-                ("bounds", _P), ("table", _P), ("ts", _L), ("mp", _I), ("ns", _I)]
+                ("bounds", _P), ("table", _P), ("ts", _L), ("mp", _I), ("ns", _I), ("stream", _P)]
 
 
 _C = ctypes.POINTER(_Cache)
 _SIGNATURES = {
-    "init": ([], _I), "error": ([], ctypes.c_char_p), "set_device": ([_I], _I), "get_device": ([], _I),
-    "set_stream": ([_P], _I), "get_stream": ([], _P),
+    "init": ([], _I), "error": ([], ctypes.c_char_p), "set_device": ([_I], _I),
     "kv_supported": ([_I, _I, _I], _I), "kv_ws_create": ([], _P), "kv_ws_free": ([_P], None),
     "kv_append": ([_C, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _L, _L, _P, _I, _P], _I),
     "attn_paged": ([_C, _I, _I, _P, _L, _L, _L, _P, _I, _I, _P, _I, _F, _P, _P, _P, _L, _L, _P, _I], _I),
@@ -50,7 +49,6 @@ for _name, (_args, _res) in _SIGNATURES.items():
     _f.argtypes, _f.restype = _args, _res
     _fn[_name] = _f
 _append, _attend, _select, _evict = (_fn[n] for n in ("kv_append", "attn_paged", "kv_select", "kv_evict"))
-_set_stream, _get_stream, _get_device = _fn["set_stream"], _fn["get_stream"], _fn["get_device"]
 _LEGACY = 1   # cudaStreamLegacy: torch's default stream (a null stream would mean the library's own)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # torch's accessor without the Stream object, 1.2 us less
 if _raw_stream is None:
@@ -69,6 +67,12 @@ def _check(status, what):
 def _need(ok, message):
     if not ok:
         raise ValueError(message)
+
+
+def set_device(index):
+    """The device of later calls of the library (gen9blas_set_device): that of the caches. Default: the one that was current
+    when the library was first used."""
+    _check(_fn["set_device"](index), "set_device")
 
 
 class Workspace:
@@ -110,7 +114,7 @@ class PagedKV:
         self.heads, self.page, self.dim = heads, page, dim
         self._index = K.device.index
         self._per_stream = torch.Size([self.streams])
-        self._ws = workspace.handle if workspace is not None else None
+        self._logs = torch.empty(0, device=K.device)
 
         def span(x):
             return 2 * (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) if x.numel() else 0
@@ -123,19 +127,20 @@ class PagedKV:
             raise RuntimeError(_fn["error"]().decode(errors="replace"))
 
     def _run(self, what, fn, *args):
-        """One library call on this cache's device and torch's current stream there; both are put back after it."""
-        stream, device = _get_stream(), _get_device()
-        if device != self._index:
-            _check(_fn["set_device"](self._index), what)
-        _set_stream(_raw_stream(self._index) or _LEGACY)
-        try:
-            status = fn(self._ref, *args)
-        finally:
-            if device != self._index:
-                _fn["set_device"](device)
-            _set_stream(stream)
+        """One library call on torch's current stream of this cache's device."""
+        self._c.stream = _raw_stream(self._index) or _LEGACY
+        status = fn(self._ref, *args)
         if status:
             _check(status, what)
+
+    def _space(self):
+        """The workspace's handle as it is now: a freed one must not reach the library."""
+        w = self.workspace
+        if w is None:
+            return None
+        if not w.handle:
+            raise ValueError("the cache's workspace has been freed")
+        return w.handle
 
     # The checks run in every call, so their messages are put together only when one fails.
     def _rows(self, name, x, heads):
@@ -212,9 +217,14 @@ class PagedKV:
             out = self._like(q, n)
         else:
             self._given(out, tuple(n), _f32)
-        logs = q.new_empty((ns, nq, h)) if lse else None
+        logs = None
+        if lse:
+            shape = n[:3]
+            if self._logs.shape != shape:
+                self._logs = q.new_empty(shape)        # only its shape is used: empty_like costs 0.5 us less than new_empty
+            logs = torch.empty_like(self._logs)
         self._run("attend", _attend, h, nq, q.data_ptr(), qs[1], qs[2], qs[0], see, step, window, sp, nsel,
-                  d ** -0.5 if scale is None else scale, out.data_ptr(), logs.data_ptr() if lse else None, a, ms, mh, self._ws, 0)
+                  d ** -0.5 if scale is None else scale, out.data_ptr(), logs.data_ptr() if lse else None, a, ms, mh, self._space(), 0)
         return (out, logs) if lse else out
 
     def select(self, q, visible, pages, step=1, first=1, last=1, out=None):
@@ -226,7 +236,7 @@ class PagedKV:
         else:
             self._given(out, (n[0], n[1], self.heads, pages), _i32)
         self._run("select", _select, n[2], n[1], q.data_ptr(), qs[1], qs[2], qs[0], self._ints("visible", visible), step, first,
-                  last, pages, out.data_ptr(), self._ws, 0)
+                  last, pages, out.data_ptr(), self._space(), 0)
         return out
 
     def evict(self, length, keep, acc, pos=None, first=0, recent=0, out=None):
@@ -239,5 +249,5 @@ class PagedKV:
             out = torch.empty_like(length)
         else:
             self._ints("out", out)
-        self._run("evict", _evict, n, keep, first, recent, a, p, ms, mh, out.data_ptr(), self._ws, 0)
+        self._run("evict", _evict, n, keep, first, recent, a, p, ms, mh, out.data_ptr(), self._space(), 0)
         return out

@@ -1,6 +1,7 @@
 /* gen9blas_kv.h -- a key-value cache in pages and the operators that write, read, search and thin it, for serving
  * (an addition of the B200 build: the reference's lib/gen9blas_ml.h keeps one contiguous cache per stream). Conventions
- * (results, threads, gen9blas_set_stream, no-wait mode, gen9blas_flush) as in gen9blas.h and gen9blas_ml.h.
+ * (results, threads, streams, no-wait mode) as in gen9blas.h and gen9blas_ml.h; gen9blas_flush waits
+ * for the stream of gen9blas_set_stream only.
  *
  * The cache: a pool of pages of `page` slots for each of HKV key-value heads, keys and values FP16, shared by ns streams
  * through a table of page numbers: slot k of stream s is slot k % page of page table[s·ts + k / page], for k below
@@ -34,12 +35,10 @@ typedef struct gen9blas_kv_cache {
     const int *table;        /* page numbers, mp per stream, streams ts apart */
     int64_t ts;
     int mp, ns;
+    void *stream;            /* cudaStream_t of the calls on this cache; NULL: as for every other call (gen9blas_set_stream) */
 } gen9blas_kv_cache;
 
 GEN9BLAS_API int gen9blas_kv_supported(int D, int H, int HKV);
-/* The stream set with gen9blas_set_stream (NULL: the library's own), for callers that change it for a call and put it
- * back. */
-GEN9BLAS_API void *gen9blas_get_stream(void);
 
 /* Workspace of attn_paged, kv_select and kv_evict. NULL in a call means the library's own one of the device: calls that
  * share a workspace run one after the other (one on another stream than the last first waits for the device). A call
