@@ -6,6 +6,7 @@
 #include "kv_plan.cuh"
 #include "mma_sync.cuh"
 #include "sm100.cuh"
+#include <cooperative_groups.h>
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -594,16 +595,72 @@ struct NthKey {   // shared memory of nth_key
     uint32_t buf[2][4][32];
     uint32_t list[NLIST];
     int n, found[3];
+    uint32_t pub[2][3];   // this CTA's part of a sum over the cluster, by turns
 };
-// The m-th largest of n keys (n >= m >= 1) of a CTA, how many are larger and how many as large. A range of keys is cut into
-// four a round, by the counts of the keys at least as large as each of three borders (added up in the warps and through
-// shared memory, one barrier a round), from the least and the largest key on, until at most NLIST keys lie in it; those are
-// ranked directly. Keys of all ones stand above the range. Thread t holds the keys t, t + NT, ... in reg (anything past the
-// end); keys beyond R·NT come from `more` in every round. Scores and weights fill their range evenly enough for about three
-// rounds; it takes 16 at most. (Radix selection with shared-memory histograms took 3 to 4 µs a digit here, for the crowding
-// of keys in few bins, its scans and four barriers each; cutting from the top bit on 0.7 µs a round, eight rounds.)
-template <int NT, int R, typename More>
-__device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int m, NthKey &sh, More more, int *larger, int *equal) {
+
+// Who shares the keys: one CTA, or the CTAs of a cluster, which add up through each other's shared memory.
+struct Solo {
+    __device__ void range(NthKey &, uint32_t &, uint32_t &, int &) {}
+    __device__ void add(NthKey &, uint32_t &, uint32_t &, uint32_t &) {}
+    __device__ NthKey *home(NthKey &sh) { return &sh; }
+    __device__ void sync() { __syncthreads(); }
+};
+struct Cluster {
+    cooperative_groups::cluster_group g;
+    int size, rank, turn;
+    __device__ Cluster() : g(cooperative_groups::this_cluster()), size((int)g.num_blocks()), rank((int)g.block_rank()), turn(0) {}
+    // Publishes three words of this CTA and returns lane's CTA's ones (nothing for lanes past the cluster). A word is written
+    // again two turns later, behind a barrier that every reader of this turn has passed.
+    __device__ bool all(NthKey &sh, uint32_t a, uint32_t b, uint32_t c, uint32_t (&out)[3]) {
+        if (threadIdx.x == 0) {
+            sh.pub[turn][0] = a;
+            sh.pub[turn][1] = b;
+            sh.pub[turn][2] = c;
+        }
+        g.sync();
+        const int lane = threadIdx.x & 31;
+        if (lane < size) {
+            const uint32_t *p = g.map_shared_rank(&sh.pub[turn][0], lane);
+            out[0] = p[0];
+            out[1] = p[1];
+            out[2] = p[2];
+        }
+        turn ^= 1;
+        return lane < size;
+    }
+    __device__ void range(NthKey &sh, uint32_t &lo, uint32_t &hi, int &top) {
+        if (size == 1) return;
+        uint32_t v[3];
+        const bool in = all(sh, lo, hi, (uint32_t)top, v);
+        lo = __reduce_min_sync(kAll, in ? v[0] : kAll);
+        hi = __reduce_max_sync(kAll, in ? v[1] : 0u);
+        top = __reduce_add_sync(kAll, in ? (int)v[2] : 0);
+    }
+    __device__ void add(NthKey &sh, uint32_t &a, uint32_t &b, uint32_t &c) {
+        if (size == 1) return;
+        uint32_t v[3];
+        const bool in = all(sh, a, b, c, v);
+        a = __reduce_add_sync(kAll, in ? v[0] : 0u);
+        b = __reduce_add_sync(kAll, in ? v[1] : 0u);
+        c = __reduce_add_sync(kAll, in ? v[2] : 0u);
+    }
+    __device__ NthKey *home(NthKey &sh) { return size == 1 ? &sh : g.map_shared_rank(&sh, 0); }
+    __device__ void sync() {
+        if (size == 1) __syncthreads();
+        else g.sync();
+    }
+};
+
+// The m-th largest of n keys (n >= m >= 1), how many are larger and how many as large. A range of keys is cut into four a
+// round, by the counts of the keys at least as large as each of three borders (added up in the warps, through shared memory
+// and over the cluster), from the least and the largest key on, until at most NLIST keys lie in it; those are ranked directly.
+// Keys of all ones stand above the range. This CTA holds `mine` of the keys: thread t the keys t, t + NT, ... in reg (anything
+// past the end); keys beyond R·NT come from `more` in every round. Scores and weights fill their range evenly enough for about
+// three rounds; it takes 16 at most. (Radix selection with shared-memory histograms took 3 to 4 µs a digit here, for the
+// crowding of keys in few bins, its scans and four barriers each; cutting from the top bit on 0.7 µs a round, eight rounds.)
+template <int NT, int R, typename Team, typename More>
+__device__ __forceinline__ uint32_t nth_key(Team &team, const uint32_t (&reg)[R], int mine, int n, int m, NthKey &sh, More more,
+                                            int *larger, int *equal) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     constexpr int W = NT / 32;
     uint32_t lo = kAll, hi = 0;
@@ -615,8 +672,8 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
     };
 #pragma unroll
     for (int i = 0; i < R; i++)
-        if ((int)threadIdx.x + i * NT < n) range(reg[i]);
-    for (int i = R * NT + threadIdx.x; i < n; i += NT) range(more(i));
+        if ((int)threadIdx.x + i * NT < mine) range(reg[i]);
+    for (int i = R * NT + threadIdx.x; i < mine; i += NT) range(more(i));
     lo = __reduce_min_sync(kAll, lo);
     hi = __reduce_max_sync(kAll, hi);
     top = __reduce_add_sync(kAll, top);
@@ -630,6 +687,7 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
     lo = __reduce_min_sync(kAll, lane < W ? sh.buf[0][0][lane] : kAll);
     hi = __reduce_max_sync(kAll, lane < W ? sh.buf[0][1][lane] : 0u);
     top = __reduce_add_sync(kAll, lane < W ? (int)sh.buf[0][2][lane] : 0);
+    team.range(sh, lo, hi, top);
     if (top >= m) {
         *larger = 0;
         *equal = top;
@@ -641,12 +699,12 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
         uint32_t c1 = 0, c2 = 0, c3 = 0;
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const uint32_t k = (int)threadIdx.x + i * NT < n ? reg[i] : 0u;   // a1 > 0
+            const uint32_t k = (int)threadIdx.x + i * NT < mine ? reg[i] : 0u;   // a1 > 0
             c1 += k >= a1;
             c2 += k >= a2;
             c3 += k >= a3;
         }
-        for (int i = R * NT + threadIdx.x; i < n; i += NT) {
+        for (int i = R * NT + threadIdx.x; i < mine; i += NT) {
             const uint32_t k = more(i);
             c1 += k >= a1;
             c2 += k >= a2;
@@ -665,6 +723,7 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
         c1 = __reduce_add_sync(kAll, lane < W ? buf[0][lane] : 0u);
         c2 = __reduce_add_sync(kAll, lane < W ? buf[1][lane] : 0u);
         c3 = __reduce_add_sync(kAll, lane < W ? buf[2][lane] : 0u);
+        team.add(sh, c1, c2, c3);
         const int all = in + above;   // keys of at least lo
         if ((int)c3 >= m) {
             lo = a3;
@@ -690,17 +749,22 @@ __device__ __forceinline__ uint32_t nth_key(const uint32_t (&reg)[R], int n, int
         *equal = in;
         return lo;
     }
+    NthKey *home = team.home(sh);
     auto put = [&](uint32_t k) {
         if (k >= lo && k <= hi) {
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < NLIST) sh.list[at] = k;   // never more
+            const int at = atomicAdd(&home->n, 1);
+            if (at < NLIST) home->list[at] = k;   // never more
         }
     };
 #pragma unroll
     for (int i = 0; i < R; i++)
-        if ((int)threadIdx.x + i * NT < n) put(reg[i]);
-    for (int i = R * NT + threadIdx.x; i < n; i += NT) put(more(i));
-    __syncthreads();
+        if ((int)threadIdx.x + i * NT < mine) put(reg[i]);
+    for (int i = R * NT + threadIdx.x; i < mine; i += NT) put(more(i));
+    team.sync();
+    if (home != &sh) {
+        if ((int)threadIdx.x < in) sh.list[threadIdx.x] = home->list[threadIdx.x];
+        __syncthreads();
+    }
     // four threads a key of the list: how many are larger, how many at least as large; the r-th is where fewer than r are
     // larger and at least r as large
     const int r = m - above, i = threadIdx.x >> 2;
@@ -845,7 +909,8 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     for (int i = 0; i < CR; i++) key[i] = tid + i * CT < have ? key_of(tid + i * CT, x[i]) : 0u;
     for (int i = tid; i < CR * CT / 32; i += CT) taken[i] = 0;
     int larger, equal;
-    const uint32_t at = nth_key<CT, CR>(key, have, m, nth, [&](int i) { return key_of(i, __ldcg(score + i)); }, &larger, &equal);
+    Solo solo;
+    const uint32_t at = nth_key<CT, CR>(solo, key, have, have, m, nth, [&](int i) { return key_of(i, __ldcg(score + i)); }, &larger, &equal);
     for (int w = 0; w < CT / 32; w++) {
         big = fmaxf(big, red[0][w]);
         l1 = fmaxf(l1, red[1][w]);
@@ -984,55 +1049,65 @@ struct EvictArgs {
     int *len_out;
 };
 
-// Which slots stay, and where the movers go: one CTA per row (s, g). The threshold is the keep-th largest key; then one
-// ordered pass over the slots, ER·ET at a time: below `keep` the given-up slots are listed and their pages marked, from
-// there on the j-th staying slot becomes the source of the j-th of them. ET threads hold ER slots each: as few as the table's
-// slots need (256 rows of 2064 slots took 61 µs with 1024 threads of 16, most of it idle registers), at most 1024 of 16,
-// beyond which the weights are read again where they are used.
+// Which slots stay, and where the movers go: a cluster of 1 to 8 CTAs per row (s, g), a stretch of the slots each. The threshold
+// is the keep-th largest key; then an ordered pass over the slots, ER·ET at a time: below `keep` the given-up slots are listed
+// and their pages marked, from there on the j-th staying slot becomes the source of the j-th of them. A CTA of ET threads
+// holds ER slots a thread in registers, those beyond are read again where they are used. As few threads as the table's slots
+// need (256 rows of 2064 slots took 61 µs with 1024 threads of 16, most of them idle), and clusters for long rows (64 rows of
+// 16384 slots: 31 µs with a CTA of 1024 threads each).
 template <int ET, int ER>
 __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArgs a) {
     __shared__ NthKey nth;
     __shared__ int order[ER * ET / 32], scan[32], sh_new;
+    constexpr int PAIRS = ER * ET / 32;
+    Cluster team;
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
-    const int row = blockIdx.x, s = row / c.HKV, g = row - s * c.HKV;
+    const int row = blockIdx.x / team.size, s = row / c.HKV, g = row - s * c.HKV;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = min(max(a.len[s], 0), c.cap), keep = a.keep;
+    const int per = ((n + team.size - 1) / team.size + 31) / 32 * 32;
+    const int from = min(team.rank * per, n), mine = min(per, n - from);   // this CTA's slots: [from, from + mine)
     if (tid == 0) {
-        a.used[2 * row] = n;
-        a.used[2 * row + 1] = 0;
+        if (team.rank == 0) {
+            a.used[2 * row] = n;
+            a.used[2 * row + 1] = 0;
+        }
         sh_new = INT_MIN;
     }
     if (n <= keep) return;
     const float *acc = a.acc + s * a.ms + g * a.mh;
     const int *pos = a.pos ? a.pos + s * a.ms + g * a.mh : nullptr;
     int *src = a.src + (long long)row * keep, *holes = a.holes + (long long)row * keep, *flag = a.flag + (long long)row * a.pages;
-    for (int i = tid; i < a.pages; i += ET) flag[i] = 0;
+    for (int i = team.rank * ET + tid; i < a.pages; i += team.size * ET) flag[i] = 0;
     uint32_t key[ER];   // the weight's key, then that with the sure ones on top
     int newest = n - 1;
     if (pos) {
         int p[ER], m = INT_MIN;
 #pragma unroll
-        for (int i = 0; i < ER; i++) p[i] = tid + i * ET < n ? __ldg(pos + tid + i * ET) : INT_MIN;
+        for (int i = 0; i < ER; i++) p[i] = tid + i * ET < mine ? __ldg(pos + from + tid + i * ET) : INT_MIN;
 #pragma unroll
-        for (int i = 0; i < ER; i++) key[i] = tid + i * ET < n ? weight_key(__ldg(acc + tid + i * ET)) : 0u;
+        for (int i = 0; i < ER; i++) key[i] = tid + i * ET < mine ? weight_key(__ldg(acc + from + tid + i * ET)) : 0u;
 #pragma unroll
         for (int i = 0; i < ER; i++) m = max(m, p[i]);
-        for (int k = ER * ET + tid; k < n; k += ET) m = max(m, __ldg(pos + k));
+        for (int k = ER * ET + tid; k < mine; k += ET) m = max(m, __ldg(pos + from + k));
         m = __reduce_max_sync(kAll, m);
         __syncthreads();   // sh_new is set
         if (lane == 0) atomicMax(&sh_new, m);
         __syncthreads();
-        newest = sh_new;
+        uint32_t none = 0, big = (uint32_t)sh_new ^ 0x80000000u;   // unsigned order
+        int zero = 0;
+        team.range(nth, none, big, zero);
+        newest = (int)(big ^ 0x80000000u);
 #pragma unroll
         for (int i = 0; i < ER; i++)
-            if (tid + i * ET < n && (p[i] < a.first || p[i] > (long long)newest - a.recent)) key[i] = kAll;
+            if (tid + i * ET < mine && (p[i] < a.first || p[i] > (long long)newest - a.recent)) key[i] = kAll;
     } else {
 #pragma unroll
         for (int i = 0; i < ER; i++) {
-            const int k = tid + i * ET;
-            key[i] = k >= n ? 0u : k < a.first || k > (long long)newest - a.recent ? kAll : weight_key(__ldg(acc + k));
+            const int k = from + tid + i * ET;
+            key[i] = tid + i * ET >= mine ? 0u : k < a.first || k > (long long)newest - a.recent ? kAll : weight_key(__ldg(acc + k));
         }
     }
     const long long old = (long long)newest - a.recent;
@@ -1041,67 +1116,150 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
         return p < a.first || p > old ? kAll : weight_key(__ldg(acc + k));
     };
     int larger, equal;
-    const uint32_t last = nth_key<ET, ER>(key, n, keep, nth, key_of, &larger, &equal);
+    const uint32_t last = nth_key<ET, ER>(team, key, mine, n, keep, nth, [&](int i) { return key_of(from + i); }, &larger, &equal);
     const int need = keep - larger;   // of the `equal` keys at the threshold the first `need` stay
-    int eq_base = 0, holes_n = 0, moved = 0;
-    for (int i0 = 0; i0 < n; i0 += ER * ET) {
-        unsigned hole[ER], mover[ER];   // ballots of the warps
-        if (i0 > 0) {
+    // sum of v over the CTA; then the sum over the earlier CTAs of the cluster
+    auto cta_sum = [&](int v) {
+        int total;
+        block_scan_incl(v, scan, &total);
+        return total;
+    };
+    auto earlier = [&](int a0, int a1, int *b0, int *b1) {
+        uint32_t v[3];
+        const bool in = team.all(nth, (uint32_t)a0, (uint32_t)a1, 0u, v) && lane < team.rank;
+        *b0 = __reduce_add_sync(kAll, in ? (int)v[0] : 0);
+        *b1 = __reduce_add_sync(kAll, in ? (int)v[1] : 0);
+    };
+    int eq_before = 0, eq_base = 0;
+    if (equal != need && team.size > 1) {
+        int e = 0;
 #pragma unroll
-            for (int i = 0; i < ER; i++) key[i] = i0 + i * ET + tid < n ? key_of(i0 + i * ET + tid) : 0u;
+        for (int i = 0; i < ER; i++) e += tid + i * ET < mine && key[i] == last;
+        for (int i = ER * ET + tid; i < mine; i += ET) e += key_of(from + i) == last;
+        int none;
+        earlier(cta_sum(e), 0, &eq_before, &none);
+    }
+    // which of the slots from + i0 + i·ET + tid stay, bit i; advances eq_base
+    auto staying = [&](int i0) -> unsigned {
+        if (i0 > 0 || mine > ER * ET) {
+#pragma unroll
+            for (int i = 0; i < ER; i++) key[i] = i0 + i * ET + tid < mine ? key_of(from + i0 + i * ET + tid) : 0u;
         }
-        unsigned stays = 0;   // bit i: slot i0 + i·ET + tid
+        unsigned stays = 0;
         if (equal == need) {
 #pragma unroll
-            for (int i = 0; i < ER; i++) stays |= (unsigned)(key[i] >= last && i0 + i * ET + tid < n) << i;
-        } else {
-            unsigned eq[ER];
-#pragma unroll
-            for (int i = 0; i < ER; i++) {
-                eq[i] = __ballot_sync(kAll, i0 + i * ET + tid < n && key[i] == last);
-                if (lane == 0) order[i * (ET / 32) + warp] = __popc(eq[i]);
-            }
-            const int eq_total = scan_counts<ER * ET / 32>(order, scan);
-#pragma unroll
-            for (int i = 0; i < ER; i++) {
-                const int rank = eq_base + order[i * (ET / 32) + warp] + __popc(eq[i] & ((1u << lane) - 1u));
-                stays |= (unsigned)(i0 + i * ET + tid < n && (key[i] > last || (key[i] == last && rank < need))) << i;
-            }
-            eq_base += eq_total;
-            __syncthreads();   // the sums are read before the next counts land on them
+            for (int i = 0; i < ER; i++) stays |= (unsigned)(key[i] >= last && i0 + i * ET + tid < mine) << i;
+            return stays;
         }
+        unsigned eq[ER];
 #pragma unroll
         for (int i = 0; i < ER; i++) {
-            const int k = i0 + i * ET + tid;
-            const bool stay = stays >> i & 1u;
-            hole[i] = __ballot_sync(kAll, k < keep && !stay);
-            mover[i] = __ballot_sync(kAll, k >= keep && stay);
-            // holes lie below keep, movers behind: their counts share a word (at most 2^14 of each at once)
-            if (lane == 0) order[i * (ET / 32) + warp] = __popc(hole[i]) | __popc(mover[i]) << 16;
-            if (k < keep) src[k] = -1;
+            eq[i] = __ballot_sync(kAll, i0 + i * ET + tid < mine && key[i] == last);
+            if (lane == 0) order[i * (ET / 32) + warp] = __popc(eq[i]);
         }
-        const int total = scan_counts<ER * ET / 32>(order, scan);
+        const int total = scan_counts<PAIRS>(order, scan);
 #pragma unroll
         for (int i = 0; i < ER; i++) {
-            const int k = i0 + i * ET + tid, before = order[i * (ET / 32) + warp];
+            const int rank = eq_base + order[i * (ET / 32) + warp] + __popc(eq[i] & ((1u << lane) - 1u));
+            stays |= (unsigned)(i0 + i * ET + tid < mine && (key[i] > last || (key[i] == last && rank < need))) << i;
+        }
+        eq_base += total;
+        __syncthreads();   // the sums are read before the next counts land on them
+        return stays;
+    };
+    int holes_n = 0, moved = 0;   // before this CTA's slots, then before the next of them
+    if (per <= ER * ET) {         // (every CTA of the cluster) all slots in registers: the counts of both kinds share a scan
+        eq_base = eq_before;
+        const unsigned stays = staying(0);
+        unsigned hole[ER], mover[ER];
+#pragma unroll
+        for (int i = 0; i < ER; i++) {
+            const int k = from + i * ET + tid;
+            const bool in = i * ET + tid < mine, stay = stays >> i & 1u;
+            hole[i] = __ballot_sync(kAll, in && k < keep && !stay);
+            mover[i] = __ballot_sync(kAll, in && k >= keep && stay);
+            if (lane == 0) order[i * (ET / 32) + warp] = __popc(hole[i]) | __popc(mover[i]) << 16;   // at most ER·ET of each
+            if (in && k < keep) src[k] = -1;
+        }
+        const int total = scan_counts<PAIRS>(order, scan);
+        if (team.size > 1) earlier(total & 0xffff, total >> 16, &holes_n, &moved);
+#pragma unroll
+        for (int i = 0; i < ER; i++)
             if (hole[i] >> lane & 1u) {
-                holes[holes_n + (before & 0xffff) + __popc(hole[i] & ((1u << lane) - 1u))] = k;
+                const int k = from + i * ET + tid;
+                holes[holes_n + (order[i * (ET / 32) + warp] & 0xffff) + __popc(hole[i] & ((1u << lane) - 1u))] = k;
                 flag[page_quot(c.div, k)] = 1;
             }
-        }
-        __syncthreads();   // the holes so far are listed: the movers of these slots fill the first of them
+        team.sync();   // every hole is listed
 #pragma unroll
-        for (int i = 0; i < ER; i++) {
-            const int k = i0 + i * ET + tid, before = order[i * (ET / 32) + warp];
+        for (int i = 0; i < ER; i++)
             if (mover[i] >> lane & 1u) {
-                const int at = moved + (before >> 16) + __popc(mover[i] & ((1u << lane) - 1u));
-                if (at < keep) src[holes[at]] = k;
+                const int at = moved + (order[i * (ET / 32) + warp] >> 16) + __popc(mover[i] & ((1u << lane) - 1u));
+                if (at < keep) src[__ldcg(holes + at)] = from + i * ET + tid;
+            }
+    } else {
+        if (team.size > 1) {
+            int h = 0, m = 0;
+            eq_base = eq_before;
+            for (int i0 = 0; i0 < mine; i0 += ER * ET) {
+                const unsigned stays = staying(i0);
+#pragma unroll
+                for (int i = 0; i < ER; i++) {
+                    const int k = from + i0 + i * ET + tid;
+                    h += i0 + i * ET + tid < mine && k < keep && !(stays >> i & 1u);
+                    m += k >= keep && (stays >> i & 1u);
+                }
+            }
+            h = cta_sum(h);
+            m = cta_sum(m);
+            earlier(h, m, &holes_n, &moved);
+        }
+        const int moved_base = moved;
+        eq_base = eq_before;
+        // two rounds over the slots: the holes, then -- once every CTA of the cluster has listed its own -- the movers
+        for (int phase = 0; phase < 2; phase++) {
+            if (phase) {
+                eq_base = eq_before;
+                moved = moved_base;
+                team.sync();
+            }
+            for (int i0 = 0; i0 < mine; i0 += ER * ET) {
+                // slots on one side of keep only have work in one of the phases
+                if (phase ? from + min(i0 + ER * ET, mine) <= keep : from + i0 >= keep) {
+                    if (equal != need) staying(i0);
+                    continue;
+                }
+                const unsigned stays = staying(i0);
+                unsigned hit[ER];
+#pragma unroll
+                for (int i = 0; i < ER; i++) {
+                    const int k = from + i0 + i * ET + tid;
+                    const bool in = i0 + i * ET + tid < mine, stay = stays >> i & 1u;
+                    hit[i] = __ballot_sync(kAll, in && (phase ? k >= keep && stay : k < keep && !stay));
+                    if (lane == 0) order[i * (ET / 32) + warp] = __popc(hit[i]);
+                    if (!phase && in && k < keep) src[k] = -1;
+                }
+                const int total = scan_counts<PAIRS>(order, scan);
+#pragma unroll
+                for (int i = 0; i < ER; i++) {
+                    const int k = from + i0 + i * ET + tid;
+                    if (!(hit[i] >> lane & 1u)) continue;
+                    const int at = (phase ? moved : holes_n) + order[i * (ET / 32) + warp] + __popc(hit[i] & ((1u << lane) - 1u));
+                    if (phase) {
+                        if (at < keep) src[__ldcg(holes + at)] = k;
+                    } else {
+                        holes[at] = k;
+                        flag[page_quot(c.div, k)] = 1;
+                    }
+                }
+                if (phase) moved += total;
+                else holes_n += total;
+                __syncthreads();   // the sums are read before the next counts land on them
             }
         }
-        holes_n += total & 0xffff;
-        moved += total >> 16;
-        __syncthreads();   // the sums are read before the next counts land on them
     }
+    team.sync();   // every page is marked, every CTA's shared memory read
+    if (team.rank) return;
     // the pages that change: those with holes, and the one that held slots on both sides of keep
     int base = 0;
     for (int i0 = 0; i0 < a.pages; i0 += ER * ET) {
@@ -1109,10 +1267,10 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
 #pragma unroll
         for (int i = 0; i < ER; i++) {
             const int p = i0 + i * ET + tid;
-            hit[i] = __ballot_sync(kAll, p < a.pages && (flag[p] || (p == a.pages - 1 && keep % c.page)));
+            hit[i] = __ballot_sync(kAll, p < a.pages && (__ldcg(flag + p) || (p == a.pages - 1 && keep % c.page)));
             if (lane == 0) order[i * (ET / 32) + warp] = __popc(hit[i]);
         }
-        const int total = scan_counts<ER * ET / 32>(order, scan);
+        const int total = scan_counts<PAIRS>(order, scan);
 #pragma unroll
         for (int i = 0; i < ER; i++)
             if (hit[i] >> lane & 1u)
@@ -1228,6 +1386,25 @@ size_t marks_bytes(const KvDev &c, int64_t ms, int64_t mh) {
     return ((size_t)std::max(c.ns - 1, 0) * (size_t)std::max<int64_t>(ms, 0) + (size_t)(c.HKV - 1) * (size_t)std::max<int64_t>(mh, 0) +
             (size_t)c.cap) * 4;
 }
+// A cluster of `size` CTAs per row, with programmatic stream serialization as launch_pdl.
+template <int ET, int ER>
+int rank_launch(const EvictArgs &a, const KvCall &call, long long rows, int size) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * size));
+    cfg.blockDim = dim3(ET);
+    cfg.stream = call.st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)size;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    G9_CU(cudaLaunchKernelEx(&cfg, kv_rank_k<ET, ER>, a));
+    return launched("kv_rank");
+}
+
 // One wave of CTAs, as many as shared memory lets an SM hold, and no more than there can be runs.
 template <int DP>
 int score_launch(const SelectArgs &a, const KvCall &call, long long most) {
@@ -1436,15 +1613,17 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     a.flag = (int *)((char *)buf + 2 * list);
     a.todo = (int *)((char *)buf + 2 * list + pages);
     a.used = (int *)((char *)buf + 2 * list + 2 * pages);
-    const dim3 grid((unsigned)rows);
-    if (a.c.cap <= 256 * 4) G9_CU(launch_pdl(kv_rank_k<256, 4>, grid, dim3(256), 0, call.st, a));
-    else if (a.c.cap <= 256 * 12) G9_CU(launch_pdl(kv_rank_k<256, 12>, grid, dim3(256), 0, call.st, a));
-    else if (a.c.cap <= 1024 * 8) G9_CU(launch_pdl(kv_rank_k<1024, 8>, grid, dim3(1024), 0, call.st, a));
-    else G9_CU(launch_pdl(kv_rank_k<1024, 16>, grid, dim3(1024), 0, call.st, a));
-    G9_TRY(launched("kv_rank"));
+    // clusters that hold a row's slots in registers, and larger ones while the GPU has SMs to spare for rows of 1024 slots a CTA
+    int size = 1;
+    while (size < 8 && (a.c.cap > 512 * 12 * size || (rows * size * 2 <= call.d->sm_count && a.c.cap > 2048 * size))) size *= 2;
+    if (rows * size > INT_MAX) size = 1;
+    if (size == 1 && a.c.cap <= 256 * 4) G9_TRY((rank_launch<256, 4>(a, call, rows, 1)));
+    else if (size == 1 && a.c.cap <= 256 * 12) G9_TRY((rank_launch<256, 12>(a, call, rows, 1)));
+    else G9_TRY((rank_launch<512, 12>(a, call, rows, size)));
     const int team = c->page > 32 ? MT / 32 : 1, teams = MT / 32 / team;
-    // a page per team where the rows are few, else one wave of CTAs in all
-    const long long ctas = std::max<long long>(1, std::min<long long>((a.pages + teams - 1) / teams, (long long)MCTAS * call.d->sm_count / rows));
+    // a page per team, as many as can change (each mover changes one, and the last may lose slots), up to four waves of CTAs
+    const long long most = std::min<long long>(a.pages, (long long)a.c.cap - a.keep + 1);
+    const long long ctas = std::max<long long>(1, std::min<long long>((most + teams - 1) / teams, 4LL * MCTAS * call.d->sm_count / rows));
     const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));

@@ -382,7 +382,8 @@ def test_select_many_equal_pages(kv, n, m):
 # ------------------------------------------------------------------------------------------------ eviction
 @pytest.mark.parametrize("lens,keep,page,heads,D,first,recent,layout", [
     ([50, 33, 32, 0, 5], 32, 16, 2, 128, 2, 4, "phsd"), ([100], 1, 8, 1, 64, 0, 0, "pshd"), ([100, 99], 37, 5, 3, 80, 4, 30, "both"),
-    ([513], 512, 64, 2, 256, 0, 1, "phsd"), ([70, 10], 500, 16, 1, 8, 4, 4, "phsd"), ([3000, 2999], 1500, 32, 2, 64, 4, 32, "phsd")])
+    ([513], 512, 64, 2, 256, 0, 1, "phsd"), ([70, 10], 500, 16, 1, 8, 4, 4, "phsd"), ([3000, 2999], 1500, 32, 2, 64, 4, 32, "phsd"),
+    ([20000, 13001, 400], 9000, 16, 1, 8, 4, 32, "phsd"), ([60000], 30001, 64, 2, 8, 4, 32, "pshd"), ([7000] * 30, 6990, 100, 2, 8, 0, 9, "phsd")])
 @pytest.mark.parametrize("with_pos", [False, True])
 def test_evict(kv, lens, keep, page, heads, D, first, recent, layout, with_pos):
     rng = np.random.default_rng(keep + page)
