@@ -212,22 +212,41 @@ struct AppendArgs {
     unsigned *bad;
 };
 
-__device__ __forceinline__ float4 row4(const float *p, int v4) {
-    return v4 ? __ldg(reinterpret_cast<const float4 *>(p)) : make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
-}
-__device__ __forceinline__ uint2 half4(float4 x) {
-    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
-    return make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-}
 __device__ __forceinline__ __half2 as_h2(unsigned x) { return *reinterpret_cast<const __half2 *>(&x); }
 __device__ __forceinline__ unsigned as_u(__half2 x) { return *reinterpret_cast<const unsigned *>(&x); }
+// eight F32 elements as FP16, to nearest even
+__device__ __forceinline__ uint4 row8(const float *p, int v4) {
+    float x[8];
+    if (v4) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __ldg(p + i);
+    }
+    return make_uint4(as_u(__floats2half2_rn(x[0], x[1])), as_u(__floats2half2_rn(x[2], x[3])), as_u(__floats2half2_rn(x[4], x[5])),
+                      as_u(__floats2half2_rn(x[6], x[7])));
+}
+// the elements' least and largest of two pairs of 8
+__device__ __forceinline__ uint4 least8(uint4 x, uint4 y) {
+    return make_uint4(as_u(__hmin2(as_h2(x.x), as_h2(y.x))), as_u(__hmin2(as_h2(x.y), as_h2(y.y))),
+                      as_u(__hmin2(as_h2(x.z), as_h2(y.z))), as_u(__hmin2(as_h2(x.w), as_h2(y.w))));
+}
+__device__ __forceinline__ uint4 largest8(uint4 x, uint4 y) {
+    return make_uint4(as_u(__hmax2(as_h2(x.x), as_h2(y.x))), as_u(__hmax2(as_h2(x.y), as_h2(y.y))),
+                      as_u(__hmax2(as_h2(x.z), as_h2(y.z))), as_u(__hmax2(as_h2(x.w), as_h2(y.w))));
+}
+__device__ __forceinline__ uint4 shfl8(uint4 x, int o) {
+    return make_uint4(__shfl_xor_sync(kAll, x.x, o), __shfl_xor_sync(kAll, x.y, o), __shfl_xor_sync(kAll, x.z, o),
+                      __shfl_xor_sync(kAll, x.w, o));
+}
 
-// One CTA per (page that may be touched, head, stream); its warps take the page's new rows in turn, a lane four elements
-// (or two times four, D > 128) of each row, and keep the elements' least and largest value for the bounds. Bound by memory:
-// the rows read once in FP32 and written once in FP16. Two rows of a warp in flight at five CTAs per SM: 18.5 µs for 81 MB (four
-// rows at three CTAs 23.4, one row at six 19.7).
-__global__ void __launch_bounds__(256, 5) kv_append_k(const __grid_constant__ AppendArgs a) {
-    __shared__ uint2 red[8][2][2][32];   // [warp][least, largest][four-element group of the lane][lane]
+// One CTA per (page that may be touched, head, stream); its warps take the page's new rows in turn, lpr lanes a row, eight
+// elements a lane, and keep the elements' least and largest value for the bounds. Bound by memory: the rows read once in
+// FP32 and written once in FP16: 16.9 µs for 81 MB, with four rounds of rows in flight per warp at four CTAs per SM (eight bytes a
+// lane instead of sixteen 18.5; two rounds at five CTAs 21.8, their registers spilled).
+__global__ void __launch_bounds__(256, 4) kv_append_k(const __grid_constant__ AppendArgs a, int lpr) {
+    __shared__ uint4 red[8][2][32];   // [warp][least, largest][lane]
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
@@ -243,26 +262,22 @@ __global__ void __launch_bounds__(256, 5) kv_append_k(const __grid_constant__ Ap
         if (threadIdx.x == 0 && a.bad) *(volatile unsigned *)a.bad = 1u;
         return;
     }
-    const int i0 = (int)(k0 - place * c.page);
-    const __half2 top = __half2half2(__ushort_as_half(0x7c00)), low = __half2half2(__ushort_as_half(0xfc00));
-    __half2 mn[2][2] = {{top, top}, {top, top}}, mx[2][2] = {{low, low}, {low, low}};
-    __half *kd = c.K + row_at(id, 0, g, c.kp, c.kk, c.kh), *vd = c.V + row_at(id, 0, g, c.vp, c.vk, c.vh);
-    const int rows = (int)(k1 - k0);
+    const int i0 = (int)(k0 - place * c.page), rows = (int)(k1 - k0);
     const long long t0 = k0 - n0;
-    const float *ksrc = a.K + s * a.ks + g * a.kh, *vsrc = a.V + s * a.vs + g * a.vh;
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int d = 4 * lane + 128 * j;
-        if (d >= c.D) break;
-#pragma unroll 2
-        for (int r = warp; r < rows; r += nw) {
-            const uint2 kv = half4(row4(ksrc + (t0 + r) * a.kt + d, a.v4)), vv = half4(row4(vsrc + (t0 + r) * a.vt + d, a.v4));
-            *reinterpret_cast<uint2 *>(kd + (long long)(i0 + r) * c.kk + d) = kv;
-            *reinterpret_cast<uint2 *>(vd + (long long)(i0 + r) * c.vk + d) = vv;
-            mn[j][0] = __hmin2(mn[j][0], as_h2(kv.x));
-            mn[j][1] = __hmin2(mn[j][1], as_h2(kv.y));
-            mx[j][0] = __hmax2(mx[j][0], as_h2(kv.x));
-            mx[j][1] = __hmax2(mx[j][1], as_h2(kv.y));
+    const int rpw = 32 / lpr, sub = lane / lpr, d = (lane - sub * lpr) * 8;   // rows of a warp at once, this lane's row and elements
+    const bool live = d < c.D;
+    uint4 mn = make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);
+    uint4 mx = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+    __half *kd = c.K + row_at(id, i0, g, c.kp, c.kk, c.kh) + d, *vd = c.V + row_at(id, i0, g, c.vp, c.vk, c.vh) + d;
+    const float *ksrc = a.K + s * a.ks + g * a.kh + t0 * a.kt + d, *vsrc = a.V + s * a.vs + g * a.vh + t0 * a.vt + d;
+    if (live) {
+#pragma unroll 4
+        for (int r = warp * rpw + sub; r < rows; r += nw * rpw) {
+            const uint4 kv = row8(ksrc + r * a.kt, a.v4), vv = row8(vsrc + r * a.vt, a.v4);
+            *reinterpret_cast<uint4 *>(kd + r * c.kk) = kv;
+            *reinterpret_cast<uint4 *>(vd + r * c.vk) = vv;
+            mn = least8(mn, kv);
+            mx = largest8(mx, kv);
         }
     }
     if (a.acc || a.pos) {
@@ -274,40 +289,29 @@ __global__ void __launch_bounds__(256, 5) kv_append_k(const __grid_constant__ Ap
         }
     }
     if (!c.bounds) return;
+    for (int o = lpr; o < 32; o <<= 1) {
+        mn = least8(mn, shfl8(mn, o));
+        mx = largest8(mx, shfl8(mx, o));
+    }
     if (nw > 1) {
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            red[warp][0][j][lane] = make_uint2(as_u(mn[j][0]), as_u(mn[j][1]));
-            red[warp][1][j][lane] = make_uint2(as_u(mx[j][0]), as_u(mx[j][1]));
-        }
+        red[warp][0][lane] = mn;
+        red[warp][1][lane] = mx;
         __syncthreads();
         if (warp > 0) return;
-        for (int w = 1; w < nw; w++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint2 x = red[w][0][j][lane], y = red[w][1][j][lane];
-                mn[j][0] = __hmin2(mn[j][0], as_h2(x.x));
-                mn[j][1] = __hmin2(mn[j][1], as_h2(x.y));
-                mx[j][0] = __hmax2(mx[j][0], as_h2(y.x));
-                mx[j][1] = __hmax2(mx[j][1], as_h2(y.y));
-            }
-    }
-    __half *b = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D;
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int d = 4 * lane + 128 * j;
-        if (d >= c.D) break;
-        uint2 *lo = reinterpret_cast<uint2 *>(b + d), *hi = reinterpret_cast<uint2 *>(b + c.D + d);
-        if (i0 > 0) {   // the page held rows before
-            const uint2 x = *lo, y = *hi;
-            mn[j][0] = __hmin2(mn[j][0], as_h2(x.x));
-            mn[j][1] = __hmin2(mn[j][1], as_h2(x.y));
-            mx[j][0] = __hmax2(mx[j][0], as_h2(y.x));
-            mx[j][1] = __hmax2(mx[j][1], as_h2(y.y));
+        for (int w = 1; w < nw; w++) {
+            mn = least8(mn, red[w][0][lane]);
+            mx = largest8(mx, red[w][1][lane]);
         }
-        *lo = make_uint2(as_u(mn[j][0]), as_u(mn[j][1]));
-        *hi = make_uint2(as_u(mx[j][0]), as_u(mx[j][1]));
     }
+    if (sub || !live) return;
+    uint4 *lo = reinterpret_cast<uint4 *>(c.bounds + ((long long)id * c.HKV + g) * 2 * c.D + d);
+    uint4 *hi = reinterpret_cast<uint4 *>(c.bounds + (((long long)id * c.HKV + g) * 2 + 1) * c.D + d);
+    if (i0 > 0) {   // the page held rows before
+        mn = least8(mn, *lo);
+        mx = largest8(mx, *hi);
+    }
+    *lo = mn;
+    *hi = mx;
 }
 
 // ---------------------------------------------------------------------------------------------- page selection
@@ -767,6 +771,7 @@ __device__ __forceinline__ uint32_t nth_key(Team &team, const uint32_t (&reg)[R]
     }
     // four threads a key of the list: how many are larger, how many at least as large; the r-th is where fewer than r are
     // larger and at least r as large
+    static_assert(NT >= 4 * NLIST, "a quad of threads per key");
     const int r = m - above, i = threadIdx.x >> 2;
     if (threadIdx.x < 4 * NLIST) {
         const uint32_t k = i < in ? sh.list[i] : 0u;
@@ -1314,12 +1319,8 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
             if (pos) pos[k0 + i] = pos[k];
         }
         if (id < 0) continue;
-        __half2 mn[4], mx[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            mn[j] = __half2half2(__ushort_as_half(0x7c00));
-            mx[j] = __half2half2(__ushort_as_half(0xfc00));
-        }
+        uint4 mn = make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);   // +inf, -inf
+        uint4 mx = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
         for (int r0 = mate * 32; r0 < rows; r0 += team * 32) {
             // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
             long long ko = 0, vo = -1;
@@ -1342,41 +1343,30 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
                     *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = vv;
                 }
                 if (!bounds) continue;
-                const unsigned x[4] = {kv.x, kv.y, kv.z, kv.w};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    mn[e] = __hmin2(mn[e], as_h2(x[e]));
-                    mx[e] = __hmax2(mx[e], as_h2(x[e]));
-                }
+                mn = least8(mn, kv);
+                mx = largest8(mx, kv);
             }
         }
         if (!bounds) continue;
-        for (int o = lpr; o < 32; o <<= 1)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                mn[j] = __hmin2(mn[j], as_h2(__shfl_xor_sync(kAll, as_u(mn[j]), o)));
-                mx[j] = __hmax2(mx[j], as_h2(__shfl_xor_sync(kAll, as_u(mx[j]), o)));
-            }
-        uint4 lo = make_uint4(as_u(mn[0]), as_u(mn[1]), as_u(mn[2]), as_u(mn[3]));
-        uint4 hi = make_uint4(as_u(mx[0]), as_u(mx[1]), as_u(mx[2]), as_u(mx[3]));
+        for (int o = lpr; o < 32; o <<= 1) {
+            mn = least8(mn, shfl8(mn, o));
+            mx = largest8(mx, shfl8(mx, o));
+        }
         if (team > 1) {   // the whole CTA: every warp is here
-            red[warp][0][lane] = lo;
-            red[warp][1][lane] = hi;
+            red[warp][0][lane] = mn;
+            red[warp][1][lane] = mx;
             __syncthreads();
             if (warp == 0)
                 for (int i = 1; i < team; i++) {
-                    const uint4 x = red[i][0][lane], y = red[i][1][lane];
-                    lo = make_uint4(as_u(__hmin2(as_h2(lo.x), as_h2(x.x))), as_u(__hmin2(as_h2(lo.y), as_h2(x.y))),
-                                    as_u(__hmin2(as_h2(lo.z), as_h2(x.z))), as_u(__hmin2(as_h2(lo.w), as_h2(x.w))));
-                    hi = make_uint4(as_u(__hmax2(as_h2(hi.x), as_h2(y.x))), as_u(__hmax2(as_h2(hi.y), as_h2(y.y))),
-                                    as_u(__hmax2(as_h2(hi.z), as_h2(y.z))), as_u(__hmax2(as_h2(hi.w), as_h2(y.w))));
+                    mn = least8(mn, red[i][0][lane]);
+                    mx = largest8(mx, red[i][1][lane]);
                 }
             __syncthreads();   // the partial bounds are read before the next page's land on them
         }
         if (mate == 0 && sub == 0 && live) {
             __half *b = c.bounds + ((long long)id * c.HKV + g) * 2 * c.D + ch * 8;
-            *reinterpret_cast<uint4 *>(b) = lo;
-            *reinterpret_cast<uint4 *>(b + c.D) = hi;
+            *reinterpret_cast<uint4 *>(b) = mn;
+            *reinterpret_cast<uint4 *>(b + c.D) = mx;
         }
     }
 }
@@ -1417,6 +1407,8 @@ int score_launch(const SelectArgs &a, const KvCall &call, long long most) {
     return launched("kv_score");
 }
 
+// lanes that carry a row, 16 bytes each
+int row_lanes(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 }  // namespace
@@ -1495,9 +1487,9 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
         a.bad = call.d->err_dev + 2;
         *flag = 0;
     }
-    const int per = std::min(nt, c->page);
+    const int lpr = row_lanes(c->D), per = std::min(nt, c->page) * lpr / 32;   // rounds of one warp over a page's rows
     const int warps = std::min(8, std::max(1, (per + 3) / 4));
-    G9_CU(launch_pdl(kv_append_k, dim3((unsigned)a.tp, (unsigned)c->HKV, (unsigned)c->ns), dim3(32 * warps), 0, call.st, a));
+    G9_CU(launch_pdl(kv_append_k, dim3((unsigned)a.tp, (unsigned)c->HKV, (unsigned)c->ns), dim3(32 * warps), 0, call.st, a, lpr));
     G9_TRY(launched("kv_append"));
     const size_t marks = marks_bytes(a.c, ms, mh);
     const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};
@@ -1624,7 +1616,7 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     // a page per team, as many as can change (each mover changes one, and the last may lose slots), up to four waves of CTAs
     const long long most = std::min<long long>(a.pages, (long long)a.c.cap - a.keep + 1);
     const long long ctas = std::max<long long>(1, std::min<long long>((most + teams - 1) / teams, 4LL * MCTAS * call.d->sm_count / rows));
-    const int lpr = c->D <= 64 ? 8 : c->D <= 128 ? 16 : 32;
+    const int lpr = row_lanes(c->D);
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);

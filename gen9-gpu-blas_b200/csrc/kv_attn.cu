@@ -5,6 +5,7 @@
 #include "mma_sync.cuh"
 #include "sm100.cuh"
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -40,6 +41,14 @@ struct PagedArgs {
     float *lse2;              // log2 of the sum of 2^score, [(s, t, h)], with weights
 };
 
+constexpr float PSCALE = 64.0f;   // of the weights as FP16
+
+// 2^x, results below 2^-126 as 0
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void cp16(unsigned dst, const void *src, int bytes) {   // bytes 16, or 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -79,10 +88,10 @@ __device__ __forceinline__ int outer_steps(const PagedArgs &a, int o, int &k0, i
     return max(1, (k1 - k0 + AKEYS - 1) / AKEYS);
 }
 
-// Elements d .. d + 3 of output row q from the sum L of its weights, the greatest score M and the sums x of 2^14-fold weights.
+// Elements d .. d + 3 of output row q from the sum L of its weights, the greatest score M and the sums x of PSCALE-fold weights.
 __device__ __forceinline__ void paged_out(const PagedArgs &a, long long q, int d, float M, float L, float4 x) {
     const bool none = L == 0.0f;   // the row sees nothing
-    const float f = none ? 0.0f : 1.0f / 16384.0f / L;
+    const float f = none ? 0.0f : 1.0f / PSCALE / L;
     if (d < a.c.D) {
         float *out = a.O + q * a.c.D + d;
         if (a.o4) {
@@ -322,10 +331,15 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                 if (r >= live_rows) see[nt][j] = 0;
             }
 
+        float *srow[2];   // one tile: the rows' scores
+        if constexpr (W && NT == 1) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) srow[j] = a.score + (long long)__shfl_sync(kAll, my_q, 2 * tq + j) * a.score_row;
+        }
         float m[NT][2], l[NT][2], o[KT][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = -INFINITY;
+            m[nt][0] = m[nt][1] = -FLT_MAX;   // no score yet: the first seen one passes it
             l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < KT; dt++) o[dt][nt][0] = o[dt][nt][1] = o[dt][nt][2] = o[dt][nt][3] = 0.0f;
@@ -357,35 +371,72 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                 }
             }
             const int ka = kidx[stage * AKEYS + gq], kc = kidx[stage * AKEYS + gq + 8];
-            float p[NT][2][2], alpha[NT][2];   // weight of (key gq or gq + 8, row 8nt + 2tq + j)
+            // sc[nt][2e + j]: key gq + 8e, row 8nt + 2tq + j. Most steps are seen by every row as a whole.
+            const bool whole = __all_sync(kAll, min(ka, kc) >= kmin_all && max(ka, kc) < kmax_all);
+            if (!whole) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        if (ka >= see[nt][j] || ka < from[nt][j]) sc[nt][j] = -INFINITY;
+                        if (kc >= see[nt][j] || kc < from[nt][j]) sc[nt][2 + j] = -INFINITY;
+                    }
+            }
+            if constexpr (W) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
+                        float *sr = NT == 1 ? srow[j] : a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
+                        if (r < live_rows && at0 < k1) sr[at0] = sc[nt][j] * inv[nt][j];
+                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = sc[nt][2 + j] * inv[nt][j];
+                    }
+            }
+            // Weights are 2^(score - m) with m a greatest score of before: it is raised, and the sums scaled down, only when
+            // a score passes it by more than 8, so that most steps need no maximum over the lanes.
+            float p[NT][2][2];   // of (key gq + 8e, row 8nt + 2tq + j), at most 2^8
+            bool over = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float x0 = ka < see[nt][j] && ka >= from[nt][j] ? sc[nt][j] * inv[nt][j] : -INFINITY;
-                    const float x1 = kc < see[nt][j] && kc >= from[nt][j] ? sc[nt][2 + j] * inv[nt][j] : -INFINITY;
-                    if constexpr (W) {
-                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
-                        float *sr = a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
-                        if (r < live_rows && at0 < k1) sr[at0] = x0;
-                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = x1;
+                    p[nt][0][j] = fmaf(sc[nt][j], inv[nt][j], -m[nt][j]);
+                    p[nt][1][j] = fmaf(sc[nt][2 + j], inv[nt][j], -m[nt][j]);
+                    over = over || fmaxf(p[nt][0][j], p[nt][1][j]) > 8.0f;
+                }
+            if (__any_sync(kAll, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float mx = fmaxf(sc[nt][j], sc[nt][2 + j]);
+                        mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 16));
+                        const float mn = fmaxf(m[nt][j], mx * inv[nt][j]), alpha = ex2(m[nt][j] - mn);
+                        m[nt][j] = mn;
+                        l[nt][j] *= alpha;
+                        p[nt][0][j] = fmaf(sc[nt][j], inv[nt][j], -mn);
+                        p[nt][1][j] = fmaf(sc[nt][2 + j], inv[nt][j], -mn);
+#pragma unroll
+                        for (int dt = 0; dt < KT; dt++) {
+                            o[dt][nt][j] *= alpha;
+                            o[dt][nt][2 + j] *= alpha;
+                        }
                     }
-                    float mx = fmaxf(x0, x1);
-                    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 16));
-                    const float mn = fmaxf(m[nt][j], mx), ref = mn == -INFINITY ? 0.0f : mn;
-                    alpha[nt][j] = exp2f(m[nt][j] - ref);
-                    m[nt][j] = mn;
-                    p[nt][0][j] = exp2f(x0 - ref);
-                    p[nt][1][j] = exp2f(x1 - ref);
-                    l[nt][j] = fmaf(l[nt][j], alpha[nt][j], p[nt][0][j] + p[nt][1][j]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    p[nt][0][j] = ex2(p[nt][0][j]);
+                    p[nt][1][j] = ex2(p[nt][1][j]);
+                    l[nt][j] += p[nt][0][j] + p[nt][1][j];
                 }
             // A slot that some rows see and others do not has weight 0 for the others, but 0·V is not 0 where V is not
             // finite: such rows of V (a sound cache has none) are added to the rows that see them by hand, then cleared.
-            const bool odd = (ka != INT_MAX && (ka < kmin_all || ka >= kmax_all)) ||
-                             (kc != INT_MAX && (kc < kmin_all || kc >= kmax_all));
-            if (__any_sync(kAll, odd)) {
+            if (!whole) {
                 // element 2·lane (and + 1) of 64 of each row: which of the 16 rows hold something that is not finite
                 unsigned wild = 0;
 #pragma unroll
@@ -396,19 +447,6 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                         if ((w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u) wild |= 1u << kk;
                     }
                 wild = __reduce_or_sync(kAll, wild);
-                if (wild) {   // the running sums take the step's factor now
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                        for (int dt = 0; dt < KT; dt++) {
-                            o[dt][nt][0] *= alpha[nt][0];
-                            o[dt][nt][1] *= alpha[nt][1];
-                            o[dt][nt][2] *= alpha[nt][0];
-                            o[dt][nt][3] *= alpha[nt][1];
-                        }
-                        alpha[nt][0] = alpha[nt][1] = 1.0f;
-                    }
-                }
                 while (wild) {
                     const int kk = __ffs(wild) - 1, key = kidx[stage * AKEYS + kk];
                     wild &= wild - 1;
@@ -421,7 +459,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                             const float lo_p = __shfl_sync(kAll, p[nt][0][j], (kk & 7) * 4 + tq);
                             const float hi_p = __shfl_sync(kAll, p[nt][1][j], (kk & 7) * 4 + tq);
                             if (key >= see[nt][j] || key < from[nt][j]) continue;
-                            const float w = (kk < 8 ? lo_p : hi_p) * 16384.0f;
+                            const float w = (kk < 8 ? lo_p : hi_p) * PSCALE;
 #pragma unroll
                             for (int dt = 0; dt < KT; dt++) {
                                 o[dt][nt][j] += w * __half2float(vp[((2 * dt) ^ (kk & 7)) * 8 + gq]);
@@ -433,13 +471,14 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                     __syncwarp();
                 }
             }
-            // weights of up to 1 as up to 2^14, in two FP16 parts: what a weight loses is below 2^-39 of the largest
+            // the weights times 2^6 in two FP16 parts: what a weight loses is below 2^-31 of the greatest, whose weight is at
+            // least 1
             unsigned bh[NT][2], bl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 unsigned h0, l0, h1, l1;
-                at_split(p[nt][0][0] * 16384.0f, p[nt][0][1] * 16384.0f, h0, l0);
-                at_split(p[nt][1][0] * 16384.0f, p[nt][1][1] * 16384.0f, h1, l1);
+                at_split(p[nt][0][0] * PSCALE, p[nt][0][1] * PSCALE, h0, l0);
+                at_split(p[nt][1][0] * PSCALE, p[nt][1][1] * PSCALE, h1, l1);
                 bh[nt][0] = at_movt(h0);
                 bh[nt][1] = at_movt(h1);
                 bl[nt][0] = at_movt(l0);
@@ -456,10 +495,10 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     at_mma(x, af, bh[nt][0], bh[nt][1]);
                     at_mma(x, af, bl[nt][0], bl[nt][1]);
-                    o[dt][nt][0] = fmaf(o[dt][nt][0], alpha[nt][0], x[0]);
-                    o[dt][nt][1] = fmaf(o[dt][nt][1], alpha[nt][1], x[1]);
-                    o[dt][nt][2] = fmaf(o[dt][nt][2], alpha[nt][0], x[2]);
-                    o[dt][nt][3] = fmaf(o[dt][nt][3], alpha[nt][1], x[3]);
+                    o[dt][nt][0] += x[0];
+                    o[dt][nt][1] += x[1];
+                    o[dt][nt][2] += x[2];
+                    o[dt][nt][3] += x[3];
                 }
             }
         }
