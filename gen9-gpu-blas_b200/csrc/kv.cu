@@ -1492,8 +1492,8 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
     G9_CU(launch_pdl(kv_append_k, dim3((unsigned)a.tp, (unsigned)c->HKV, (unsigned)c->ns), dim3(32 * warps), 0, call.st, a, lpr));
     G9_TRY(launched("kv_append"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};
-    G9_TRY(kv_finish(call, sync, w, 4));
+    const KvWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};   // positions are no early reader's operand
+    G9_TRY(kv_finish(call, sync, w, 3));
     if (sync && bad) *bad = (int)*flag;
     return 0;
 }
@@ -1566,8 +1566,7 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
     else if (c->mp <= 8 * CT) G9_CU(launch_pdl(kv_choose_k<8>, grid, dim3(CT), 0, call.st, a));
     else G9_CU(launch_pdl(kv_choose_k<16>, grid, dim3(CT), 0, call.st, a));
     G9_TRY(launched("kv_choose"));
-    const KvWrite w[1] = {{sel, (size_t)rows * nsel * 4}};
-    return kv_finish(call, sync, w, 1);
+    return kv_finish(call, sync, nullptr, 0);   // page places are no early reader's operand
 }
 
 GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, int keep, int first, int recent, float *acc,
@@ -1620,8 +1619,8 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const KvWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {pos, marks}};
-    return kv_finish(call, sync, w, 4);
+    const KvWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};
+    return kv_finish(call, sync, w, 3);
 }
 
 }  // extern "C"

@@ -157,21 +157,25 @@ class PagedKV:
                              f"{x.device}")
         return x.data_ptr()
 
+    def _mark(self, name, x, dtype):
+        n, st = x.shape, x.stride()
+        if not (x.dtype is dtype and len(n) == 3 and n[0] == self.streams and n[1] == self.heads and n[2] >= self.slots and
+                x.get_device() == self._index and (st[2] == 1 or n[2] <= 1)):
+            raise ValueError(f"{name}: {dtype} [{self.streams}, {self.heads}, at least {self.slots}] on {self.device}, unit "
+                             f"stride last; got {x.dtype} {list(n)} on {x.device}")
+        return st
+
     def _marks(self, acc, pos):
-        st = None
-        for name, x, dt in (("acc", acc, _f32), ("pos", pos, _i32)):
-            if x is None:
-                continue
-            n = x.shape
-            if not (x.dtype is dt and len(n) == 3 and n[0] == self.streams and n[1] == self.heads and n[2] >= self.slots and
-                    x.get_device() == self._index and (x.stride(2) == 1 or n[2] <= 1)):
-                raise ValueError(f"{name}: {dt} [{self.streams}, {self.heads}, at least {self.slots}] on {self.device}, unit "
-                                 f"stride last; got {x.dtype} {list(n)} on {x.device}")
-            if st is not None and st != x.stride():
+        """Pointers of acc and pos, and the strides (stream, head) that they share."""
+        st = (0, 0)
+        if acc is not None:
+            st = self._mark("acc", acc, _f32)
+        if pos is not None:
+            other = self._mark("pos", pos, _i32)
+            if acc is not None and other != st:
                 raise ValueError("acc and pos differ in their strides")
-            st = x.stride()
-        return (None if acc is None else acc.data_ptr(), None if pos is None else pos.data_ptr(),
-                *((0, 0) if st is None else st[:2]))
+            st = other
+        return None if acc is None else acc.data_ptr(), None if pos is None else pos.data_ptr(), st[0], st[1]
 
     def _like(self, q, n):
         """A contiguous float32 tensor of q's shape."""
