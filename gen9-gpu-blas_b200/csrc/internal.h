@@ -53,12 +53,16 @@ struct DevState {
                                                                // grown; each call leaves every counter it used at 0)
     // Device ranges written by no-wait calls that may still be queued, each with an event recorded right after the
     // call that wrote it (an entry whose event has completed is dropped); a kernel that reads an input before
-    // griddepcontrol.wait checks its input against them.
+    // griddepcontrol.wait checks its input against them. An entry holds writes of one stream, and waiting for a stream
+    // drops that stream's entries only.
     static constexpr int kQueuedRanges = 32;
     uintptr_t queued_lo[kQueuedRanges] = {}, queued_hi[kQueuedRanges] = {};
     cudaEvent_t queued_ev[kQueuedRanges] = {};
+    cudaStream_t queued_st[kQueuedRanges] = {};
     int queued_n = 0;
-    bool queued_overflow = false;
+    bool queued_overflow = false, queued_overflow_many = false;   // a write that has no entry; such writes of several streams
+    cudaStream_t queued_overflow_st = nullptr;
+    bool queued_captured = false;   // captured calls have written ranges without an entry: later captured ones ask no more
     void *shard = nullptr;                                     // operand copies of a column-sharded GEMM (grow-only)
     size_t shard_n = 0;
     void *ml = nullptr;                                        // FP16 activations / results of the ML entry points
@@ -129,7 +133,8 @@ int finish_op(Operand *ops, int n);
 // library's stream has been waited for, and ask whether [p, p + bytes) may still be written by queued work (true also
 // when more ranges were queued than the ledger holds).
 void queued_writes_add(DevState *d, const void *p, size_t bytes, cudaStream_t st);
-void queued_writes_clear(DevState *d);
+void queued_writes_lost(DevState *d, cudaStream_t st);    // a write on st that has no entry
+void queued_writes_clear(DevState *d, cudaStream_t st);   // st has been waited for
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes);
 // Hand-over flags of the GEMM kernels that split tiles over CTAs (kGemmFlags zeroed words, created on first use) and
 // the epoch of the launch about to be enqueued (never 0).

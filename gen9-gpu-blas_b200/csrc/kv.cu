@@ -34,7 +34,7 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     if (c->page < 1 || c->n_pages < 0 || c->mp < 0 || c->ns < 0 || c->ts < 0)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: page = %d, n_pages = %d, mp = %d, ns = %d, ts = %lld", who, c->page,
                     c->n_pages, c->mp, c->ns, (long long)c->ts);
-    if ((long long)c->mp * c->page > INT_MAX - 64)
+    if ((long long)c->mp * c->page > INT_MAX - 65536)   // slots are counted in 32 bits, in steps of up to 6144
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %d pages of %d slots per stream pass 2^31 slots", who, c->mp, c->page);
     if ((long long)c->ns * c->HKV > INT_MAX)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %d streams of %d heads pass 2^31 rows", who, c->ns, c->HKV);
@@ -175,13 +175,12 @@ int kv_too_large(const char *who) { return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s:
 
 int kv_finish(const KvCall &call, int sync, const KvWrite *w, int n) {
     if (call.capturing) {
-        // a replay writes without passing here: later calls of this library treat any range as possibly being written
-        call.d->queued_overflow = true;
+        call.d->queued_captured = true;   // an event recorded here could not be queried
         return 0;
     }
     if (sync) {
         G9_CU(cudaStreamSynchronize(call.st));
-        queued_writes_clear(call.d);
+        queued_writes_clear(call.d, call.st);
         return check_dev_err(call.d);
     }
     for (int i = 0; i < n; i++)
@@ -832,7 +831,8 @@ __device__ __forceinline__ void pick_bin(const int *hist, int need, int *scan, i
     __syncthreads();
 }
 
-// A page's score in 64 bits, by one warp: the key of the largest over the heads h0 .. h1 - 1 (0: NaN, or no page).
+// A page's score in 64 bits, by one warp: the key of the largest over the heads h0 .. h1 - 1 (0: NaN, or no page). Both
+// products are taken, each exact: where a bound is not finite the sign of the query's element does not tell the larger.
 __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int s, int t, int g, int place, int h0, int h1) {
     const KvDev &c = a.c;
     const int lane = threadIdx.x & 31;
@@ -846,8 +846,8 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int
         double x = 0.0;
 #pragma unroll 4
         for (int d = lane; d < c.D; d += 32) {
-            const float v = q[d];
-            x = fma((double)v, (double)__half2float(v >= 0.0f ? hi[d] : lo[d]), x);
+            const double v = (double)q[d], y = v * (double)__half2float(lo[d]), z = v * (double)__half2float(hi[d]);
+            x += y >= z || y != y ? y : z;
         }
         for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kAll, x, o);
         nan = nan || x != x;
@@ -892,7 +892,8 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     for (int i = 0; i < CR; i++) x[i] = tid + i * CT < have ? __ldcg(score + tid + i * CT) : 0.0f;
     // ---- E = 2^-14 · max |q|_1 · max |bound| (2^-13 for D > 128): each of the 4·D/16 tensor-core steps adds 17 numbers, each cut
     // off at worst 2^-23 below the largest, which is at most |q|_1·|bound|, 2^-18.9 in all; 32 steps at D = 128 make 2^-13.9
-    // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21
+    // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21. 2^-126 more covers what scores and E
+    // itself lose where they fall below FP32's normal numbers
     float big = 0.0f, l1 = 0.0f;
     {
         const float *peak = a.peak + (((long long)s * c.HKV + g) * a.zs + t * a.hg / a.zt) * a.unit_steps;
@@ -920,7 +921,7 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
         big = fmaxf(big, red[0][w]);
         l1 = fmaxf(l1, red[1][w]);
     }
-    const float E = (c.D > 128 ? 0x1p-13f : 0x1p-14f) * l1 * big;
+    const float E = (c.D > 128 ? 0x1p-13f : 0x1p-14f) * l1 * big + 0x1p-126f;
     const bool full = at == kAll;   // enough pages that are always taken: the lowest of them
     const float tau = __uint_as_float(at & 0x80000000u ? at & 0x7fffffffu : ~at);
     const bool know = E < INFINITY && at != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
@@ -966,7 +967,11 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
                 }
             }
             __syncthreads();
-            auto rank_key = [&](int i) { return lnan[i] ? 0ull : lkey[i]; };
+            if (nb > r) {   // a NaN of one head makes the page's score NaN
+                for (int i = tid; i < nb; i += CT)
+                    if (lnan[i]) lkey[i] = 0ull;
+                __syncthreads();
+            }
             for (int i = tid; i < nb; i += CT) {
                 int better = 0;
                 if (nb > r)
@@ -1465,7 +1470,7 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
     if (pos) G9_TRY(kv_operand(call, pos, who, "pos"));
     if (pos && pos0) G9_TRY(kv_operand(call, pos0, who, "pos0"));
     a.nt = nt;
-    a.tp = (nt - 1) / c->page + 2;   // nt slots from anywhere in a page
+    a.tp = std::min((nt - 1) / c->page, c->mp - 1) + 2;   // nt slots from anywhere in a page; one behind the table tells bad
     a.K = K;
     a.V = V;
     a.kt = kt;

@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
     const int vs = a.vis[s];
     if (!a.sel) {
         const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
-        if (k >= seen_slots(vs, a.dvis, a.nq - 1, c.cap)) return;
+        if (k >= seen_slots(vs, a.dvis, a.nq - 1, c.cap) || k + 3 < first_slot(seen_slots(vs, a.dvis, 0, c.cap), a.window)) return;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int t = 0; t < a.nq; t++) {
             const int see = seen_slots(vs, a.dvis, t, c.cap), from = first_slot(see, a.window);

@@ -245,7 +245,7 @@ int gemm_sharded(int type, int tA, int tB, int M, int N, int K, double alpha, co
     G9_CU(cudaSetDevice(home));
     bool home_synced = false;
     for (int i = 0; i < launched_n; i++) home_synced = home_synced || g_shard.ids[i] == home;
-    if (home_synced) queued_writes_clear(hd);   // the caller's stream was waited for
+    if (home_synced) queued_writes_clear(hd, stream());   // the caller's stream was waited for
     G.last_zc = 0;
     if (first_err) {
         memcpy(G.err, msg, sizeof msg);

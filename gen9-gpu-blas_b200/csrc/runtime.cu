@@ -326,6 +326,7 @@ static void queued_drop(DevState *d, int i) {
         cudaEvent_t e = d->queued_ev[i];
         d->queued_ev[i] = d->queued_ev[last];
         d->queued_ev[last] = e;
+        d->queued_st[i] = d->queued_st[last];
     }
     d->queued_n = last;
 }
@@ -341,41 +342,67 @@ void queued_writes_add(DevState *d, const void *p, size_t bytes, cudaStream_t st
     if (!bytes) return;
     const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
     int slot = -1;
-    for (int i = 0; i < d->queued_n && slot < 0; i++)   // a range that overlaps or touches an entry widens it
-        if (lo <= d->queued_hi[i] && d->queued_lo[i] <= hi) slot = i;
+    for (int i = 0; i < d->queued_n && slot < 0; i++)   // a range that overlaps or touches an entry of its stream widens it
+        if (lo <= d->queued_hi[i] && d->queued_lo[i] <= hi && d->queued_st[i] == st) slot = i;
     if (slot < 0 && d->queued_n == DevState::kQueuedRanges)
         for (int i = d->queued_n - 1; i >= 0; i--)       // full: forget the writes that have completed
             if (queued_done(d, i)) queued_drop(d, i);
+    if (slot < 0 && d->queued_n == DevState::kQueuedRanges) {   // still full: the entry of the stream that grows least takes it in
+        size_t least = SIZE_MAX;
+        for (int i = 0; i < d->queued_n; i++) {
+            if (d->queued_st[i] != st) continue;
+            const size_t grown = lo < d->queued_lo[i] ? d->queued_lo[i] - lo : hi > d->queued_hi[i] ? hi - d->queued_hi[i] : 0;
+            if (grown < least) {
+                least = grown;
+                slot = i;
+            }
+        }
+    }
     if (slot < 0) {
-        if (d->queued_n == DevState::kQueuedRanges) {    // still full: every later check answers "maybe written"
-            d->queued_overflow = true;
+        if (d->queued_n == DevState::kQueuedRanges) {    // none of its stream: every later check answers "maybe written"
+            queued_writes_lost(d, st);
             return;
         }
         slot = d->queued_n++;
         d->queued_lo[slot] = lo;
         d->queued_hi[slot] = hi;
+        d->queued_st[slot] = st;
     } else {
         if (lo < d->queued_lo[slot]) d->queued_lo[slot] = lo;
         if (hi > d->queued_hi[slot]) d->queued_hi[slot] = hi;
     }
     if (!d->queued_ev[slot] && cudaEventCreateWithFlags(&d->queued_ev[slot], cudaEventDisableTiming) != cudaSuccess) {
         cudaGetLastError();
-        d->queued_overflow = true;   // cannot tell when it completes: stay conservative
+        queued_writes_lost(d, st);   // cannot tell when it completes: stay conservative
         return;
     }
     if (cudaEventRecord(d->queued_ev[slot], st) != cudaSuccess) {
         cudaGetLastError();
-        d->queued_overflow = true;
+        queued_writes_lost(d, st);
     }
 }
 
-void queued_writes_clear(DevState *d) {
-    d->queued_n = 0;
-    d->queued_overflow = false;
+void queued_writes_lost(DevState *d, cudaStream_t st) {
+    d->queued_overflow_many = d->queued_overflow && (d->queued_overflow_many || d->queued_overflow_st != st);
+    d->queued_overflow = true;
+    d->queued_overflow_st = st;
+}
+
+void queued_writes_clear(DevState *d, cudaStream_t st) {
+    for (int i = d->queued_n - 1; i >= 0; i--)
+        if (d->queued_st[i] == st) queued_drop(d, i);
+    if (d->queued_overflow_st == st && !d->queued_overflow_many) d->queued_overflow = false;
 }
 
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
     if (d->queued_overflow) return true;
+    if (d->queued_captured) {   // calls outside a capture start after a replayed graph as a whole
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream(), &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            return true;
+        }
+    }
     const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
     for (int i = d->queued_n - 1; i >= 0; i--) {
         if (!(lo < d->queued_hi[i] && d->queued_lo[i] < hi)) continue;
@@ -405,7 +432,7 @@ int finish_op(Operand *ops, int n) {
             G9_CU(cudaMemcpyAsync(const_cast<void *>(ops[i].user), ops[i].dptr, ops[i].bytes, cudaMemcpyDeviceToHost, st));
     }
     G9_CU(cudaStreamSynchronize(st));
-    queued_writes_clear(d);
+    queued_writes_clear(d, st);
     return check_dev_err(d);
 }
 
@@ -613,7 +640,7 @@ GEN9BLAS_API int gen9blas_ipc_close(void *peer_ptr) {
 GEN9BLAS_API int gen9blas_flush(void) {
     if (begin_op()) return G.status;
     G9_CU(cudaStreamSynchronize(stream()));
-    queued_writes_clear(dev_state());
+    queued_writes_clear(dev_state(), stream());
     return check_dev_err(dev_state());
 }
 

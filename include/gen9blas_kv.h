@@ -43,7 +43,8 @@ GEN9BLAS_API int gen9blas_kv_supported(int D, int H, int HKV);
 /* Workspace of attn_paged, kv_select and kv_evict. NULL in a call means the library's own one of the device: calls that
  * share a workspace run one after the other (one on another stream than the last first waits for the device). A call
  * that is captured into a CUDA graph needs a workspace of its own here, large enough from an earlier call of the same
- * shape outside the capture (GEN9BLAS_ERR_INVALID_ARG otherwise); graphs that share one must not run at the same time.
+ * shape outside the capture (GEN9BLAS_ERR_INVALID_ARG otherwise); a replay must not run at the same time as another
+ * replay or call that uses its workspace: the library does not see replays, so that order is the caller's.
  * kv_ws_free waits for the device; the graphs that use the workspace must not run after it. */
 typedef struct gen9blas_kv_ws gen9blas_kv_ws;
 GEN9BLAS_API gen9blas_kv_ws *gen9blas_kv_ws_create(void);
@@ -52,9 +53,9 @@ GEN9BLAS_API void gen9blas_kv_ws_free(gen9blas_kv_ws *ws);
 /* Writes nt new tokens per stream: slots len[s] + t, t < min(cnt[s], nt) (cnt NULL: nt; a negative len or cnt counts as
  * 0). K and V: F32, element d of (token t, head g, stream s) at K[t·kt + g·kh + s·ks + d], rounded to FP16 (nearest
  * even). With bounds in the cache, the bounds of the pages written are set (slot 0 of the page among the new ones) or
- * widened. acc and pos (each NULL or element k of (s, g) at acc[s·ms + g·mh + k]): acc = 0, pos = pos0[s] + t (pos0 NULL:
- * the slot's number) for the new slots. Tokens past mp·page or without a page are dropped; with sync = 1, *bad (NULL
- * allowed) = 1 if there were any, else 0. len is not changed. */
+ * widened, NaN elements left out (+inf and -inf if there is no other). acc and pos (each NULL or element k of (s, g) at
+ * acc[s·ms + g·mh + k]): acc = 0, pos = pos0[s] + t (pos0 NULL: the slot's number) for the new slots. Tokens past mp·page
+ * or without a page are dropped; with sync = 1, *bad (NULL allowed) = 1 if there were any, else 0. len is not changed. */
 GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const float *K, int64_t kt, int64_t kh, int64_t ks,
                                     const float *V, int64_t vt, int64_t vh, int64_t vs, const int *len, const int *cnt,
                                     float *acc, int *pos, int64_t ms, int64_t mh, const int *pos0, int sync, int *bad);
@@ -64,7 +65,7 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
  * at Q[t·qt + h·qh + s·qs + d]; query head h reads key-value head h / (H / HKV). lse (NULL or [s][t][h]): log of the sum of
  * exp(score). A token that sees nothing gets O = 0, lse = -inf. dvis and window >= 0.
  * What lies in slots that a token does not see (NaN, infinities) does not enter its result; a seen key or value that is
- * not finite makes the results of the heads that see it not finite.
+ * not finite enters as the formula has it (NaN, as a rule; a score of -inf has no weight), for the heads that see it only.
  * sel (NULL or int [s][t][HKV][nsel]): only the slots of the listed pages, given by their place k / page in the stream,
  * ascending; an entry that is negative, not below mp or not above the one before it is skipped. Not with window > 0.
  * acc (NULL or as in kv_append): acc[k] += the softmax weights that slot k got from all tokens and query heads of the
@@ -77,7 +78,8 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
 /* Pages for the attention above: for each (s, t, g), sel[s][t][g][0 .. nsel) = places of the pages that count among those
  * holding visible slots (vt as above): the first `first` and the last `last` of them, then those with the largest score
  * max over the head's queries of sum_d max(q_d·lo_d, q_d·hi_d) -- no key of the page has a larger q·k -- ties to the
- * lowest place; ascending, -1 behind if there are fewer than nsel. The sums are taken in 64 bits. A NaN score and a place
+ * lowest place; ascending, -1 behind if there are fewer than nsel. The sums are taken in 64 bits; lo <= hi in bounds that
+ * are finite. A NaN score and a place
  * without a page rank last. first, last >= 0; if they are more than nsel, the lowest places among them. Needs bounds. */
 GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, const float *Q, int64_t qt, int64_t qh,
                                     int64_t qs, const int *vis, int dvis, int first, int last, int nsel, int *sel,

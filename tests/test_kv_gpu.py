@@ -358,6 +358,37 @@ def test_select_near_ties_follow_the_exact_order(kv):
     assert np.array_equal(got.cpu().numpy(), kv_ref.select(host, q, [n], 10, first=0, last=0))
 
 
+def test_select_a_nan_of_one_head_ranks_the_page_last(kv):
+    """Infinite bounds against a query element of zero: NaN for that head, +inf or a number for the others of its group."""
+    rng = np.random.default_rng(31)
+    n, D = 40, 64
+    K = torch.zeros(n, 1, 1, D, dtype=torch.float16, device="cuda")
+    bounds = np.sort(rng.standard_normal((n, 1, 2, D)).astype(np.float16), axis=2)
+    bounds[3::5, 0, 1, 0] = np.inf
+    bounds[4::10, 0, 0, 1] = -np.inf
+    bounds[9, 0, 0, 2], bounds[9, 0, 1, 2] = np.inf, -np.inf     # a page all of whose keys are NaN there
+    q = rng.standard_normal((1, 3, 4, D)).astype(np.float32)
+    q[:, :, :, 0] = [[[0.0, 1.0, -1.0, 2.0], [1.0, 1.0, 2.0, 3.0], [-1.0, -2.0, -1.0, -3.0]]]
+    q[:, :, :, 1] = [[[1.0, 1.0, 1.0, 1.0], [1.0, 0.0, 1.0, -1.0], [-1.0, -2.0, -1.0, -3.0]]]
+    table = np.arange(n, dtype=np.int32)[None]
+    host = {"K": K.cpu().numpy(), "V": K.cpu().numpy(), "bounds": bounds, "table": table}
+    cache = kv.PagedKV(K, K, ints(table), bounds=torch.from_numpy(bounds).cuda())
+    for m in (1, 3, 10, 30, 35):
+        got = cache.select(torch.from_numpy(q).cuda(), ints([n - 2]), m, first=0, last=0).cpu().numpy()
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(got, kv_ref.select(host, q, [n - 2], m, first=0, last=0)), m
+
+
+@pytest.mark.parametrize("size", [1e-44, 3e-42, 1e-38, 1e-30, 1e30, 3e38])
+def test_select_with_queries_at_the_ends_of_float32(kv, size):
+    """Scores that FP32 rounds to a few units of its least number, or to infinity, still rank as their 64-bit values."""
+    rng = np.random.default_rng(32)
+    host, K, V, table, bounds = make(rng, [16 * 60], 16, 2, 64)
+    q = (np.clip(rng.standard_normal((1, 1, 4, 64)), -1, 1) * size).astype(np.float32)
+    got = kv.PagedKV(K, V, table, bounds=bounds).select(torch.from_numpy(q).cuda(), ints([16 * 60]), 12, first=0, last=0)
+    assert np.array_equal(got.cpu().numpy(), kv_ref.select(host, q, [16 * 60], 12, first=0, last=0))
+
+
 @pytest.mark.parametrize("n,m", [(3000, 700), (600, 30)])
 def test_select_many_equal_pages(kv, n, m):
     """Hundreds of pages with the same bounds, some infinite or missing: the lowest places of the equal ones."""
@@ -639,3 +670,56 @@ def test_queued_write_is_seen_by_the_contiguous_attention(kv, gpu_lib):
         ref = kv_ref.attend(host, q.cpu().numpy(), [n])
         _, lse = cache.attend(q, vis, lse=True)
         attend_close((O, lse), ref, D)
+
+
+def test_waiting_on_one_stream_keeps_the_writes_queued_on_another(kv, gpu_lib):
+    """As above, with a waiting call on another stream between the write and the read: the write is still in the ledger."""
+    D, heads, n = 128, 2, 4096
+    K = torch.zeros(1, heads, n, D, dtype=torch.float16, device="cuda")
+    V = torch.zeros_like(K)
+    q = torch.randn(1, 1, 8, D, device="cuda")
+    O = torch.empty(1, 1, 8, D, device="cuda")
+    cache = kv.PagedKV(K, V, ints([[0]]))
+    small = torch.zeros(2, 1, heads, 16, D, dtype=torch.float16, device="cuda")
+    other = kv.PagedKV(small[0], small[1], ints([[0]]))
+    one = torch.randn(1, 1, heads, D, device="cuda")
+    vis, zero = ints([n]), ints([0])
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for it in range(5):
+        k, v = (torch.randn(1, n, heads, D, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            for _ in range(20):
+                cache.append(k, v, zero)
+        with torch.cuda.stream(b):
+            assert other.append(one, one, zero, wait=True) is True
+        with torch.cuda.stream(a):
+            cache.append(k, v, zero)
+        assert gpu_lib.set_stream(a.cuda_stream) == 0
+        size = K.numel() * 2
+        status = gpu_lib.attn_dec(D, 8, heads, 1, 1, n, q.data_ptr(), 8 * D, D, 8 * D, K.data_ptr(), D, n * D, heads * n * D, size,
+                                  V.data_ptr(), D, n * D, heads * n * D, size, O.data_ptr(), D ** -0.5, vis.data_ptr(), 0, 0, 0)
+        assert gpu_lib.set_stream(None) == 0
+        torch.cuda.synchronize()
+        assert status == 0
+        host = {"K": k.half().cpu().numpy().transpose(0, 2, 1, 3), "V": v.half().cpu().numpy().transpose(0, 2, 1, 3),
+                "table": np.zeros((1, 1), np.int32), "bounds": None}
+        _, lse = cache.attend(q, vis, lse=True)
+        attend_close((O, lse), kv_ref.attend(host, q.cpu().numpy(), [n]), D)
+
+
+def test_append_of_more_tokens_than_the_table_holds(kv):
+    """The launch covers the table and one page behind it; what passes it is dropped and told."""
+    heads, D, page = 1, 8, 4
+    K, V = (torch.zeros(3, heads, page, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    cache = kv.PagedKV(K, V, ints([[0, 1], [2, -1]]))
+    k = torch.arange(1, 1 + 2 * 1000 * D, device="cuda", dtype=torch.float32).reshape(2, 1000, 1, D) / 64
+    assert cache.append(k, -k, ints([3, 0]), count=ints([5, 4]), wait=True) is True
+    assert cache.append(k, -k, ints([3, 0]), wait=True) is False
+    want = torch.zeros(3, page, D)
+    flat = k[:, :, 0].cpu().half().float()
+    want[0, 3], want[1], want[2] = flat[0, 0], flat[0, 1:5], flat[1, :4]
+    assert torch.equal(K[:, 0].cpu().float(), want) and torch.equal(V[:, 0].cpu().float(), -want)
+    for at in (8, 9, 2 ** 31 - 1):                                    # behind the table altogether
+        assert cache.append(k, k, ints([at, at]), wait=True) is False
+    assert torch.equal(K[:, 0].cpu().float(), want)
