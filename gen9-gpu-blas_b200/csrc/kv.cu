@@ -88,6 +88,25 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     return 0;
 }
 
+int kv_marks_apart(const gen9blas_kv_cache *c, bool used, int64_t ms, int64_t mh, const char *who) {
+    if (!c || !used) return 0;
+    const long long cap = (long long)c->mp * c->page;
+    if ((c->ns > 1 && ms < cap) || (c->HKV > 1 && mh < cap))
+        return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: rows of acc or pos overlap: strides %lld and %lld, %lld slots", who,
+                    (long long)ms, (long long)mh, cap);
+    return 0;
+}
+
+int kv_rows_apart(const gen9blas_kv_cache *c, const char *who) {
+    if (!c) return 0;
+    const int64_t st[6] = {c->kp, c->kk, c->kh, c->vp, c->vk, c->vh};
+    const int n[3] = {c->n_pages, c->page, c->HKV};
+    for (int i = 0; i < 6; i++)
+        if (n[i % 3] > 1 && c->n_pages > 0 && st[i] < c->D)
+            return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: rows of K or V overlap: a stride of %lld elements", who, (long long)st[i]);
+    return 0;
+}
+
 int kv_operand(const KvCall &call, const void *p, const char *who, const char *name) {
     cudaPointerAttributes a;
     if (!p) return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: no %s", who, name);
@@ -1458,6 +1477,8 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
     AppendArgs a{};
     KvCall call;
     if (bad) *bad = 0;
+    G9_TRY(kv_rows_apart(c, who));
+    G9_TRY(kv_marks_apart(c, acc || pos, ms, mh, who));
     if (int e = kv_begin(c, 0, sync, who, &a.c, &call)) return e;
     if (c->ns == 0 || nt <= 0) return 0;
     if (c->ns > 65535 || c->HKV > 65535)
@@ -1581,6 +1602,8 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     KvCall call;
     if (c && (keep < 1 || first < 0 || recent < 0 || (long long)first + recent > keep))
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: keep = %d, first = %d, recent = %d", who, keep, first, recent);
+    G9_TRY(kv_rows_apart(c, who));
+    G9_TRY(kv_marks_apart(c, true, ms, mh, who));
     if (int e = kv_begin(c, 0, sync, who, &a.c, &call)) return e;
     if (c->ns == 0) return 0;
     G9_TRY(kv_operand(call, len, who, "len"));

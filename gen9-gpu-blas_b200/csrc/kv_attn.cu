@@ -741,6 +741,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
                     sel && window > 0 ? ": chosen pages and a window together" : "");
     if (c && sel && (long long)nsel * c->page > INT_MAX - 64)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: %d chosen pages of %d slots pass 2^31", who, nsel, c->page);
+    G9_TRY(kv_marks_apart(c, acc != nullptr, ms, mh, who));
     if (int e = kv_begin(c, H, sync, who, &a.c, &call)) return e;
     if (c->ns == 0 || nq <= 0) return 0;
     G9_TRY(kv_operand(call, Q, who, "Q"));

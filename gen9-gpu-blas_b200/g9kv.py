@@ -11,8 +11,8 @@
 K and V: float16 [pages, kv heads, page size, head size], unit stride in the last dimension, any others a multiple of 8
 elements (so both [page][head][slot] and [page][slot][head] pools serve, the latter as a permuted view). table: int32
 [streams, pages per stream], -1 where a stream has no page. q, k, v: float32 [streams, tokens, heads, head size], unit
-stride in the last dimension. Everything lies on one GPU; calls run on torch's current stream and do not wait. Shape and
-type errors raise ValueError, library errors RuntimeError with gen9blas_error().
+stride in the last dimension. Everything lies on one GPU; calls run on torch's current stream and do not wait. They are for
+serving: results carry no gradient. Shape and type errors raise ValueError, library errors RuntimeError with gen9blas_error().
 
 One cache object is used by one thread at a time, as the library is. A captured call (torch.cuda.graph) needs a workspace
 of its own: pass `workspace=g9kv.Workspace()` to the constructor and make one call of each shape before the capture.
@@ -55,6 +55,7 @@ if _raw_stream is None:
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 _f32, _i32 = torch.float32, torch.int32
+_END = 2 ** 31   # of the library's counts; ctypes would cut larger ones short without a word
 
 
 def _check(status, what):
@@ -209,6 +210,8 @@ class PagedKV:
         ns, nq, h, d = n
         see = self._ints("visible", visible)
         a, _, ms, mh = self._marks(acc, None) if acc is not None else (None, None, 0, 0)
+        if not (-_END <= step < _END and -_END <= window < _END):
+            raise ValueError(f"step = {step}, window = {window}")
         nsel = 0
         sp = None
         if sel is not None:
@@ -235,6 +238,8 @@ class PagedKV:
         """The `pages` pages that each token and kv head attends to: the first and the last ones it sees, then those whose
         bounds allow the largest q·k. int32 [streams, tokens, kv heads, pages], ascending, -1 behind."""
         n, qs = self._rows("q", q, None)
+        if not (max(step, first, last, pages) < _END and 0 <= min(step, first, last, pages)):
+            raise ValueError(f"step = {step}, first = {first}, last = {last}, pages = {pages}")
         if out is None:
             out = q.new_empty((n[0], n[1], self.heads, pages), dtype=_i32)
         else:
@@ -249,6 +254,8 @@ class PagedKV:
         Returns the new lengths."""
         a, p, ms, mh = self._marks(acc, pos)
         n = self._ints("length", length)
+        if not (max(keep, first, recent) < _END and 0 <= min(keep, first, recent)):
+            raise ValueError(f"keep = {keep}, first = {first}, recent = {recent}")
         if out is None:
             out = torch.empty_like(length)
         else:

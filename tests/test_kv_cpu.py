@@ -138,6 +138,23 @@ def test_arguments_that_are_refused(kv):
     assert kv._fn["kv_supported"](128, 32, 8) == 1 and kv._fn["kv_supported"](128, 32, 5) == 0
 
 
+def test_what_a_call_writes_must_not_overlap_itself(kv):
+    """Broadcast rows (stride 0) or rows closer than their length, of the pool, acc or pos, where a call writes them."""
+    buf = ctypes.create_string_buffer(40000)
+    c, q = _cache(kv, buf), ctypes.addressof(buf)
+    append, evict, attn = kv._fn["kv_append"], kv._fn["kv_evict"], kv._fn["attn_paged"]
+    tokens = (1, q, 64, 64, 64, q, 64, 64, 64, q, None)
+    for over in (dict(kp=0), dict(kh=0), dict(kk=56), dict(vh=0), dict(vp=32), dict(vk=0)):
+        bad = _cache(kv, buf, **over)
+        assert append(bad, *tokens, None, None, 0, 0, None, 0, None) == -3 and b"overlap" in kv._fn["error"]()
+        assert evict(bad, q, 8, 0, 0, q, None, 64, 32, q, None, 0) == -3 and b"overlap" in kv._fn["error"]()
+    for ms, mh in ((0, 32), (31, 32), (64, 0), (64, 31)):
+        assert append(c, *tokens, q, None, ms, mh, None, 0, None) == -3 and b"overlap" in kv._fn["error"]()
+        assert append(c, *tokens, None, q, ms, mh, None, 0, None) == -3 and b"overlap" in kv._fn["error"]()
+        assert evict(c, q, 8, 0, 0, q, None, ms, mh, q, None, 0) == -3 and b"overlap" in kv._fn["error"]()
+        assert attn(c, 4, 1, q, 256, 64, 256, q, 1, 0, None, 0, 1.0, q, None, q, ms, mh, None, 0) == -3 and b"overlap" in kv._fn["error"]()
+
+
 def test_python_face_checks_types(kv):
     torch = pytest.importorskip("torch")
     with pytest.raises(ValueError, match="float16"):

@@ -638,6 +638,14 @@ def test_refusals_on_the_device(kv, gpu_lib):
         cache.attend(torch.randn(1, 1, 3, 64, device="cuda"), n)           # 3 query heads over 2
     with pytest.raises(RuntimeError, match="bounds"):
         kv.PagedKV(K, V, table).select(q, n, 2)
+    wide = 2 ** 32 + 4                                                     # 4 in 32 bits
+    for call in (lambda: cache.attend(q, n, window=wide), lambda: cache.attend(q, n, step=wide),
+                 lambda: cache.select(q, n, 2, first=wide), lambda: cache.evict(n, wide, torch.zeros(1, 2, 32, device="cuda")),
+                 lambda: cache.evict(n, 8, torch.zeros(1, 2, 32, device="cuda"), recent=wide)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError, match="overlap"):
+        cache.attend(q, n, acc=torch.zeros(1, 1, 32, device="cuda").expand(1, 2, 32))
     hostv = (ctypes.c_int * 4)(20)
     args = (4, 1, q.data_ptr(), 256, 64, 256, ctypes.addressof(hostv), 1, 0, None, 0, 0.125, q.data_ptr(), None, None, 0, 0, None, 0)
     assert kv._fn["attn_paged"](cache._c, *args) == -3 and b"vis" in kv._fn["error"]()
