@@ -57,7 +57,9 @@ struct DevState {
     // drops that stream's entries only.
     static constexpr int kQueuedRanges = 32;
     uintptr_t queued_lo[kQueuedRanges] = {}, queued_hi[kQueuedRanges] = {};
-    cudaEvent_t queued_ev[kQueuedRanges] = {};
+    int queued_ev[kQueuedRanges] = {};                         // the entry's event: ranges of one call share one
+    cudaEvent_t queued_evs[kQueuedRanges + 1] = {};
+    int queued_ev_used[kQueuedRanges + 1] = {};                // entries that hold it
     cudaStream_t queued_st[kQueuedRanges] = {};
     int queued_n = 0;
     bool queued_overflow = false, queued_overflow_many = false;   // a write that has no entry; such writes of several streams
@@ -132,7 +134,11 @@ int finish_op(Operand *ops, int n);
 // Ledger of the outputs of queued no-wait calls (see DevState::queued_lo): add a range, forget them all once the
 // library's stream has been waited for, and ask whether [p, p + bytes) may still be written by queued work (true also
 // when more ranges were queued than the ledger holds).
-void queued_writes_add(DevState *d, const void *p, size_t bytes, cudaStream_t st);
+struct QueuedWrite {
+    const void *p;   // NULL: none
+    size_t bytes;
+};
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st);   // the ranges of one call
 void queued_writes_lost(DevState *d, cudaStream_t st);    // a write on st that has no entry
 void queued_writes_clear(DevState *d, cudaStream_t st);   // st has been waited for
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes);

@@ -192,7 +192,7 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
 
 int kv_too_large(const char *who) { return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s: the call's workspace passes 2^46 bytes", who); }
 
-int kv_finish(const KvCall &call, int sync, const KvWrite *w, int n) {
+int kv_finish(const KvCall &call, int sync, const QueuedWrite *w, int n) {
     if (call.capturing) {
         call.d->queued_captured = true;   // an event recorded here could not be queried
         return 0;
@@ -202,8 +202,7 @@ int kv_finish(const KvCall &call, int sync, const KvWrite *w, int n) {
         queued_writes_clear(call.d, call.st);
         return check_dev_err(call.d);
     }
-    for (int i = 0; i < n; i++)
-        if (w[i].p) queued_writes_add(call.d, w[i].p, w[i].bytes, call.st);
+    queued_writes_add(call.d, w, n, call.st);
     return 0;
 }
 
@@ -875,13 +874,14 @@ __device__ __forceinline__ unsigned long long exact_key(const SelectArgs &a, int
     return nan ? 0ull : score_key(best);
 }
 
-constexpr int CT = 256, CLIST = 512;   // threads, pages decided by hand in shared memory
+constexpr int CLIST = 512;   // pages decided by hand in shared memory
 // One CTA per row (s, t, g). Keys are the FP32 scores' order-preserving bits (pages that are always taken above all); tau is
 // the nsel-th largest. With E the bound of a score's error, a page above tau + 2E is taken, one below tau - 2E is not: nsel pages
 // have scores of at least tau - E, and fewer than nsel more than tau + E. The pages between are ranked by their 64-bit scores.
 // CR: scores a thread holds in registers, as many as the table's pages need (more are read again where they are used).
-template <int CR>
+template <int CT, int CR>
 __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ SelectArgs a) {
+    constexpr int CBITS = CT == 256 ? 9 : CT == 512 ? 10 : 11;   // of a digit of the 64-bit keys: 2·CT bins
     __shared__ NthKey nth;
     __shared__ int hist[2 * CT], scan[32], got[3];
     __shared__ int order[CR * CT / 32];
@@ -1009,8 +1009,8 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
             __syncthreads();
             unsigned long long pre = 0, msk = 0;
             int left = r;
-            for (int shift = 55; shift >= -8; shift -= 9) {   // 2·CT bins
-                const int sh = max(shift, 0), bits = shift < 0 ? 1 : 9;
+            for (int shift = 64 - CBITS; shift > -CBITS; shift -= CBITS) {   // 2·CT bins
+                const int sh = max(shift, 0), bits = min(CBITS + shift, CBITS);
                 for (int i = tid; i < 2 * CT; i += CT) hist[i] = 0;
                 __syncthreads();
                 for (int i = tid; i < (have + CT - 1) / CT * CT; i += CT) {
@@ -1518,7 +1518,7 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
     G9_CU(launch_pdl(kv_append_k, dim3((unsigned)a.tp, (unsigned)c->HKV, (unsigned)c->ns), dim3(32 * warps), 0, call.st, a, lpr));
     G9_TRY(launched("kv_append"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const KvWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};   // positions are no early reader's operand
+    const QueuedWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};   // positions are no early reader's operand
     G9_TRY(kv_finish(call, sync, w, 3));
     if (sync && bad) *bad = (int)*flag;
     return 0;
@@ -1588,10 +1588,22 @@ GEN9BLAS_API int gen9blas_kv_select(const gen9blas_kv_cache *c, int H, int nq, c
         else G9_TRY(score_launch<256>(a, call, most));
     }
     const dim3 grid((unsigned)rows);
-    if (c->mp <= 4 * CT) G9_CU(launch_pdl(kv_choose_k<4>, grid, dim3(CT), 0, call.st, a));
-    else if (c->mp <= 8 * CT) G9_CU(launch_pdl(kv_choose_k<8>, grid, dim3(CT), 0, call.st, a));
-    else G9_CU(launch_pdl(kv_choose_k<16>, grid, dim3(CT), 0, call.st, a));
-    G9_TRY(launched("kv_choose"));
+    // Threads of a row: 512; 1024 for long rows that all fit on the GPU (scoring and choosing of 128 rows of 2048 pages 37.0 µs,
+    // 39.8 with 512, 41.6 with 256; 512 rows of 1500 pages 118, 104 and 153; 8 rows of 1250 pages 15.7, 14.7 and 16.7); 256
+    // where they hold all (8 rows of 256 pages 11.1, 12.3 with 512). Rows longer than the registers hold read the rest again in
+    // every round.
+    const auto choose = [&](auto kernel, int threads) -> int {
+        G9_CU(launch_pdl(kernel, grid, dim3((unsigned)threads), 0, call.st, a));
+        return launched("kv_choose");
+    };
+    if (c->mp <= 256) G9_TRY(choose(kv_choose_k<256, 1>, 256));
+    else if (c->mp <= 1024) G9_TRY(choose(kv_choose_k<512, 2>, 512));
+    else if (rows <= call.d->sm_count && c->mp > 1536) {
+        if (c->mp <= 2048) G9_TRY(choose(kv_choose_k<1024, 2>, 1024));
+        else if (c->mp <= 4096) G9_TRY(choose(kv_choose_k<1024, 4>, 1024));
+        else G9_TRY(choose(kv_choose_k<1024, 8>, 1024));
+    } else if (c->mp <= 2048) G9_TRY(choose(kv_choose_k<512, 4>, 512));
+    else G9_TRY(choose(kv_choose_k<512, 16>, 512));
     return kv_finish(call, sync, nullptr, 0);   // page places are no early reader's operand
 }
 
@@ -1647,7 +1659,7 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const KvWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};
+    const QueuedWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};
     return kv_finish(call, sync, w, 3);
 }
 

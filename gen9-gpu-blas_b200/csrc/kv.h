@@ -58,11 +58,7 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
 constexpr long long kKvMost = 1LL << 46;
 int kv_too_large(const char *who);
 // Ends a call: waits if sync, else records what was written for the no-wait ledger.
-struct KvWrite {
-    const void *p;
-    size_t bytes;
-};
-int kv_finish(const KvCall &call, int sync, const KvWrite *w, int n);
+int kv_finish(const KvCall &call, int sync, const QueuedWrite *w, int n);
 
 }  // namespace g9
 #pragma GCC visibility pop

@@ -815,7 +815,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     }
     const size_t marks = ((size_t)(c->ns - 1) * (size_t)std::max<int64_t>(ms, 0) +
                           (size_t)(c->HKV - 1) * (size_t)std::max<int64_t>(mh, 0) + (size_t)a.c.cap) * 4;
-    const KvWrite w[3] = {{O, (size_t)heads * c->D * 4}, {lse, (size_t)heads * 4}, {acc, marks}};
+    const QueuedWrite w[3] = {{O, (size_t)heads * c->D * 4}, {lse, (size_t)heads * 4}, {acc, marks}};
     return kv_finish(call, sync, w, 3);
 }
 

@@ -320,65 +320,76 @@ int check_dev_err(DevState *d) {
 // Drops entry i (its write has completed), keeping the others' order irrelevant: the last entry takes its place.
 static void queued_drop(DevState *d, int i) {
     const int last = d->queued_n - 1;
+    d->queued_ev_used[d->queued_ev[i]]--;
     if (i != last) {
         d->queued_lo[i] = d->queued_lo[last];
         d->queued_hi[i] = d->queued_hi[last];
-        cudaEvent_t e = d->queued_ev[i];
         d->queued_ev[i] = d->queued_ev[last];
-        d->queued_ev[last] = e;
         d->queued_st[i] = d->queued_st[last];
     }
     d->queued_n = last;
 }
 
 static bool queued_done(DevState *d, int i) {
-    const cudaError_t e = cudaEventQuery(d->queued_ev[i]);
+    const cudaError_t e = cudaEventQuery(d->queued_evs[d->queued_ev[i]]);
     if (e == cudaErrorNotReady) return false;
     cudaGetLastError();
     return e == cudaSuccess;
 }
 
-void queued_writes_add(DevState *d, const void *p, size_t bytes, cudaStream_t st) {
-    if (!bytes) return;
-    const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
-    int slot = -1;
-    for (int i = 0; i < d->queued_n && slot < 0; i++)   // a range that overlaps or touches an entry of its stream widens it
-        if (lo <= d->queued_hi[i] && d->queued_lo[i] <= hi && d->queued_st[i] == st) slot = i;
-    if (slot < 0 && d->queued_n == DevState::kQueuedRanges)
+// The entry that takes a range of stream st: one that it overlaps or touches, a free one, or, where all are taken, that
+// of the stream which grows least. -1: all belong to other streams.
+static int queued_slot(DevState *d, uintptr_t lo, uintptr_t hi, cudaStream_t st) {
+    for (int i = 0; i < d->queued_n; i++)
+        if (lo <= d->queued_hi[i] && d->queued_lo[i] <= hi && d->queued_st[i] == st) return i;
+    if (d->queued_n == DevState::kQueuedRanges)
         for (int i = d->queued_n - 1; i >= 0; i--)       // full: forget the writes that have completed
             if (queued_done(d, i)) queued_drop(d, i);
-    if (slot < 0 && d->queued_n == DevState::kQueuedRanges) {   // still full: the entry of the stream that grows least takes it in
-        size_t least = SIZE_MAX;
-        for (int i = 0; i < d->queued_n; i++) {
-            if (d->queued_st[i] != st) continue;
-            const size_t grown = lo < d->queued_lo[i] ? d->queued_lo[i] - lo : hi > d->queued_hi[i] ? hi - d->queued_hi[i] : 0;
-            if (grown < least) {
-                least = grown;
-                slot = i;
+    if (d->queued_n < DevState::kQueuedRanges) return d->queued_n;
+    int slot = -1;
+    size_t least = SIZE_MAX;
+    for (int i = 0; i < d->queued_n; i++) {
+        if (d->queued_st[i] != st) continue;
+        const size_t grown = lo < d->queued_lo[i] ? d->queued_lo[i] - lo : hi > d->queued_hi[i] ? hi - d->queued_hi[i] : 0;
+        if (grown < least) {
+            least = grown;
+            slot = i;
+        }
+    }
+    return slot;
+}
+
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st) {
+    int ev = -1;   // recorded behind the call for the first of its ranges
+    for (int k = 0; k < n; k++) {
+        if (!w[k].p || !w[k].bytes) continue;
+        if (ev < 0) {
+            for (ev = 0; d->queued_ev_used[ev]; ev++) {}   // one event more than there are entries
+            if ((!d->queued_evs[ev] && cudaEventCreateWithFlags(&d->queued_evs[ev], cudaEventDisableTiming) != cudaSuccess) ||
+                cudaEventRecord(d->queued_evs[ev], st) != cudaSuccess) {
+                cudaGetLastError();
+                queued_writes_lost(d, st);   // cannot tell when it completes: stay conservative
+                return;
             }
         }
-    }
-    if (slot < 0) {
-        if (d->queued_n == DevState::kQueuedRanges) {    // none of its stream: every later check answers "maybe written"
-            queued_writes_lost(d, st);
+        const uintptr_t lo = (uintptr_t)w[k].p, hi = lo + w[k].bytes;
+        const int i = queued_slot(d, lo, hi, st);
+        if (i < 0) {
+            queued_writes_lost(d, st);       // every later check answers "maybe written"
             return;
         }
-        slot = d->queued_n++;
-        d->queued_lo[slot] = lo;
-        d->queued_hi[slot] = hi;
-        d->queued_st[slot] = st;
-    } else {
-        if (lo < d->queued_lo[slot]) d->queued_lo[slot] = lo;
-        if (hi > d->queued_hi[slot]) d->queued_hi[slot] = hi;
-    }
-    if (!d->queued_ev[slot] && cudaEventCreateWithFlags(&d->queued_ev[slot], cudaEventDisableTiming) != cudaSuccess) {
-        cudaGetLastError();
-        queued_writes_lost(d, st);   // cannot tell when it completes: stay conservative
-        return;
-    }
-    if (cudaEventRecord(d->queued_ev[slot], st) != cudaSuccess) {
-        cudaGetLastError();
-        queued_writes_lost(d, st);
+        if (i == d->queued_n) {
+            d->queued_n++;
+            d->queued_lo[i] = lo;
+            d->queued_hi[i] = hi;
+            d->queued_st[i] = st;
+        } else {
+            d->queued_ev_used[d->queued_ev[i]]--;
+            if (lo < d->queued_lo[i]) d->queued_lo[i] = lo;
+            if (hi > d->queued_hi[i]) d->queued_hi[i] = hi;
+        }
+        d->queued_ev[i] = ev;
+        d->queued_ev_used[ev]++;
     }
 }
 
@@ -420,7 +431,10 @@ int finish_op(Operand *ops, int n) {
     for (int i = 0; i < n; i++) all_zc = all_zc && ops[i].zc;
     if (G.nowait && all_zc) {
         for (int i = 0; i < n; i++)
-            if (ops[i].written) queued_writes_add(d, ops[i].dptr, ops[i].bytes, st);
+            if (ops[i].written) {
+                const QueuedWrite w = {ops[i].dptr, ops[i].bytes};
+                queued_writes_add(d, &w, 1, st);
+            }
         return 0;
     }
     for (int i = 0; i < n; i++) {
