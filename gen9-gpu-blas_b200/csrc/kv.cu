@@ -1644,13 +1644,21 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     a.flag = (int *)((char *)buf + 2 * list);
     a.todo = (int *)((char *)buf + 2 * list + pages);
     a.used = (int *)((char *)buf + 2 * list + 2 * pages);
-    // clusters that hold a row's slots in registers, and larger ones while the GPU has SMs to spare for rows of 1024 slots a CTA
+    // Clusters that hold a row's slots in registers, and larger ones while the GPU has SMs to spare for rows of 1024 slots a CTA;
+    // rows of up to 8192 slots still go to one CTA of 1024 threads (256 rows of 8000: 71 µs against 89 with two of 512), as
+    // do stretches beyond what eight CTAs of 512 hold (8 rows of 60000: 65 µs against 104).
     int size = 1;
-    while (size < 8 && (a.c.cap > 512 * 12 * size || (rows * size * 2 <= call.d->sm_count && a.c.cap > 2048 * size))) size *= 2;
+    auto more = [&]() {
+        if (rows * size * 2 <= call.d->sm_count && a.c.cap > 2048 * size) return true;
+        return a.c.cap > 512 * 12 * size && (size > 1 || a.c.cap > 1024 * 8);
+    };
+    while (size < 8 && more()) size *= 2;
     if (rows * size > INT_MAX) size = 1;
-    if (size == 1 && a.c.cap <= 256 * 4) G9_TRY((rank_launch<256, 4>(a, call, rows, 1)));
-    else if (size == 1 && a.c.cap <= 256 * 12) G9_TRY((rank_launch<256, 12>(a, call, rows, 1)));
-    else G9_TRY((rank_launch<512, 12>(a, call, rows, size)));
+    const int per = (a.c.cap + size - 1) / size;
+    if (size == 1 && per <= 256 * 4) G9_TRY((rank_launch<256, 4>(a, call, rows, 1)));
+    else if (per <= 512 * 6) G9_TRY((rank_launch<512, 6>(a, call, rows, size)));
+    else if (per <= 512 * 12) G9_TRY((rank_launch<512, 12>(a, call, rows, size)));
+    else G9_TRY((rank_launch<1024, 8>(a, call, rows, size)));
     const int team = c->page > 32 ? MT / 32 : 1, teams = MT / 32 / team;
     // a page per team, as many as can change (each mover changes one, and the last may lose slots), up to four waves of CTAs
     const long long most = std::min<long long>(a.pages, (long long)a.c.cap - a.keep + 1);
