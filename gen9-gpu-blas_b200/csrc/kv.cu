@@ -1657,6 +1657,7 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     const int per = (a.c.cap + size - 1) / size;
     if (size == 1 && per <= 256 * 4) G9_TRY((rank_launch<256, 4>(a, call, rows, 1)));
     else if (per <= 512 * 6) G9_TRY((rank_launch<512, 6>(a, call, rows, size)));
+    else if (per <= 512 * 9) G9_TRY((rank_launch<512, 9>(a, call, rows, size)));
     else if (per <= 512 * 12) G9_TRY((rank_launch<512, 12>(a, call, rows, size)));
     else G9_TRY((rank_launch<1024, 8>(a, call, rows, size)));
     const int team = c->page > 32 ? MT / 32 : 1, teams = MT / 32 / team;
