@@ -60,12 +60,12 @@ struct PagedCfg {
     static constexpr int ROWS = 8 * NT;                         // query rows of a unit
     static constexpr int STAGE = AKEYS * DP * 2 * 2;            // bytes of a warp's stage: K rows, V rows
     // resident CTAs of an SM, held to by registers and shared memory: as many warps as fit serve the latencies of a step better
-    // than deeper rings of fewer (one row tile, D 128: three CTAs of two stages against two of three 24.9 and 26.2 µs at 8
-    // streams of 4096 keys, 31.5 and 35.5 at 64 chosen pages of 16; D 64: four of three against two of six 79 and 107 µs at
-    // 2 streams of 131071 keys)
+    // than deeper rings of fewer (D 128: three CTAs of two stages against two of three 24.9 and 26.2 µs at 8 streams of 4096
+    // keys, 31.5 and 35.5 at 64 chosen pages of 16, two row tiles 185 and 201 at 64 streams of 4096; D 64: four of three against
+    // two of six 79 and 107 µs at 2 streams of 131071 keys, two row tiles 106 and 140 at 64 streams of 8192)
     // W, with weights: the addresses of the scores take the registers of a third CTA (65 against 52 µs at 8 streams of 8192 keys).
-    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? (NT == 1 && !W ? 3 : 2) : NT == 1 ? 4 : NT == 2 ? 3 : 2;
-    static constexpr int NST = DP == 64 ? (NT == 1 ? 3 : NT == 2 ? 4 : 6) : CTAS == 3 ? 2 : 3;
+    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? (W ? 2 : 3) : 4;
+    static constexpr int NST = CTAS == 3 ? 2 : 3;
     static constexpr int RING = AW * NST * STAGE;
     static constexpr int QF = NT == 1 ? 0 : DP / 16 * NT * 32 * 16;   // query fragments, hi and lo (NT = 1: registers)
     static constexpr int KIDX = AW * NST * AKEYS * 4;
@@ -709,18 +709,11 @@ int paged_either(const PagedArgs &a, const KvCall &call, bool weights, bool plan
 
 // The kernel of a padded head size and a number of 8-row tiles; plan: only its resident CTAs.
 int paged(int dp, int nt, const PagedArgs &a, const KvCall &call, bool weights, bool plan, int *ctas) {
-    if (dp == 64) {
-        if (nt == 1) return paged_either<64, 1>(a, call, weights, plan, ctas);
-        if (nt == 2) return paged_either<64, 2>(a, call, weights, plan, ctas);
-        return paged_either<64, 4>(a, call, weights, plan, ctas);
-    }
-    if (dp == 128) {
-        if (nt == 1) return paged_either<128, 1>(a, call, weights, plan, ctas);
-        if (nt == 2) return paged_either<128, 2>(a, call, weights, plan, ctas);
-        return paged_either<128, 4>(a, call, weights, plan, ctas);
-    }
-    if (nt == 1) return paged_either<256, 1>(a, call, weights, plan, ctas);
-    return paged_either<256, 2>(a, call, weights, plan, ctas);
+    if (dp == 64)
+        return nt == 1 ? paged_either<64, 1>(a, call, weights, plan, ctas) : paged_either<64, 2>(a, call, weights, plan, ctas);
+    if (dp == 128)
+        return nt == 1 ? paged_either<128, 1>(a, call, weights, plan, ctas) : paged_either<128, 2>(a, call, weights, plan, ctas);
+    return nt == 1 ? paged_either<256, 1>(a, call, weights, plan, ctas) : paged_either<256, 2>(a, call, weights, plan, ctas);
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -769,7 +762,14 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     a.qn = sel ? 1 : nq;
     const long long rows = (long long)a.qn * a.G;
     const int dp = c->D <= 64 ? 64 : c->D <= 128 ? 128 : 256;
-    const int nt = rows <= 8 ? 1 : rows <= 16 || dp == 256 ? 2 : 4;
+    // Sixteen rows a unit, or eight with the keys read once for each eight, while that is little to read (one stream of 4096
+    // keys, 16 rows, D 128: 16.1 µs against 20.3; 16 streams of 1000 keys 27.2 against 24.7; two and four tokens of 8 heads
+    // in 16 windows of 2048 keys, D 64: 12.6 and 17.2 against 13.9 and 16.7). Units of 32 rows were slower at every shape
+    // (32 heads, 8 streams of 8192 keys 35 µs against 27; 4 tokens in the windows 20.6) but long ones of D 64 (64 streams of
+    // 8192 keys, 32 rows: 105 against 115).
+    const long long slots = sel ? (long long)nsel * c->page : std::min<long long>(a.c.cap, window > 0 ? (long long)window + (long long)dvis * nq : a.c.cap);
+    const bool little = (__int128)c->ns * c->HKV * ((rows + 7) / 8) * slots * c->D * 4 <= 48 << 20;
+    const int nt = rows <= 8 || little ? 1 : 2;
     const long long tiles = (rows + 8 * nt - 1) / (8 * nt), outer = (long long)c->ns * (sel ? nq : 1);
     // never more steps than this; they and the (s, t, h) rows are counted in 32 bits
     const long long per = (sel ? a.sel_steps : (a.c.cap + AKEYS - 1) / AKEYS + 1) + PagedCfg<64, 1, false>::COST;
