@@ -63,8 +63,7 @@ struct PagedCfg {
     // than deeper rings of fewer (D 128: three CTAs of two stages against two of three 24.9 and 26.2 µs at 8 streams of 4096
     // keys, 31.5 and 35.5 at 64 chosen pages of 16, two row tiles 185 and 201 at 64 streams of 4096; D 64: four of three against
     // two of six 79 and 107 µs at 2 streams of 131071 keys, two row tiles 106 and 140 at 64 streams of 8192)
-    // W, with weights: the addresses of the scores take the registers of a third CTA (65 against 52 µs at 8 streams of 8192 keys).
-    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? (W ? 2 : 3) : 4;
+    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? 3 : 4;
     static constexpr int NST = CTAS == 3 ? 2 : 3;
     static constexpr int RING = AW * NST * STAGE;
     static constexpr int QF = NT == 1 ? 0 : DP / 16 * NT * 32 * 16;   // query fragments, hi and lo (NT = 1: registers)
@@ -124,7 +123,6 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
     const KvDev &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, tq = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // ---- this CTA's run of steps. Counting a segment's latencies in (about 6 µs, COST steps; see kv_plan.cuh) took 8 streams of
     // 4096 keys from 32.4 to 26.3 µs and one stream of 1000 keys from 14.1 to 9.6.
@@ -698,7 +696,10 @@ int paged_one(const PagedArgs &a, const KvCall &call, bool plan, int *ctas) {
         *ctas = std::max(occ[call.d->dev], 1) * call.d->sm_count;
         return 0;
     }
-    G9_CU(launch_pdl(attn_paged_k<DP, NT, W>, dim3((unsigned)*ctas), dim3(AW * 32), C::SMEM, call.st, a));
+    // Not launched early: the CTAs fill an SM's registers, and one that finds a CTA of the kernel before among them leaves a hole
+    // too small for the last one, which then waits for a whole run (8 streams of 4193 to 8193 keys behind an append 53 µs
+    // against 42, the same with weights 62 against 48). Without a wave to fill, starting early saves 0.5 µs.
+    attn_paged_k<DP, NT, W><<<(unsigned)*ctas, AW * 32, C::SMEM, call.st>>>(a);
     return launched("attn_paged");
 }
 
