@@ -369,7 +369,7 @@ __device__ __forceinline__ void bulk_row(void *dst, const void *src, unsigned by
 constexpr uint64_t SWAIT_NS = 2000000000ull;   // a row that has not landed after 2 s is an error
 constexpr int SCOST = 8;   // steps that a CTA reads in the time of a segment's latencies
 constexpr int SW = 4, SPAGES = 16, SNST = 2;   // warps of a CTA, pages of a step, stages of a warp's ring: two, so that an SM
-// holds 12 warps (D = 128), because a step computes about as long as its copy takes (46.7 µs with three stages, 41.2 with two)
+// holds 12 warps (D = 128), because a step computes about as long as its copy takes (three stages took 5.5 µs longer at 101 MB)
 template <int DP>
 struct ScoreCfg {
     static constexpr int PITCH = DP * 2 * 2 + 16;                   // a page's lower and upper row; 16 bytes more spread the banks
@@ -1311,14 +1311,20 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
 }
 
 // The moves: the CTAs of a row (`ctas` of them) take its changed pages in turn, a page to `team` warps (1 or all four), which
-// take its rows 32 at a time; lpr lanes carry a row, 16 bytes each. The bounds of a page are taken over the rows it now holds, the
-// movers' from their sources. Every source lies at or above keep and every target below, so that the order of the moves does
-// not matter. Bound by memory, rows in and out: many warps with a row each in flight -- 12 CTAs per SM took 63 µs for 8 × 8
-// heads, 16384 -> 8192 slots in pages of 32 (335 MB), 6 CTAs with four rows a lane 79 µs, all warps on one page 82 µs. Pages
-// of more than 32 slots take the whole CTA, or 64 rows come one after the other.
-constexpr int MT = 128, MCTAS = 12;
+// take its rows 4·32 / lpr at a time; lpr lanes carry a row, 16 bytes each, by asynchronous copies into a place of the lane's
+// own in shared memory and out from there. The bounds of a page are taken over the rows it now holds, the movers' from their
+// sources. Every source lies at or above keep and every target below, so that the order of the moves does not matter. Bound by
+// memory, rows in and out: ranking and moves of 8 × 8 heads, 16384 -> 8192 slots in pages of 32 (335 MB) take 88.9 µs with four
+// rows of a lane in flight and nine CTAs per SM, 87.1 with ten -- but 22.1 against 21.0 µs where a few of 2064 slots go, their
+// registers spill -- and 95.6 with a row at a time through registers and twelve CTAs. Pages of more than 32 slots take the whole
+// CTA, or 64 rows come one after the other (142 µs against 104 at pages of 64).
+constexpr int MT = 128, MCTAS = 9, MR = 4;   // threads of a CTA, CTAs of an SM, rows of a lane at once
+__device__ __forceinline__ void async16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_all;\n" ::: "memory"); }
 __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ EvictArgs a, int ctas, int lpr, int team) {
-    __shared__ uint4 red[MT / 32][2][32];   // [warp][least, largest][lane]
+    __shared__ uint4 buf[MT / 32][MR][2][32];   // [warp][row of the lane][K, V][lane]; then [warp][0][least, largest][lane]
     pdl_next();
     pdl_wait();
     const KvDev &c = a.c;
@@ -1329,6 +1335,7 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
     const int todo = a.used[2 * row + 1], teams = MT / 32 / team, mate = warp % team;
     const int rpw = 32 / lpr, sub = lane / lpr, ch = lane - sub * lpr;   // rows of a warp at once, this lane's row, its 16 bytes
     const bool live = ch * 8 < c.D, bounds = c.bounds != nullptr;
+    const int step = MR * rpw;   // rows of a warp at once
     for (int w = part * teams + warp / team; w < todo; w += ctas * teams) {
         const int place = a.todo[(long long)row * a.pages + w];
         const int k0 = place * c.page, rows = min(c.page, keep - k0);
@@ -1345,26 +1352,36 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
         if (id < 0) continue;
         uint4 mn = make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);   // +inf, -inf
         uint4 mx = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-        for (int r0 = mate * 32; r0 < rows; r0 += team * 32) {
+        for (int r0 = mate * step; r0 < rows; r0 += team * step) {
             // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
             long long ko = 0, vo = -1;
-            if (r0 + lane < rows) {
+            if (lane < step && r0 + lane < rows) {
                 const int k = __ldg(src + r0 + lane), pl = page_quot(c.div, max(k, 0));
                 const int from = k >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
                 ko = from >= 0 ? row_at(from, k - pl * c.page, g, c.kp, c.kk, c.kh) : row_at(id, r0 + lane, g, c.kp, c.kk, c.kh);
                 if (from >= 0) vo = row_at(from, k - pl * c.page, g, c.vp, c.vk, c.vh);
             }
             __half *kd = c.K + row_at(id, r0, g, c.kp, c.kk, c.kh) + ch * 8, *vd = c.V + row_at(id, r0, g, c.vp, c.vk, c.vh) + ch * 8;
-            const int here = min(32, rows - r0);
-            for (int i0 = 0; i0 < here; i0 += rpw) {
-                const int i = i0 + sub;
-                const long long kr = __shfl_sync(kAll, ko, i & 31), vr = __shfl_sync(kAll, vo, i & 31);
-                if (i >= here || !live || (!bounds && vr < 0)) continue;
-                const uint4 kv = __ldcg(reinterpret_cast<const uint4 *>(c.K + kr + ch * 8));
-                if (vr >= 0) {
-                    const uint4 vv = __ldcg(reinterpret_cast<const uint4 *>(c.V + vr + ch * 8));
+            const int here = min(step, rows - r0);
+            // all rows at once into this warp's shared memory, each lane its own 16 bytes of them, then out from there
+#pragma unroll
+            for (int j = 0; j < MR; j++) {
+                const int i = j * rpw + sub;
+                const long long kr = __shfl_sync(kAll, ko, i), vr = __shfl_sync(kAll, vo, i);
+                if (i >= here || !live) continue;
+                if (bounds || vr >= 0) async16(&buf[warp][j][0][lane], c.K + kr + ch * 8);
+                if (vr >= 0) async16(&buf[warp][j][1][lane], c.V + vr + ch * 8);
+            }
+            async_wait();
+#pragma unroll
+            for (int j = 0; j < MR; j++) {
+                const int i = j * rpw + sub;
+                const bool moves = __shfl_sync(kAll, vo, i) >= 0;
+                if (i >= here || !live || (!bounds && !moves)) continue;
+                const uint4 kv = buf[warp][j][0][lane];
+                if (moves) {
                     *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
-                    *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = vv;
+                    *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = buf[warp][j][1][lane];
                 }
                 if (!bounds) continue;
                 mn = least8(mn, kv);
@@ -1377,13 +1394,13 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
             mx = largest8(mx, shfl8(mx, o));
         }
         if (team > 1) {   // the whole CTA: every warp is here
-            red[warp][0][lane] = mn;
-            red[warp][1][lane] = mx;
+            buf[warp][0][0][lane] = mn;
+            buf[warp][0][1][lane] = mx;
             __syncthreads();
             if (warp == 0)
                 for (int i = 1; i < team; i++) {
-                    mn = least8(mn, red[i][0][lane]);
-                    mx = largest8(mx, red[i][1][lane]);
+                    mn = least8(mn, buf[i][0][0][lane]);
+                    mx = largest8(mx, buf[i][0][1][lane]);
                 }
             __syncthreads();   // the partial bounds are read before the next page's land on them
         }
