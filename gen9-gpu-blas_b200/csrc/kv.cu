@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
                 __half2 pk0 = __half2half2(__ushort_as_half(0)), pk1 = pk0;
                 bool wild = false;
                 for (int tile = 0; tile < ntile; tile++) {
-                    float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                    float sc[4][4] = {};   // lower and upper bounds, by the queries' first and second parts: four chains, not one
                     const uint4 *q0 = qf + tile * 2 * KT * 32 + lane, *q1 = q0 + KT * 32;
 #pragma unroll
                     for (int kt = 0; kt < KT; kt++) {
@@ -533,18 +533,19 @@ __global__ void __launch_bounds__(SW * 32) kv_score_k(const __grid_constant__ Se
                             pk1 = __hmax2(__hmax2(pk1, __hmax2(__habs2(as_h2(l4[1])), __habs2(as_h2(l4[3])))),
                                           __hmax2(__habs2(as_h2(u4[1])), __habs2(as_h2(u4[3]))));
                         }
-                    const uint4 f = q0[kt * 32], h = q1[kt * 32];
+                        const uint4 f = q0[kt * 32], h = q1[kt * 32];
                         at_mma(sc[0], l4, f.x, f.y);
                         at_mma(sc[1], u4, h.x, h.y);
-                        at_mma(sc[0], l4, f.z, f.w);
-                        at_mma(sc[1], u4, h.z, h.w);
+                        at_mma(sc[2], l4, f.z, f.w);
+                        at_mma(sc[3], u4, h.z, h.w);
                     }
                     const int t = (tile0 + tile) / a.hg, hb = (tile0 + tile - t * a.hg) * 8;
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         if (hb + 2 * tq + j >= a.G) continue;
                         const float inv = qinv[tile * 8 + 2 * tq + j];
-                        const float x0 = (sc[0][j] + sc[1][j]) * inv, x1 = (sc[0][2 + j] + sc[1][2 + j]) * inv;
+                        const float x0 = ((sc[0][j] + sc[1][j]) + (sc[2][j] + sc[3][j])) * inv;
+                        const float x1 = ((sc[0][2 + j] + sc[1][2 + j]) + (sc[2][2 + j] + sc[3][2 + j])) * inv;
                         wild = wild || (in0 && !(fabsf(x0) < INFINITY)) || (in1 && !(fabsf(x1) < INFINITY));
                         top[0] = fmaxf(top[0], x0);
                         top[1] = fmaxf(top[1], x1);
@@ -909,10 +910,11 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     float x[CR];
 #pragma unroll
     for (int i = 0; i < CR; i++) x[i] = tid + i * CT < have ? __ldcg(score + tid + i * CT) : 0.0f;
-    // ---- E = 2^-14 · max |q|_1 · max |bound| (2^-13 for D > 128): each of the 4·D/16 tensor-core steps adds 17 numbers, each cut
-    // off at worst 2^-23 below the largest, which is at most |q|_1·|bound|, 2^-18.9 in all; 32 steps at D = 128 make 2^-13.9
-    // of twice the mean running sum; the two FP16 parts of the query lose another 2^-21. 2^-126 more covers what scores and E
-    // itself lose where they fall below FP32's normal numbers
+    // ---- E = 2^-15 · max |q|_1 · max |bound| (2^-14 for D > 128): each of a chain's D/16 tensor-core steps adds 17 numbers, each
+    // cut off at worst 2^-23 below the largest, 2^-18.9 of what bounds the chain's sums; those bounds of the two chains of the
+    // queries' first parts add up to |q|_1·|bound|, so that 8 steps at D = 128 make 2^-15.9. The second parts' chains are 2^-11 of
+    // that, what those parts leave out 2^-21, the sums and the scale in FP32 2^-22. 2^-126 more covers what scores and E itself lose
+    // where they fall below FP32's normal numbers.
     float big = 0.0f, l1 = 0.0f;
     {
         const float *peak = a.peak + (((long long)s * c.HKV + g) * a.zs + t * a.hg / a.zt) * a.unit_steps;
@@ -940,7 +942,7 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
         big = fmaxf(big, red[0][w]);
         l1 = fmaxf(l1, red[1][w]);
     }
-    const float E = (c.D > 128 ? 0x1p-13f : 0x1p-14f) * l1 * big + 0x1p-126f;
+    const float E = (c.D > 128 ? 0x1p-14f : 0x1p-15f) * l1 * big + 0x1p-126f;
     const bool full = at == kAll;   // enough pages that are always taken: the lowest of them
     const float tau = __uint_as_float(at & 0x80000000u ? at & 0x7fffffffu : ~at);
     const bool know = E < INFINITY && at != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
@@ -1317,7 +1319,7 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
 // memory, rows in and out: ranking and moves of 8 × 8 heads, 16384 -> 8192 slots in pages of 32 (335 MB) take 88.9 µs with four
 // rows of a lane in flight and nine CTAs per SM, 87.1 with ten -- but 22.1 against 21.0 µs where a few of 2064 slots go, their
 // registers spill -- and 95.6 with a row at a time through registers and twelve CTAs. Pages of more than 32 slots take the whole
-// CTA, or 64 rows come one after the other (142 µs against 104 at pages of 64).
+// CTA, or 64 rows come one after the other.
 constexpr int MT = 128, MCTAS = 9, MR = 4;   // threads of a CTA, CTAs of an SM, rows of a lane at once
 __device__ __forceinline__ void async16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
