@@ -59,11 +59,12 @@ template <int DP, int NT, bool W>
 struct PagedCfg {
     static constexpr int ROWS = 8 * NT;                         // query rows of a unit
     static constexpr int STAGE = AKEYS * DP * 2 * 2;            // bytes of a warp's stage: K rows, V rows
-    // resident CTAs of an SM, held to by registers and shared memory: as many warps as fit serve the latencies of a step better
+    // Resident CTAs of an SM, held to by registers and shared memory: as many warps as fit serve the latencies of a step better
     // than deeper rings of fewer (D 128: three CTAs of two stages against two of three 24.9 and 26.2 µs at 8 streams of 4096
     // keys, 31.5 and 35.5 at 64 chosen pages of 16, two row tiles 185 and 201 at 64 streams of 4096; D 64: four of three against
-    // two of six 79 and 107 µs at 2 streams of 131071 keys, two row tiles 106 and 140 at 64 streams of 8192)
-    static constexpr int CTAS = DP == 256 ? 1 : DP == 128 ? 3 : 4;
+    // two of six 79 and 107 µs at 2 streams of 131071 keys). Two row tiles of D 64: three of two 15.9 µs at 16 windows of 2048
+    // keys and 114 at 64 streams of 8192, three of four 16.6 and 115, four of three 17.7 and 111, two of six 17.9 and 140.
+    static constexpr int CTAS = DP == 256 ? 1 : DP == 64 && NT == 1 ? 4 : 3;
     static constexpr int NST = CTAS == 3 ? 2 : 3;
     static constexpr int RING = AW * NST * STAGE;
     static constexpr int QF = NT == 1 ? 0 : DP / 16 * NT * 32 * 16;   // query fragments, hi and lo (NT = 1: registers)
@@ -772,7 +773,7 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     const int dp = c->D <= 64 ? 64 : c->D <= 128 ? 128 : 256;
     // Sixteen rows a unit, or eight with the keys read once for each eight, while that is little to read (one stream of 4096
     // keys, 16 rows, D 128: 16.1 µs against 20.3; 16 streams of 1000 keys 27.2 against 24.7; two and four tokens of 8 heads
-    // in 16 windows of 2048 keys, D 64: 12.6 and 17.2 against 13.9 and 16.7). Units of 32 rows were slower at every shape
+    // in 16 windows of 2048 keys, D 64: 12.6 and 17.2 against 13.9 and 15.9). Units of 32 rows were slower at every shape
     // (32 heads, 8 streams of 8192 keys 35 µs against 27; 4 tokens in the windows 20.6) but long ones of D 64 (64 streams of
     // 8192 keys, 32 rows: 105 against 115).
     const long long slots = sel ? (long long)nsel * c->page : std::min<long long>(a.c.cap, window > 0 ? (long long)window + (long long)dvis * nq : a.c.cap);
