@@ -1316,11 +1316,11 @@ __global__ void __launch_bounds__(ET) kv_rank_k(const __grid_constant__ EvictArg
 // take its rows 4·32 / lpr at a time; lpr lanes carry a row, 16 bytes each, by asynchronous copies into a place of the lane's
 // own in shared memory and out from there. The bounds of a page are taken over the rows it now holds, the movers' from their
 // sources. Every source lies at or above keep and every target below, so that the order of the moves does not matter. Bound by
-// memory, rows in and out: ranking and moves of 8 × 8 heads, 16384 -> 8192 slots in pages of 32 (335 MB) take 88.9 µs with four
-// rows of a lane in flight and nine CTAs per SM, 87.1 with ten -- but 22.1 against 21.0 µs where a few of 2064 slots go, their
-// registers spill -- and 95.6 with a row at a time through registers and twelve CTAs. Pages of more than 32 slots take the whole
-// CTA, or 64 rows come one after the other.
-constexpr int MT = 128, MCTAS = 9, MR = 4;   // threads of a CTA, CTAs of an SM, rows of a lane at once
+// memory, rows in and out, and by issuing: ranking and moves of 8 × 8 heads, 16384 -> 8192 slots in pages of 32 (335 MB) take 83.5 µs
+// with four rows of a lane in flight and ten CTAs per SM (nine 86.4, but 20.9 against 21.4 µs where a few of 2064 slots go; places
+// worked out for those four rows at a time 87.1; a row at a time through registers, twelve CTAs, 95.6). Pages of more than 32
+// slots take the whole CTA, or 64 rows come one after the other.
+constexpr int MT = 128, MCTAS = 10, MR = 4;   // threads of a CTA, CTAs of an SM, rows of a lane at once
 __device__ __forceinline__ void async16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
 }
@@ -1337,7 +1337,7 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
     const int todo = a.used[2 * row + 1], teams = MT / 32 / team, mate = warp % team;
     const int rpw = 32 / lpr, sub = lane / lpr, ch = lane - sub * lpr;   // rows of a warp at once, this lane's row, its 16 bytes
     const bool live = ch * 8 < c.D, bounds = c.bounds != nullptr;
-    const int step = MR * rpw;   // rows of a warp at once
+    const int step = MR * rpw, span = team > 1 ? step : 32;   // rows of a warp at once; rows whose places are worked out at once
     for (int w = part * teams + warp / team; w < todo; w += ctas * teams) {
         const int place = a.todo[(long long)row * a.pages + w];
         const int k0 = place * c.page, rows = min(c.page, keep - k0);
@@ -1354,40 +1354,42 @@ __global__ void __launch_bounds__(MT, MCTAS) kv_move_k(const __grid_constant__ E
         if (id < 0) continue;
         uint4 mn = make_uint4(0x7c007c00u, 0x7c007c00u, 0x7c007c00u, 0x7c007c00u);   // +inf, -inf
         uint4 mx = make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-        for (int r0 = mate * step; r0 < rows; r0 += team * step) {
+        for (int r0 = mate * span; r0 < rows; r0 += team * span) {
             // lane: the source of row r0 + lane, offsets in the pools (V: -1 where the row stays)
             long long ko = 0, vo = -1;
-            if (lane < step && r0 + lane < rows) {
+            if (lane < span && r0 + lane < rows) {
                 const int k = __ldg(src + r0 + lane), pl = page_quot(c.div, max(k, 0));
                 const int from = k >= 0 ? page_id(c.table, c.ts, s, pl, c.mp, c.n_pages) : -1;
                 ko = from >= 0 ? row_at(from, k - pl * c.page, g, c.kp, c.kk, c.kh) : row_at(id, r0 + lane, g, c.kp, c.kk, c.kh);
                 if (from >= 0) vo = row_at(from, k - pl * c.page, g, c.vp, c.vk, c.vh);
             }
             __half *kd = c.K + row_at(id, r0, g, c.kp, c.kk, c.kh) + ch * 8, *vd = c.V + row_at(id, r0, g, c.vp, c.vk, c.vh) + ch * 8;
-            const int here = min(step, rows - r0);
-            // all rows at once into this warp's shared memory, each lane its own 16 bytes of them, then out from there
+            const int here = min(span, rows - r0);
+            const unsigned moves = __ballot_sync(kAll, vo >= 0);   // by row
+            // MR rows of each lane at once into this warp's shared memory, each lane its own 16 bytes of them, then out from there
+            for (int i0 = 0; i0 < here; i0 += step) {
 #pragma unroll
-            for (int j = 0; j < MR; j++) {
-                const int i = j * rpw + sub;
-                const long long kr = __shfl_sync(kAll, ko, i), vr = __shfl_sync(kAll, vo, i);
-                if (i >= here || !live) continue;
-                if (bounds || vr >= 0) async16(&buf[warp][j][0][lane], c.K + kr + ch * 8);
-                if (vr >= 0) async16(&buf[warp][j][1][lane], c.V + vr + ch * 8);
-            }
-            async_wait();
-#pragma unroll
-            for (int j = 0; j < MR; j++) {
-                const int i = j * rpw + sub;
-                const bool moves = __shfl_sync(kAll, vo, i) >= 0;
-                if (i >= here || !live || (!bounds && !moves)) continue;
-                const uint4 kv = buf[warp][j][0][lane];
-                if (moves) {
-                    *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
-                    *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = buf[warp][j][1][lane];
+                for (int j = 0; j < MR; j++) {
+                    const int i = i0 + j * rpw + sub;
+                    const long long kr = __shfl_sync(kAll, ko, i), vr = __shfl_sync(kAll, vo, i);
+                    if (i >= here || !live) continue;
+                    if (bounds || vr >= 0) async16(&buf[warp][j][0][lane], c.K + kr + ch * 8);
+                    if (vr >= 0) async16(&buf[warp][j][1][lane], c.V + vr + ch * 8);
                 }
-                if (!bounds) continue;
-                mn = least8(mn, kv);
-                mx = largest8(mx, kv);
+                async_wait();
+#pragma unroll
+                for (int j = 0; j < MR; j++) {
+                    const int i = i0 + j * rpw + sub;
+                    if (i >= here || !live || (!bounds && !(moves >> i & 1u))) continue;
+                    const uint4 kv = buf[warp][j][0][lane];
+                    if (moves >> i & 1u) {
+                        *reinterpret_cast<uint4 *>(kd + (long long)i * c.kk) = kv;
+                        *reinterpret_cast<uint4 *>(vd + (long long)i * c.vk) = buf[warp][j][1][lane];
+                    }
+                    if (!bounds) continue;
+                    mn = least8(mn, kv);
+                    mx = largest8(mx, kv);
+                }
             }
         }
         if (!bounds) continue;
