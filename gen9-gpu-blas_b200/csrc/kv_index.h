@@ -78,7 +78,4 @@ KV_HD uint64_t score_key(double x) {
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-// The CTA of a split of T steps over B CTAs (CTA b takes steps [⌊bT/B⌋, ⌊(b+1)T/B⌋), B <= T) that holds step x.
-KV_HD int64_t cta_of(int64_t x, int64_t T, int64_t B) { return (x * B + B - 1) / T; }
-
 }  // namespace g9kv

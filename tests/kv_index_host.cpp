@@ -25,5 +25,4 @@ int kv_page(const int *table, int64_t ts, int s, int place, int mp, int n_pages)
 int64_t kv_row(int id, int slot, int g, int64_t sp, int64_t sk, int64_t sh) { return g9kv::row_at(id, slot, g, sp, sk, sh); }
 uint32_t kv_wkey(float w) { return g9kv::weight_key(w); }
 uint64_t kv_skey(double x) { return g9kv::score_key(x); }
-int64_t kv_cta(int64_t x, int64_t T, int64_t B) { return g9kv::cta_of(x, T, B); }
 }

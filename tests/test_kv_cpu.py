@@ -26,8 +26,7 @@ def idx(tmp_path_factory):
     i, l, p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
     for name, args, res in (("kv_quot", [i, i], i), ("kv_quot_wrong", [i, l, l, l], l), ("kv_seen", [i] * 4, i),
                             ("kv_first", [i, i], i), ("kv_page", [p, l, i, i, i, i], i), ("kv_row", [i, i, i, l, l, l], l),
-                            ("kv_wkey", [ctypes.c_float], ctypes.c_uint32), ("kv_skey", [ctypes.c_double], ctypes.c_uint64),
-                            ("kv_cta", [l, l, l], l)):
+                            ("kv_wkey", [ctypes.c_float], ctypes.c_uint32), ("kv_skey", [ctypes.c_double], ctypes.c_uint64)):
         f = getattr(d, name)
         f.argtypes, f.restype = args, res
     return d
@@ -70,14 +69,6 @@ def test_keys_keep_the_order(idx):
     keys = [idx.kv_skey(v) for v in x]
     assert keys == sorted(keys) and len(set(keys)) == len(keys) and 0 < keys[0] and keys[-1] < 2 ** 64 - 1
     assert idx.kv_skey(-0.0) == idx.kv_skey(0.0) and idx.kv_skey(np.nan) == 0
-
-
-@pytest.mark.parametrize("T,B", [(1, 1), (7, 7), (100, 7), (296, 296), (12345, 296)])
-def test_split_of_the_steps(idx, T, B):
-    owner = [idx.kv_cta(x, T, B) for x in range(T)]
-    for b in range(B):
-        lo, hi = b * T // B, (b + 1) * T // B
-        assert hi > lo and owner[lo:hi] == [b] * (hi - lo)
 
 
 # ------------------------------------------------------------------------------------------------ refusals, no GPU
