@@ -71,6 +71,14 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     k->table = c->table;
     k->ts = c->ts;
     k->div = page_div(c->page);
+    if (!gen9blas_init() && !dev_state_if_ready(G.cur_dev)) {   // setting the device up allocates, which would end a capture
+        const cudaStream_t st = c->stream ? (cudaStream_t)c->stream : G.user_stream_set ? G.user_stream : nullptr;
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (st && cudaStreamIsCapturing(st, &cs) != cudaSuccess) cudaGetLastError();
+        if (cs != cudaStreamCaptureStatusNone)
+            return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: the first call on a device cannot be captured: make one before, with the "
+                        "workspace (gen9blas_kv_ws_create) of the captured one", who);
+    }
     if (int e = begin_op()) return e;
     call->d = dev_state();
     call->st = c->stream ? (cudaStream_t)c->stream : stream();

@@ -15,7 +15,8 @@ stride in the last dimension. Everything lies on one GPU; calls run on torch's c
 serving: results carry no gradient. Shape and type errors raise ValueError, library errors RuntimeError with gen9blas_error().
 
 One cache object is used by one thread at a time, as the library is. A captured call (torch.cuda.graph) needs a workspace
-of its own: pass `workspace=g9kv.Workspace()` to the constructor and make one call of each shape before the capture.
+of its own: pass `workspace=g9kv.Workspace()` to the constructor and make one call of each shape before the capture. The
+tensors and the workspace of a captured call have to live as long as its graph is replayed.
 """
 import ctypes
 import os
@@ -54,6 +55,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # torch's a
 if _raw_stream is None:
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
+_capturing = torch.cuda.is_current_stream_capturing
 _f32, _i32 = torch.float32, torch.int32
 _END = 2 ** 31   # of the library's counts; ctypes would cut larger ones short without a word
 
@@ -77,9 +79,11 @@ def set_device(index):
 
 
 class Workspace:
-    """Device memory for attend, select and evict of calls that run one after the other (see gen9blas_kv_ws_create)."""
+    """Device memory for attend, select and evict of calls that run one after the other (see gen9blas_kv_ws_create). One that
+    a captured call has used keeps its memory until `free`, whether or not anything still refers to it: its graph may."""
 
     def __init__(self):
+        self.captured = False
         self.handle = _fn["kv_ws_create"]()
         if not self.handle:
             raise RuntimeError(_fn["error"]().decode(errors="replace"))
@@ -90,7 +94,7 @@ class Workspace:
             self.handle = None
 
     def __del__(self):
-        if getattr(self, "handle", None) and _fn:
+        if getattr(self, "handle", None) and _fn and not self.captured:
             self.free()
 
 
@@ -141,6 +145,8 @@ class PagedKV:
             return None
         if not w.handle:
             raise ValueError("the cache's workspace has been freed")
+        if not w.captured and _capturing():
+            w.captured = True
         return w.handle
 
     # The checks run in every call, so their messages are put together only when one fails.

@@ -731,3 +731,53 @@ def test_append_of_more_tokens_than_the_table_holds(kv):
     for at in (8, 9, 2 ** 31 - 1):                                    # behind the table altogether
         assert cache.append(k, k, ints([at, at]), wait=True) is False
     assert torch.equal(K[:, 0].cpu().float(), want)
+
+
+def test_two_graphs_with_their_own_workspaces_at_once(kv):
+    """Replayed on two streams with nothing between them: each gives what its calls gave before the capture. The workspaces'
+    objects are gone by then; their memory stays, because captured calls have used it."""
+    rng = np.random.default_rng(41)
+    graphs = []
+    for k in range(2):
+        lens = [900 + 300 * k, 1200, 5]
+        _, K, V, table, bounds = make(rng, lens, 16, 2, 64, extra=8)
+        cache = kv.PagedKV(K, V, table, bounds=bounds, workspace=kv.Workspace())
+        q, vis = torch.randn(3, 2, 8, 64, device="cuda"), ints([n - 1 for n in lens])
+        acc = torch.zeros(3, 2, table.shape[1] * 16, device="cuda")
+
+        def step(cache=cache, q=q, vis=vis, acc=acc):
+            out, lse = cache.attend(q, vis, lse=True, acc=acc)
+            sel = cache.select(q, vis, 9)
+            return out, lse, sel, cache.attend(q, vis, sel=sel)
+        first = [x.clone() for x in step()]
+        torch.cuda.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step()
+        graphs.append((graph, stream, out, first, (K, V, table, bounds, q, vis, acc)))     # the workspace: no one's any more
+        del step, cache
+    torch.cuda.synchronize()
+    for _ in range(50):
+        for graph, stream, *_ in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, first, _ in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("vis,step,window", [([2 ** 31 - 1, -2 ** 31, 100], 1, 0), ([2 ** 31 - 1] * 3, 2 ** 31 - 1, 0),
+                                             ([-5, 0, 2 ** 31 - 1], 2 ** 31 - 1, 2 ** 31 - 1), ([100, 100, 100], 0, 1)])
+def test_counts_at_the_ends_of_their_type(kv, vis, step, window):
+    rng = np.random.default_rng(42)
+    host, K, V, table, bounds = make(rng, [100, 100, 100], 10, 2, 64)
+    q = rng.standard_normal((3, 2, 4, 64)).astype(np.float32)
+    cache = kv.PagedKV(K, V, table, bounds=bounds)
+    attend_close(cache.attend(torch.from_numpy(q).cuda(), ints(vis), step=step, window=window, lse=True),
+                 kv_ref.attend(host, q, vis, step=step, window=window), 64)
+    got = cache.select(torch.from_numpy(q).cuda(), ints(vis), 4, step=step)
+    assert np.array_equal(got.cpu().numpy(), kv_ref.select(host, q, vis, 4, step=step))
+    acc = torch.rand(3, 2, 100, device="cuda")
+    before = K.clone()
+    assert cache.evict(ints(vis), 2 ** 31 - 1, acc).tolist() == [min(max(v, 0), 100) for v in vis]
+    assert torch.equal(K, before)
