@@ -1429,6 +1429,7 @@ size_t marks_bytes(const KvDev &c, int64_t ms, int64_t mh) {
     return ((size_t)std::max(c.ns - 1, 0) * (size_t)std::max<int64_t>(ms, 0) + (size_t)(c.HKV - 1) * (size_t)std::max<int64_t>(mh, 0) +
             (size_t)c.cap) * 4;
 }
+size_t bounds_bytes(const KvDev &c) { return (size_t)c.n_pages * (size_t)c.HKV * 2 * (size_t)c.D * sizeof(__half); }
 // A cluster of `size` CTAs per row, with programmatic stream serialization as launch_pdl.
 template <int ET, int ER>
 int rank_launch(const EvictArgs &a, const KvCall &call, long long rows, int size) {
@@ -1547,8 +1548,9 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
     G9_CU(launch_pdl(kv_append_k, dim3((unsigned)a.tp, (unsigned)c->HKV, (unsigned)c->ns), dim3(32 * warps), 0, call.st, a, lpr));
     G9_TRY(launched("kv_append"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const QueuedWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};   // positions are no early reader's operand
-    G9_TRY(kv_finish(call, sync, w, 3));
+    // positions and lengths are no early reader's operand; the bounds can be one, as the weights of a product
+    const QueuedWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {c->bounds, bounds_bytes(a.c)}};
+    G9_TRY(kv_finish(call, sync, w, 4));
     if (sync && bad) *bad = (int)*flag;
     return 0;
 }
@@ -1697,8 +1699,8 @@ GEN9BLAS_API int gen9blas_kv_evict(const gen9blas_kv_cache *c, const int *len, i
     G9_CU(launch_pdl(kv_move_k, dim3((unsigned)(rows * ctas)), dim3(MT), 0, call.st, a, (int)ctas, lpr, team));
     G9_TRY(launched("kv_move"));
     const size_t marks = marks_bytes(a.c, ms, mh);
-    const QueuedWrite w[3] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}};
-    return kv_finish(call, sync, w, 3);
+    const QueuedWrite w[4] = {{c->K, c->k_bytes}, {c->V, c->v_bytes}, {acc, marks}, {c->bounds, bounds_bytes(a.c)}};
+    return kv_finish(call, sync, w, 4);
 }
 
 }  // extern "C"

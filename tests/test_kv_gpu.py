@@ -781,3 +781,45 @@ def test_counts_at_the_ends_of_their_type(kv, vis, step, window):
     before = K.clone()
     assert cache.evict(ints(vis), 2 ** 31 - 1, acc).tolist() == [min(max(v, 0), 100) for v in vis]
     assert torch.equal(K, before)
+
+
+@pytest.mark.parametrize("call", ["append", "evict"])
+@pytest.mark.parametrize("tokens", [1, 16])
+def test_queued_bounds_are_seen_by_a_product_with_them(kv, gpu_lib, call, tokens):
+    """Bounds as the weights of an FP16 product (a caller's own page scores) right behind the call that writes them: the
+    product's first loads may precede its wait on the kernel before, unless the ledger of queued writes holds the bounds.
+    The product's FP32 sums of exact products over D = 64 are off by 64 roundings of the sum of their absolute values, and its
+    FP16 result by half a step more."""
+    D, heads, page, mp, ns = 64, 2, 16, 512, 4
+    K = torch.zeros(ns * mp, heads, page, D, dtype=torch.float16, device="cuda")
+    V = torch.zeros_like(K)
+    bounds = torch.zeros(ns * mp, heads, 2, D, dtype=torch.float16, device="cuda")
+    table = ints(np.arange(ns * mp).reshape(ns, mp))
+    cache = kv.PagedKV(K, V, table, bounds=bounds)
+    n = mp * page
+    full, zero = ints([n] * ns), ints([0] * ns)
+    A = torch.randn(tokens, D, device="cuda").half()
+    rows = ns * mp * heads * 2
+    C = torch.empty(tokens, rows, dtype=torch.float16, device="cuda")
+    acc = torch.rand(ns, heads, n, device="cuda")
+    for it in range(4):
+        k = torch.randn(ns, n, heads, D, device="cuda") + it
+        if call == "evict":
+            cache.append(k, k, zero)
+        torch.cuda.synchronize()
+        assert gpu_lib.set_stream(torch.cuda.current_stream().cuda_stream or 1) == 0
+        gpu_lib.set_nowait(1)
+        try:
+            if call == "append":
+                cache.append(k, k, zero)
+            else:
+                cache.evict(full, n // 2, acc)
+            status = gpu_lib.gemm(0, 0, 1, tokens, rows, D, 1.0, A.data_ptr(), D, bounds.data_ptr(), D, 0.0, C.data_ptr(), rows)
+        finally:
+            gpu_lib.set_nowait(0)
+            assert gpu_lib.set_stream(None) == 0
+        torch.cuda.synchronize()
+        assert status == 0, gpu_lib.error()
+        W = bounds.reshape(rows, D).double()
+        ref, mass = A.double() @ W.T, A.double().abs() @ W.abs().T
+        assert bool(((C.double() - ref).abs() <= mass * D * 2.0 ** -24 + ref.abs() * 2.0 ** -11 + 2.0 ** -24).all()), it
