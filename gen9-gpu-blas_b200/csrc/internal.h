@@ -6,6 +6,7 @@
 // gen9blas_set_device. Everything in this header has hidden visibility.
 #pragma once
 #include "gen9blas.h"
+#include "ledger.h"
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstddef>
@@ -19,6 +20,14 @@ constexpr int kStageSlots = 3;   // staged operands per call (A, B, C or x, y, A
 
 // Device-side error codes written into DevState::err_host by kernels whose waits gave up.
 enum : unsigned { kDevErrNone = 0, kDevErrWaitTimeout = 1, kDevErrTmemAlloc = 2 };
+
+struct LedgerApi {
+    using Stream = cudaStream_t;
+    using Event = cudaEvent_t;
+    static bool record(Event &e, Stream st);
+    static bool done(Event e);
+    static void wait(Stream st);
+};
 
 struct DevState {
     bool ready = false;
@@ -51,19 +60,9 @@ struct DevState {
     unsigned *at_cnt = nullptr;                                // arrival counters of the attention kernel's rows and
     size_t at_cnt_n = 0;                                       // the FFN gate / up pairs (zeroed when created or
                                                                // grown; each call leaves every counter it used at 0)
-    // Device ranges written by no-wait calls that may still be queued, each with an event recorded right after the
-    // call that wrote it (an entry whose event has completed is dropped); a kernel that reads an input before
-    // griddepcontrol.wait checks its input against them. An entry holds writes of one stream, and waiting for a stream
-    // drops that stream's entries only.
-    static constexpr int kQueuedRanges = 32;
-    uintptr_t queued_lo[kQueuedRanges] = {}, queued_hi[kQueuedRanges] = {};
-    int queued_ev[kQueuedRanges] = {};                         // the entry's event: ranges of one call share one
-    cudaEvent_t queued_evs[kQueuedRanges + 1] = {};
-    int queued_ev_used[kQueuedRanges + 1] = {};                // entries that hold it
-    cudaStream_t queued_st[kQueuedRanges] = {};
-    int queued_n = 0;
-    bool queued_overflow = false, queued_overflow_many = false;   // a write that has no entry; such writes of several streams
-    cudaStream_t queued_overflow_st = nullptr;
+    // Device ranges written by no-wait calls that may still be queued; a kernel that reads an input before
+    // griddepcontrol.wait checks its input against them.
+    QueuedLedger<LedgerApi> queued;
     bool queued_captured = false;   // captured calls have written ranges without an entry: later captured ones ask no more
     void *shard = nullptr;                                     // operand copies of a column-sharded GEMM (grow-only)
     size_t shard_n = 0;
@@ -131,16 +130,10 @@ int map_operand(Operand &op, const void *p, size_t bytes, int slot, bool copy_in
 // Ends a call: waits for the stream (unless no-wait applies), copies staged written operands back, checks the
 // device error word. ops may be empty.
 int finish_op(Operand *ops, int n);
-// Ledger of the outputs of queued no-wait calls (see DevState::queued_lo): add a range, forget them all once the
-// library's stream has been waited for, and ask whether [p, p + bytes) may still be written by queued work (true also
-// when more ranges were queued than the ledger holds).
-struct QueuedWrite {
-    const void *p;   // NULL: none
-    size_t bytes;
-};
-void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st);   // the ranges of one call
-void queued_writes_lost(DevState *d, cudaStream_t st);    // a write on st that has no entry
-void queued_writes_clear(DevState *d, cudaStream_t st);   // st has been waited for
+// The ledger of a device's queued calls (DevState::queued): adds the ranges that one call has written,
+// forgets those of a stream that has been waited for, and asks whether [p, p + bytes) may still be written by queued work.
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st);
+void queued_writes_clear(DevState *d, cudaStream_t st);
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes);
 // Hand-over flags of the GEMM kernels that split tiles over CTAs (kGemmFlags zeroed words, created on first use) and
 // the epoch of the launch about to be enqueued (never 0).

@@ -1,0 +1,141 @@
+// ledger.h -- the ledger of queued writes: which device ranges calls that were queued without a wait may still write. A kernel
+// that reads an input before griddepcontrol.wait asks it first. Plain C++ over a few operations on events and streams, so that
+// its rules are checked on the CPU (tests/test_ledger_cpu.py compiles this file with a scripted Api).
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+namespace g9 {
+
+struct QueuedWrite {
+    const void *p;   // NULL: none
+    size_t bytes;
+};
+
+// Api: Stream and Event types (a default Event is "not made yet") and, all static,
+//   bool record(Event &, Stream)   records the event behind all work queued on the stream so far (makes it on first use); false: cannot
+//   bool done(Event)               whether that work has ended (false also where it cannot tell)
+//   void wait(Stream)              waits for the stream
+template <typename Api>
+class QueuedLedger {
+    using Stream = typename Api::Stream;
+    using Event = typename Api::Event;
+
+public:
+    static constexpr int kRanges = 32;
+    static constexpr int kLost = 16;
+
+    // The ranges of one call, queued on st just now. They share one event, recorded for the first of them.
+    void add(const QueuedWrite *w, int n, Stream st) {
+        int ev = -1;
+        for (int k = 0; k < n; k++) {
+            if (!w[k].p || !w[k].bytes) continue;
+            if (ev < 0) {
+                for (ev = 0; used_[ev]; ev++) {}   // one event more than there are entries
+                if (!Api::record(ev_[ev], st)) return lost(st);
+            }
+            const uintptr_t lo = (uintptr_t)w[k].p, hi = lo + w[k].bytes;
+            const int i = slot(lo, hi, st);
+            if (i < 0) return lost(st);
+            Entry &e = e_[i];
+            if (i == n_) {
+                n_++;
+                e.lo = lo;
+                e.hi = hi;
+                e.st = st;
+            } else {
+                used_[e.ev]--;
+                if (lo < e.lo) e.lo = lo;
+                if (hi > e.hi) e.hi = hi;
+            }
+            e.ev = ev;
+            used_[ev]++;
+        }
+    }
+
+    // st has been waited for: its writes are done.
+    void clear(Stream st) {
+        for (int i = n_ - 1; i >= 0; i--)
+            if (e_[i].st == st) drop(i);
+        for (int i = lost_n_ - 1; i >= 0; i--)
+            if (lost_[i].st == st) lost_drop(i);
+    }
+
+    // Whether queued work may still write some of [p, p + bytes): by the entries, or always while a write without one is under way.
+    bool overlap(const void *p, size_t bytes) {
+        for (int i = lost_n_ - 1; i >= 0; i--)
+            if (Api::done(lost_[i].ev)) lost_drop(i);
+        if (lost_n_) return true;
+        const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+        for (int i = n_ - 1; i >= 0; i--) {
+            if (!(lo < e_[i].hi && e_[i].lo < hi)) continue;
+            if (!Api::done(ev_[e_[i].ev])) return true;
+            drop(i);
+        }
+        return false;
+    }
+
+private:
+    // An entry holds writes of one stream, up to its event.
+    struct Entry {
+        uintptr_t lo, hi;
+        Stream st;
+        int ev;
+    };
+    struct Lost {
+        Stream st;
+        Event ev{};
+    };
+    Entry e_[kRanges];
+    int n_ = 0;
+    Event ev_[kRanges + 1]{};
+    int used_[kRanges + 1] = {};   // entries that hold the event
+    Lost lost_[kLost]{};           // streams with writes that found no entry, each with an event behind the last of them
+    int lost_n_ = 0;
+
+    // The entry that takes a range of stream st: one that it overlaps or touches, a free one, or, where all are taken, that
+    // of the stream which grows least. -1: all belong to other streams.
+    int slot(uintptr_t lo, uintptr_t hi, Stream st) {
+        for (int i = 0; i < n_; i++)
+            if (lo <= e_[i].hi && e_[i].lo <= hi && e_[i].st == st) return i;
+        if (n_ == kRanges)
+            for (int i = n_ - 1; i >= 0; i--)   // full: forget the writes that have completed
+                if (Api::done(ev_[e_[i].ev])) drop(i);
+        if (n_ < kRanges) return n_;
+        int best = -1;
+        size_t least = SIZE_MAX;
+        for (int i = 0; i < n_; i++) {
+            if (e_[i].st != st) continue;
+            const size_t grown = lo < e_[i].lo ? e_[i].lo - lo : hi > e_[i].hi ? hi - e_[i].hi : 0;
+            if (grown < least) {
+                least = grown;
+                best = i;
+            }
+        }
+        return best;
+    }
+
+    // The last entry takes the place of one that is dropped.
+    void drop(int i) {
+        used_[e_[i].ev]--;
+        e_[i] = e_[--n_];
+    }
+    void lost_drop(int i) {
+        const Lost gone = lost_[i];
+        lost_[i] = lost_[--lost_n_];
+        lost_[lost_n_] = gone;   // its event is kept for the next one
+    }
+
+    // A write on st that has no entry: overlap() answers true until it has ended. Where that could not be told, it is waited for.
+    void lost(Stream st) {
+        for (int i = lost_n_ - 1; i >= 0; i--)
+            if (Api::done(lost_[i].ev)) lost_drop(i);
+        int i = 0;
+        while (i < lost_n_ && lost_[i].st != st) i++;
+        if (i == kLost || !Api::record(lost_[i].ev, st)) return Api::wait(st);
+        lost_[i].st = st;
+        if (i == lost_n_) lost_n_++;
+    }
+};
+
+}  // namespace g9

@@ -317,96 +317,24 @@ int check_dev_err(DevState *d) {
     return 0;
 }
 
-// Drops entry i (its write has completed), keeping the others' order irrelevant: the last entry takes its place.
-static void queued_drop(DevState *d, int i) {
-    const int last = d->queued_n - 1;
-    d->queued_ev_used[d->queued_ev[i]]--;
-    if (i != last) {
-        d->queued_lo[i] = d->queued_lo[last];
-        d->queued_hi[i] = d->queued_hi[last];
-        d->queued_ev[i] = d->queued_ev[last];
-        d->queued_st[i] = d->queued_st[last];
-    }
-    d->queued_n = last;
-}
-
-static bool queued_done(DevState *d, int i) {
-    const cudaError_t e = cudaEventQuery(d->queued_evs[d->queued_ev[i]]);
-    if (e == cudaErrorNotReady) return false;
+bool LedgerApi::record(Event &e, Stream st) {
+    if ((e || cudaEventCreateWithFlags(&e, cudaEventDisableTiming) == cudaSuccess) && cudaEventRecord(e, st) == cudaSuccess) return true;
     cudaGetLastError();
-    return e == cudaSuccess;
+    return false;
+}
+bool LedgerApi::done(Event e) {
+    const cudaError_t r = cudaEventQuery(e);
+    if (r == cudaErrorNotReady) return false;
+    cudaGetLastError();
+    return r == cudaSuccess;
+}
+void LedgerApi::wait(Stream st) {
+    if (cudaStreamSynchronize(st) != cudaSuccess) cudaGetLastError();   // the next call meets what has failed
 }
 
-// The entry that takes a range of stream st: one that it overlaps or touches, a free one, or, where all are taken, that
-// of the stream which grows least. -1: all belong to other streams.
-static int queued_slot(DevState *d, uintptr_t lo, uintptr_t hi, cudaStream_t st) {
-    for (int i = 0; i < d->queued_n; i++)
-        if (lo <= d->queued_hi[i] && d->queued_lo[i] <= hi && d->queued_st[i] == st) return i;
-    if (d->queued_n == DevState::kQueuedRanges)
-        for (int i = d->queued_n - 1; i >= 0; i--)       // full: forget the writes that have completed
-            if (queued_done(d, i)) queued_drop(d, i);
-    if (d->queued_n < DevState::kQueuedRanges) return d->queued_n;
-    int slot = -1;
-    size_t least = SIZE_MAX;
-    for (int i = 0; i < d->queued_n; i++) {
-        if (d->queued_st[i] != st) continue;
-        const size_t grown = lo < d->queued_lo[i] ? d->queued_lo[i] - lo : hi > d->queued_hi[i] ? hi - d->queued_hi[i] : 0;
-        if (grown < least) {
-            least = grown;
-            slot = i;
-        }
-    }
-    return slot;
-}
-
-void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st) {
-    int ev = -1;   // recorded behind the call for the first of its ranges
-    for (int k = 0; k < n; k++) {
-        if (!w[k].p || !w[k].bytes) continue;
-        if (ev < 0) {
-            for (ev = 0; d->queued_ev_used[ev]; ev++) {}   // one event more than there are entries
-            if ((!d->queued_evs[ev] && cudaEventCreateWithFlags(&d->queued_evs[ev], cudaEventDisableTiming) != cudaSuccess) ||
-                cudaEventRecord(d->queued_evs[ev], st) != cudaSuccess) {
-                cudaGetLastError();
-                queued_writes_lost(d, st);   // cannot tell when it completes: stay conservative
-                return;
-            }
-        }
-        const uintptr_t lo = (uintptr_t)w[k].p, hi = lo + w[k].bytes;
-        const int i = queued_slot(d, lo, hi, st);
-        if (i < 0) {
-            queued_writes_lost(d, st);       // every later check answers "maybe written"
-            return;
-        }
-        if (i == d->queued_n) {
-            d->queued_n++;
-            d->queued_lo[i] = lo;
-            d->queued_hi[i] = hi;
-            d->queued_st[i] = st;
-        } else {
-            d->queued_ev_used[d->queued_ev[i]]--;
-            if (lo < d->queued_lo[i]) d->queued_lo[i] = lo;
-            if (hi > d->queued_hi[i]) d->queued_hi[i] = hi;
-        }
-        d->queued_ev[i] = ev;
-        d->queued_ev_used[ev]++;
-    }
-}
-
-void queued_writes_lost(DevState *d, cudaStream_t st) {
-    d->queued_overflow_many = d->queued_overflow && (d->queued_overflow_many || d->queued_overflow_st != st);
-    d->queued_overflow = true;
-    d->queued_overflow_st = st;
-}
-
-void queued_writes_clear(DevState *d, cudaStream_t st) {
-    for (int i = d->queued_n - 1; i >= 0; i--)
-        if (d->queued_st[i] == st) queued_drop(d, i);
-    if (d->queued_overflow_st == st && !d->queued_overflow_many) d->queued_overflow = false;
-}
-
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st) { d->queued.add(w, n, st); }
+void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
-    if (d->queued_overflow) return true;
     if (d->queued_captured) {   // calls outside a capture start after a replayed graph as a whole
         cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
         if (cudaStreamIsCapturing(stream(), &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
@@ -414,13 +342,7 @@ bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
             return true;
         }
     }
-    const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
-    for (int i = d->queued_n - 1; i >= 0; i--) {
-        if (!(lo < d->queued_hi[i] && d->queued_lo[i] < hi)) continue;
-        if (!queued_done(d, i)) return true;
-        queued_drop(d, i);   // that write has finished
-    }
-    return false;
+    return d->queued.overlap(p, bytes);
 }
 
 int finish_op(Operand *ops, int n) {

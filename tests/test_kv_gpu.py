@@ -823,3 +823,36 @@ def test_queued_bounds_are_seen_by_a_product_with_them(kv, gpu_lib, call, tokens
         W = bounds.reshape(rows, D).double()
         ref, mass = A.double() @ W.T, A.double().abs() @ W.abs().T
         assert bool(((C.double() - ref).abs() <= mass * D * 2.0 ** -24 + ref.abs() * 2.0 ** -11 + 2.0 ** -24).all()), it
+
+
+def test_writes_of_more_streams_than_the_ledger_holds(kv, gpu_lib):
+    """Appends on 40 streams at once, each read back by the contiguous attention of its stream; twice."""
+    D, heads, n = 128, 1, 256
+    streams = [torch.cuda.Stream() for _ in range(40)]
+    K = torch.zeros(40, 1, heads, n, D, dtype=torch.float16, device="cuda")
+    V = torch.zeros_like(K)
+    q, O = torch.randn(40, 1, 1, 4, D, device="cuda"), torch.empty(40, 1, 1, 4, D, device="cuda")
+    table, zero, vis = ints([[0]]), ints([0]), ints([n])
+    caches = [kv.PagedKV(K[i], V[i], table) for i in range(40)]
+    for it in range(2):
+        k, v = (torch.randn(40, 1, n, heads, D, device="cuda") for _ in range(2))
+        torch.cuda.synchronize()
+        try:
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    for _ in range(3):
+                        caches[i].append(k[i], v[i], zero)
+            for i, st in enumerate(streams):
+                assert gpu_lib.set_stream(st.cuda_stream) == 0
+                size = K[i].numel() * 2
+                assert gpu_lib.attn_dec(D, 4, heads, 1, 1, n, q[i].data_ptr(), 4 * D, D, 4 * D, K[i].data_ptr(), D, n * D, n * D, size,
+                                        V[i].data_ptr(), D, n * D, n * D, size, O[i].data_ptr(), D ** -0.5, vis.data_ptr(), 0, 0,
+                                        1) == 0, gpu_lib.error()
+        finally:
+            assert gpu_lib.set_stream(None) == 0
+        torch.cuda.synchronize()
+        for i in range(0, 40, 7):
+            host = {"K": k[i].half().cpu().numpy().transpose(0, 2, 1, 3), "V": v[i].half().cpu().numpy().transpose(0, 2, 1, 3),
+                    "table": np.zeros((1, 1), np.int32), "bounds": None}
+            ref = kv_ref.attend(host, q[i].cpu().numpy(), [n])
+            attend_close((O[i], torch.from_numpy(ref[1])), ref, D)
