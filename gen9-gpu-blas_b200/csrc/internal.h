@@ -130,9 +130,13 @@ int map_operand(Operand &op, const void *p, size_t bytes, int slot, bool copy_in
 // Ends a call: waits for the stream (unless no-wait applies), copies staged written operands back, checks the
 // device error word. ops may be empty.
 int finish_op(Operand *ops, int n);
+// The capture that a stream is in: its number, 0 for none, kCaptureUnknown where the stream cannot tell.
+constexpr unsigned long long kCaptureUnknown = ~0ull;
+unsigned long long capture_of(cudaStream_t st);
 // The ledger of a device's queued calls (DevState::queued): adds the ranges that one call has written,
 // forgets those of a stream that has been waited for, and asks whether [p, p + bytes) may still be written by queued work.
-void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st);
+// capture: that of the stream (capture_of).
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st, unsigned long long capture);
 void queued_writes_clear(DevState *d, cudaStream_t st);
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes);
 // Hand-over flags of the GEMM kernels that split tiles over CTAs (kGemmFlags zeroed words, created on first use) and

@@ -82,10 +82,8 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     if (int e = begin_op()) return e;
     call->d = dev_state();
     call->st = c->stream ? (cudaStream_t)c->stream : stream();
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    G9_CU(cudaStreamIsCapturing(call->st, &cs));
-    call->capturing = cs != cudaStreamCaptureStatusNone;
-    if (call->capturing && sync)
+    call->capture = capture_of(call->st);
+    if (call->capture && sync)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: sync = 1 while the stream is being captured", who);
     if (c->n_pages > 0) {
         G9_TRY(kv_operand(*call, c->K, who, "K"));
@@ -136,7 +134,7 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
                  unsigned **cnt) {
     const bool own = ws == nullptr;
     if (own) {
-        if (call.capturing)
+        if (call.capture)
             return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: a captured call needs a workspace (gen9blas_kv_ws_create)", who);
         ws = &g_ws[call.d->dev];
         ws->magic = kKvWsMagic;
@@ -148,7 +146,7 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: the workspace belongs to device %d, the current device is %d", who, ws->dev,
                     call.d->dev);
     const bool grow = ws->n < bytes || ws->cnt_n < counters;
-    if (call.capturing) {
+    if (call.capture) {
         if (grow)
             return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: the workspace is too small and cannot grow during a capture: make a call "
                         "of this shape before it", who);
@@ -201,16 +199,12 @@ int kv_workspace(gen9blas_kv_ws *ws, const KvCall &call, const char *who, size_t
 int kv_too_large(const char *who) { return fail(GEN9BLAS_ERR_OUT_OF_MEMORY, "%s: the call's workspace passes 2^46 bytes", who); }
 
 int kv_finish(const KvCall &call, int sync, const QueuedWrite *w, int n) {
-    if (call.capturing) {
-        call.d->queued_captured = true;   // an event recorded here could not be queried
-        return 0;
-    }
     if (sync) {
         G9_CU(cudaStreamSynchronize(call.st));
         queued_writes_clear(call.d, call.st);
         return check_dev_err(call.d);
     }
-    queued_writes_add(call.d, w, n, call.st);
+    queued_writes_add(call.d, w, n, call.st, call.capture);
     return 0;
 }
 

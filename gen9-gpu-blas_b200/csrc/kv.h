@@ -36,11 +36,11 @@ struct KvDev {
     g9kv::PageDiv div;
 };
 
-// One call: its stream and whether that is being captured.
+// One call: its stream and the capture that is in (0: none).
 struct KvCall {
     DevState *d = nullptr;
     cudaStream_t st = nullptr;
-    bool capturing = false;
+    unsigned long long capture = 0;
 };
 
 // Starts a call: checks the cache's description and the shape (H = HKV for calls without query heads), then the device

@@ -825,7 +825,7 @@ extern "C" GEN9BLAS_API int gen9blas_gemv_noalloc(int type, int trans, int M, in
         G9_CU(cudaStreamSynchronize(st));
     } else if (ds) {   // queued on the library's stream: later calls that read y early must know
         const QueuedWrite w = {y, vec_span(ny, incy) * (size_t)es};
-        queued_writes_add(ds, &w, 1, st);
+        queued_writes_add(ds, &w, 1, st, 0);
     }
     return 0;
 }

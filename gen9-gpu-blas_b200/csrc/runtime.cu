@@ -323,7 +323,11 @@ bool LedgerApi::record(Event &e, Stream st) {
     return false;
 }
 bool LedgerApi::done(Event e) {
+    // asking for an event ends another stream's capture of this thread, unless the thread says that it means no harm
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
     const cudaError_t r = cudaEventQuery(e);
+    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     if (r == cudaErrorNotReady) return false;
     cudaGetLastError();
     return r == cudaSuccess;
@@ -332,16 +336,26 @@ void LedgerApi::wait(Stream st) {
     if (cudaStreamSynchronize(st) != cudaSuccess) cudaGetLastError();   // the next call meets what has failed
 }
 
-void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st) { d->queued.add(w, n, st); }
-void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
-bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
-    if (d->queued_captured) {   // calls outside a capture start after a replayed graph as a whole
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream(), &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
-            cudaGetLastError();
-            return true;
-        }
+unsigned long long capture_of(cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(st, &cs, &id) != cudaSuccess) {
+        cudaGetLastError();
+        return kCaptureUnknown;
     }
+    return cs == cudaStreamCaptureStatusNone ? 0 : cs == cudaStreamCaptureStatusActive && id ? id : kCaptureUnknown;
+}
+
+void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st, unsigned long long capture) {
+    if (capture) d->queued_captured = true;   // an event recorded here could not be queried
+    else d->queued.add(w, n, st);
+}
+void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
+// Within a capture only captured writes count: whatever else is queued has ended when a replay starts, as a replay has when a
+// call outside a capture starts. (And what is queued cannot be asked about there: the query would end the capture.)
+bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
+    const unsigned long long capture = capture_of(stream());
+    if (capture) return capture == kCaptureUnknown || d->queued_captured;
     return d->queued.overlap(p, bytes);
 }
 
@@ -352,10 +366,11 @@ int finish_op(Operand *ops, int n) {
     bool all_zc = true;
     for (int i = 0; i < n; i++) all_zc = all_zc && ops[i].zc;
     if (G.nowait && all_zc) {
+        const unsigned long long capture = capture_of(st);
         for (int i = 0; i < n; i++)
             if (ops[i].written) {
                 const QueuedWrite w = {ops[i].dptr, ops[i].bytes};
-                queued_writes_add(d, &w, 1, st);
+                queued_writes_add(d, &w, 1, st, capture);
             }
         return 0;
     }

@@ -856,3 +856,54 @@ def test_writes_of_more_streams_than_the_ledger_holds(kv, gpu_lib):
                     "table": np.zeros((1, 1), np.int32), "bounds": None}
             ref = kv_ref.attend(host, q[i].cpu().numpy(), [n])
             attend_close((O[i], torch.from_numpy(ref[1])), ref, D)
+
+
+def _dec(gpu_lib, K, V, q, O, n, vis):
+    """gen9blas_attn_dec of all keys of a contiguous [1, heads, n, D] cache on torch's current stream, queued."""
+    heads, D = K.shape[1], K.shape[3]
+    H, size = q.shape[2], K.numel() * 2
+    assert gpu_lib.set_stream(torch.cuda.current_stream().cuda_stream or 1) == 0
+    try:
+        return gpu_lib.attn_dec(D, H, heads, 1, 1, n, q.data_ptr(), H * D, D, H * D, K.data_ptr(), D, n * D, heads * n * D, size,
+                                V.data_ptr(), D, n * D, heads * n * D, size, O.data_ptr(), D ** -0.5, vis.data_ptr(), 0, 0, 0)
+    finally:
+        assert gpu_lib.set_stream(None) == 0
+
+
+@pytest.mark.parametrize("where", ["captured", "beside a capture"])
+def test_a_write_in_the_queue_does_not_end_a_capture(kv, gpu_lib, where):
+    """append queued outside of a capture; then the contiguous attention of the same memory, itself captured, or called on
+    another stream while a capture runs: the ledger has an entry for its keys and must not ask for its event there."""
+    D, heads, n = 128, 2, 4096
+    K = torch.zeros(1, heads, n, D, dtype=torch.float16, device="cuda")
+    V = torch.zeros_like(K)
+    q, O, x = torch.randn(1, 1, 8, D, device="cuda"), torch.zeros(1, 1, 8, D, device="cuda"), torch.zeros(1, device="cuda")
+    cache, vis, zero = kv.PagedKV(K, V, ints([[0]])), ints([n]), ints([0])
+    k, v = (torch.randn(1, n, heads, D, device="cuda") for _ in range(2))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert _dec(gpu_lib, K, V, q, O, n, vis) == 0          # buffers and kernels are there before the capture
+    with torch.cuda.stream(side):
+        assert _dec(gpu_lib, K, V, q, O, n, vis) == 0
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    if where == "captured":
+        cache.append(k, v, zero)
+        with torch.cuda.graph(graph):
+            x.add_(1)
+            assert _dec(gpu_lib, K, V, q, O, n, vis) == 0, gpu_lib.error()
+        assert not O.any()
+    else:
+        with torch.cuda.stream(side):
+            cache.append(k, v, zero)
+        with torch.cuda.graph(graph):
+            x.add_(1)
+            with torch.cuda.stream(side):
+                assert _dec(gpu_lib, K, V, q, O, n, vis) == 0, gpu_lib.error()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert x.item() == 1
+    host = {"K": k.half().cpu().numpy().transpose(0, 2, 1, 3), "V": v.half().cpu().numpy().transpose(0, 2, 1, 3),
+            "table": np.zeros((1, 1), np.int32), "bounds": None}
+    ref = kv_ref.attend(host, q.cpu().numpy(), [n])
+    attend_close((O, torch.from_numpy(ref[1])), ref, D)
