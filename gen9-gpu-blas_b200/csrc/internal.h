@@ -63,7 +63,7 @@ struct DevState {
     // Device ranges written by no-wait calls that may still be queued; a kernel that reads an input before
     // griddepcontrol.wait checks its input against them.
     QueuedLedger<LedgerApi> queued;
-    bool queued_captured = false;   // captured calls have written ranges without an entry: later captured ones ask no more
+    CaptureLedger queued_captured;                             // the same of calls captured into graphs
     void *shard = nullptr;                                     // operand copies of a column-sharded GEMM (grow-only)
     size_t shard_n = 0;
     void *ml = nullptr;                                        // FP16 activations / results of the ML entry points

@@ -138,4 +138,84 @@ private:
     }
 };
 
+// The ranges that captured calls write, by the capture's number: within its graph a kernel may start before the one ahead of it
+// has ended. A replay as a whole starts and ends in its stream's order, so that a record matters to calls of the same capture
+// alone, and its end needs no event. The latest kCaptures captures are kept; one older than those that went is answered for
+// as if it wrote everything (numbers rise; where they did not, that is what a new capture would get).
+class CaptureLedger {
+public:
+    static constexpr int kCaptures = 32;
+    static constexpr int kRanges = 24;
+
+    void add(const QueuedWrite *w, int n, unsigned long long capture) {
+        if (lost(capture)) return;
+        Record &r = record(capture);
+        for (int k = 0; k < n; k++) {
+            if (!w[k].p || !w[k].bytes) continue;
+            const uintptr_t lo = (uintptr_t)w[k].p, hi = lo + w[k].bytes;
+            int best = 0;
+            size_t least = SIZE_MAX;
+            for (int i = 0; i < r.n; i++) {   // 0: overlapping or touching
+                const size_t far = lo > r.hi[i] ? lo - r.hi[i] : r.lo[i] > hi ? r.lo[i] - hi : 0;
+                if (far < least) {
+                    least = far;
+                    best = i;
+                }
+            }
+            if (least > 0 && r.n < kRanges) {
+                best = r.n++;
+                r.lo[best] = lo;
+                r.hi[best] = hi;
+            } else {                          // full: the nearest one grows over what lies between
+                if (lo < r.lo[best]) r.lo[best] = lo;
+                if (hi > r.hi[best]) r.hi[best] = hi;
+            }
+        }
+    }
+
+    bool overlap(const void *p, size_t bytes, unsigned long long capture) const {
+        if (lost(capture)) return true;
+        const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+        for (int i = 0; i < n_; i++) {
+            if (r_[i].capture != capture) continue;
+            for (int k = 0; k < r_[i].n; k++)
+                if (lo < r_[i].hi[k] && r_[i].lo[k] < hi) return true;
+        }
+        return false;
+    }
+
+private:
+    struct Record {
+        unsigned long long capture, used;   // used: when a range was last added
+        int n;
+        uintptr_t lo[kRanges], hi[kRanges];
+    };
+    Record r_[kCaptures];
+    int n_ = 0;
+    unsigned long long clock_ = 0, gone_ = 0;   // gone_: the highest number of those that went
+
+    bool lost(unsigned long long capture) const {
+        if (capture > gone_) return false;
+        for (int i = 0; i < n_; i++)
+            if (r_[i].capture == capture) return false;
+        return true;
+    }
+    Record &record(unsigned long long capture) {
+        int at = 0;
+        for (int i = 0; i < n_; i++) {
+            if (r_[i].capture == capture) {
+                r_[i].used = ++clock_;
+                return r_[i];
+            }
+            if (r_[i].used < r_[at].used) at = i;
+        }
+        if (n_ < kCaptures) at = n_++;
+        else if (r_[at].capture > gone_) gone_ = r_[at].capture;
+        r_[at].capture = capture;
+        r_[at].used = ++clock_;
+        r_[at].n = 0;
+        return r_[at];
+    }
+};
+
 }  // namespace g9

@@ -347,7 +347,8 @@ unsigned long long capture_of(cudaStream_t st) {
 }
 
 void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st, unsigned long long capture) {
-    if (capture) d->queued_captured = true;   // an event recorded here could not be queried
+    if (capture == kCaptureUnknown) return;   // a capture that has failed: nothing of it will run
+    if (capture) d->queued_captured.add(w, n, capture);
     else d->queued.add(w, n, st);
 }
 void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
@@ -355,7 +356,7 @@ void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
 // call outside a capture starts. (And what is queued cannot be asked about there: the query would end the capture.)
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
     const unsigned long long capture = capture_of(stream());
-    if (capture) return capture == kCaptureUnknown || d->queued_captured;
+    if (capture) return capture == kCaptureUnknown || d->queued_captured.overlap(p, bytes, capture);
     return d->queued.overlap(p, bytes);
 }
 

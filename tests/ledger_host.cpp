@@ -59,3 +59,21 @@ int led_waits() { return (int)Script::waits.size(); }
 int led_ranges() { return g9::QueuedLedger<Script>::kRanges; }
 int led_lost() { return g9::QueuedLedger<Script>::kLost; }
 }
+
+namespace {
+g9::CaptureLedger *captured = nullptr;
+}
+extern "C" {
+void cap_new() {
+    delete captured;
+    captured = new g9::CaptureLedger;
+}
+void cap_call(uint64_t capture, int n, const uint64_t *lo, const uint64_t *bytes) {
+    std::vector<g9::QueuedWrite> w;
+    for (int i = 0; i < n; i++) w.push_back({(const void *)lo[i], (size_t)bytes[i]});
+    captured->add(w.data(), n, capture);
+}
+int cap_overlap(uint64_t lo, uint64_t bytes, uint64_t capture) { return captured->overlap((const void *)lo, bytes, capture); }
+int cap_captures() { return g9::CaptureLedger::kCaptures; }
+int cap_ranges() { return g9::CaptureLedger::kRanges; }
+}

@@ -907,3 +907,47 @@ def test_a_write_in_the_queue_does_not_end_a_capture(kv, gpu_lib, where):
             "table": np.zeros((1, 1), np.int32), "bounds": None}
     ref = kv_ref.attend(host, q.cpu().numpy(), [n])
     attend_close((O, torch.from_numpy(ref[1])), ref, D)
+
+
+def test_captured_writes_are_seen_by_captured_early_readers(kv, gpu_lib):
+    """append, the contiguous attention of the same memory and a product with the bounds, captured into one graph: at each replay
+    the readers wait for that replay's writes. Two graphs of the same calls, replayed in turn."""
+    D, heads, n = 64, 2, 4096
+    K = torch.zeros(1, heads, n, D, dtype=torch.float16, device="cuda")
+    V = torch.zeros_like(K)
+    bounds = torch.zeros(1, heads, 2, D, dtype=torch.float16, device="cuda")
+    q, O = torch.randn(1, 1, 8, D, device="cuda"), torch.zeros(1, 1, 8, D, device="cuda")
+    A, C = torch.randn(2, D, device="cuda").half(), torch.zeros(2, heads * 2, dtype=torch.float16, device="cuda")
+    k, v = (torch.zeros(1, n, heads, D, device="cuda") for _ in range(2))
+    cache, vis, zero = kv.PagedKV(K, V, ints([[0]]), bounds=bounds), ints([n]), ints([0])
+
+    def step():
+        cache.append(k, v, zero)
+        assert _dec(gpu_lib, K, V, q, O, n, vis) == 0, gpu_lib.error()
+        assert gpu_lib.set_stream(torch.cuda.current_stream().cuda_stream or 1) == 0
+        gpu_lib.set_nowait(1)
+        try:
+            assert gpu_lib.gemm(0, 0, 1, 2, heads * 2, D, 1.0, A.data_ptr(), D, bounds.data_ptr(), D, 0.0, C.data_ptr(), heads * 2) == 0
+        finally:
+            gpu_lib.set_nowait(0)
+            assert gpu_lib.set_stream(None) == 0
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            step()
+    for it in range(6):
+        kn, vn = (torch.randn(1, n, heads, D, device="cuda") + it for _ in range(2))
+        k.copy_(kn)
+        v.copy_(vn)
+        graphs[it % 2].replay()
+        torch.cuda.synchronize()
+        host = {"K": kn.half().cpu().numpy().transpose(0, 2, 1, 3), "V": vn.half().cpu().numpy().transpose(0, 2, 1, 3),
+                "table": np.zeros((1, 1), np.int32), "bounds": None}
+        ref = kv_ref.attend(host, q.cpu().numpy(), [n])
+        attend_close((O, torch.from_numpy(ref[1])), ref, D)
+        W = torch.stack([kn[0].half().amin(0), kn[0].half().amax(0)], 1).reshape(heads * 2, D).double()   # FP16 products, as above
+        want, mass = A.double() @ W.T, A.double().abs() @ W.abs().T
+        assert bool(((C.double() - want).abs() <= mass * D * 2.0 ** -24 + want.abs() * 2.0 ** -11 + 2.0 ** -24).all()), it

@@ -153,3 +153,59 @@ def test_random_calls_never_miss_an_open_write(led):
     for x in range(64):
         led.end(x, led.open(x))
     assert not led.overlap(0, 10 ** 9)
+
+
+# ------------------------------------------------------------------------------------------------ captured calls
+@pytest.fixture
+def cap(dll):
+    dll.cap_new()
+    dll.cap_call.argtypes = [ctypes.c_uint64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]
+    dll.cap_overlap.argtypes = [ctypes.c_uint64] * 3
+
+    class Cap:
+        captures, ranges = dll.cap_captures(), dll.cap_ranges()
+
+        @staticmethod
+        def call(capture, *ranges):
+            lo = (ctypes.c_uint64 * len(ranges))(*[r[0] for r in ranges])
+            n = (ctypes.c_uint64 * len(ranges))(*[r[1] for r in ranges])
+            dll.cap_call(capture, len(ranges), lo, n)
+
+        @staticmethod
+        def overlap(capture, lo, n=8):
+            return bool(dll.cap_overlap(lo, n, capture))
+    return Cap
+
+
+def test_a_captured_write_counts_in_its_capture_alone(cap):
+    cap.call(7, (1000, 100), (5000, 10), (0, 9), (8000, 0))
+    assert cap.overlap(7, 1092) and cap.overlap(7, 5000) and not cap.overlap(7, 1100) and not cap.overlap(7, 8000)
+    assert not cap.overlap(8, 1000)             # another graph's calls read early, whatever this one wrote
+    cap.call(8, (3000, 10))
+    assert cap.overlap(8, 3000) and not cap.overlap(8, 1000) and not cap.overlap(7, 3000) and cap.overlap(7, 1000)
+
+
+def test_more_captured_ranges_than_are_kept(cap):
+    rng = random.Random(3)
+    ranges = [(rng.randrange(1, 10 ** 6), rng.randrange(1, 100)) for _ in range(4 * cap.ranges)]
+    for i, r in enumerate(ranges):
+        cap.call(1, r)
+        assert all(cap.overlap(1, lo, n) for lo, n in ranges[:i + 1])
+    assert not cap.overlap(1, 2 * 10 ** 6)
+
+
+def test_more_captures_than_are_kept(cap):
+    for c in range(1, 3 * cap.captures):
+        assert not cap.overlap(c, 1000)         # a new capture starts open, however many there were
+        cap.call(c, (1000, 10))
+        assert cap.overlap(c, 1000) and not cap.overlap(c, 2000)
+    assert cap.overlap(1, 2000)                 # one that went: it may have written anything
+    cap.call(1, (1, 1))
+    assert cap.overlap(1, 2000) and not cap.overlap(3 * cap.captures - 1, 2000)
+
+
+def test_a_capture_in_use_stays_while_others_come(cap):
+    for c in range(2, 5 * cap.captures):
+        cap.call(1, (1000, 10))
+        cap.call(c, (2000, 10))
+    assert cap.overlap(1, 1000) and not cap.overlap(1, 2000)
