@@ -32,6 +32,7 @@ struct PagedArgs {
     int q2, o4;               // pairs of a query's elements are 8-byte aligned, fours of an output's 16-byte
     const int *vis, *sel;
     int nsel, sel_steps;      // chosen pages per unit, their steps
+    int *list;                // room for the entries that count: nsel for each unit, one more for each (CTA, unit)
     float qscale;             // scale · log2 e
     float *O, *lse;
     float *part;              // partial results, slot (CTA + unit)
@@ -76,8 +77,9 @@ struct PagedCfg {
 
 // Steps of one outer index: its slots [k0, k1) from the first visible one on, held to a multiple of a step; at least one,
 // so that every unit is finished by some CTA.
+template <bool SEL>
 __device__ __forceinline__ int outer_steps(const PagedArgs &a, int o, int &k0, int &k1) {
-    if (a.sel) {
+    if constexpr (SEL) {
         k0 = 0;
         k1 = a.nsel * a.c.page;
         return a.sel_steps;
@@ -86,6 +88,36 @@ __device__ __forceinline__ int outer_steps(const PagedArgs &a, int o, int &k0, i
     k1 = seen_slots(v, a.dvis, a.nq - 1, a.c.cap);
     k0 = a.window > 0 ? first_slot(seen_slots(v, a.dvis, 0, a.c.cap), a.window) / AKEYS * AKEYS : 0;
     return max(1, (k1 - k0 + AKEYS - 1) / AKEYS);
+}
+
+// A list of chosen pages: an entry counts if it names a place of the table above every earlier entry that does, so that each page
+// counts once, and in key order.
+__device__ __forceinline__ int named(int e, int mp) { return e >= 0 && e < mp ? e : -1; }
+// Whether the first n entries are as a selection leaves them, ascending places and what names none behind: then each that names a
+// place counts. By a whole CTA of NT threads; a barrier.
+template <int NT>
+__device__ __forceinline__ bool list_plain(const int *sel, int n, int mp) {
+    int odd = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i + 1 < n; i += NT) {
+        const int x = sel[i], y = sel[i + 1];
+        odd |= (int)(y >= 0) & (int)(y < mp) & (int)(x < 0 | x >= y);
+    }
+    return !__syncthreads_or(odd);
+}
+// Entry i + lane of any list, -1 where it does not count or i + lane >= n; by a whole warp.
+__device__ __forceinline__ int list_counts(const int *sel, int i, int n, int mp) {
+    const int lane = threadIdx.x & 31, e = i + lane < n ? named(sel[i + lane], mp) : -1;
+    int top = -1, x = e;
+    for (int k = lane; k < i; k += 32) top = max(top, named(sel[k], mp));
+    top = __reduce_max_sync(kAll, top);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kAll, x, o);
+        if (lane >= o) x = max(x, y);
+    }
+    const int before = __shfl_up_sync(kAll, x, 1);
+    return e > max(top, lane ? before : -1) ? e : -1;
 }
 
 // Elements d .. d + 3 of output row q from the sum L of its weights, the greatest score M and the sums x of PSCALE-fold weights.
@@ -110,12 +142,13 @@ __device__ __forceinline__ void paged_out(const PagedArgs &a, long long q, int d
     }
 }
 
-template <int DP, int NT, bool W>
+template <int DP, int NT, bool W, bool SEL>
 __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged_k(const __grid_constant__ PagedArgs a) {
     using C = PagedCfg<DP, NT, W>;
     constexpr int ROWS = C::ROWS, NST = C::NST, KT = DP / 16, PITCH = DP * 2;
     extern __shared__ __align__(128) uint8_t pa_sm[];
     __shared__ bool sh_last;
+    __shared__ const int *sh_sel[AW];   // the unit's list, for each warp (a register pair less in the loop)
     uint8_t *ring = pa_sm;
     uint4 *qf = reinterpret_cast<uint4 *>(pa_sm + C::RING);               // [kt][nt][lane]: hi, hi, lo, lo
     int *kidx_all = reinterpret_cast<int *>(pa_sm + C::RING + C::QF);     // [warp][stage][16]: slot, INT_MAX if not visible
@@ -129,7 +162,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
     // 4096 keys from 32.4 to 26.3 µs and one stream of 1000 keys from 14.1 to 9.6.
     const Run run = find_run(a.outer, a.inner, C::COST, AW, [&](int o) {
         int k0, k1;
-        return outer_steps(a, o, k0, k1);
+        return outer_steps<SEL>(a, o, k0, k1);
     });
     const int lo = run.lo, hi = run.hi, chunk = run.chunk, b = blockIdx.x;
     int outer = run.outer, pre = run.pre;
@@ -143,7 +176,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
 
     for (int at = lo; at < hi;) {
         int k0, k1;
-        const int n = outer_steps(a, outer, k0, k1), nv = n + C::COST, iu = (at - pre) / nv;
+        const int n = outer_steps<SEL>(a, outer, k0, k1), nv = n + C::COST, iu = (at - pre) / nv;
         if (iu >= a.inner) {
             pre += nv * a.inner;
             outer++;
@@ -156,10 +189,24 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
         // the unit's nsl slots, one a CTA, follow one another from slot0 on in key order
         const int slot = b + u, slot0 = rs0 / chunk + u, nsl = (rs0 + n - 1) / chunk + u - slot0 + 1;
         const int g = page_quot(a.by_tiles, iu), row0 = (iu - g * a.tiles) * ROWS;
-        const int s = a.sel ? page_quot(a.by_nq, outer) : outer, t0 = a.sel ? outer - s * a.nq : 0;
+        const int s = SEL ? page_quot(a.by_nq, outer) : outer, t0 = SEL ? outer - s * a.nq : 0;
         const int live_rows = min(ROWS, a.qn * a.G - row0);
         const int vs = a.vis[s];
-        const int *sel = a.sel ? a.sel + ((long long)outer * c.HKV + g) * a.nsel : nullptr;
+        if constexpr (SEL) {   // the entries that count, from this segment's first one to its last
+            const int *sel = a.sel + ((long long)outer * c.HKV + g) * a.nsel;
+            const int e0 = page_quot(c.div, sb * AKEYS), e1 = min(a.nsel, page_quot(c.div, se * AKEYS - 1) + 1);
+            if (!list_plain<AW * 32>(sel, e1, c.mp)) {   // a copy: segments that follow one another share an entry at most
+                int *own = a.list + (long long)u * a.nsel + slot;
+                for (int e = e0 + 32 * warp; e < e1; e += 32 * AW) {
+                    const int place = list_counts(sel, e, e1, c.mp);
+                    if (e + lane < e1) own[e + lane] = place;
+                }
+                __syncthreads();
+                sel = own;
+            }
+            if (lane == 0) sh_sel[warp] = sel;
+            __syncwarp();
+        }
         // lane r: row r of the unit -- the slots it sees, its query head's place among all (s, t, h)
         const int my_row = row0 + (lane < live_rows ? lane : 0), my_t = t0 + page_quot(a.by_g, my_row);
         const int my_h = g * a.G + my_row - (my_t - t0) * a.G;
@@ -179,13 +226,10 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
             const int j = k0 + (sb + warp + AW * i) * AKEYS + (lane & 15);
             int k = INT_MAX, place = -1, slot_in = 0;
             if (i < my) {
-                if (sel) {
+                if constexpr (SEL) {
                     const int e = page_quot(c.div, j);
                     slot_in = j - e * c.page;
-                    if (e < a.nsel) {
-                        place = sel[e];
-                        if (e > 0 && place <= sel[e - 1]) place = -1;
-                    }
+                    if (e < a.nsel) place = sh_sel[warp][e];
                     k = (int)((unsigned)place * c.page + slot_in);   // read only below mp places
                 } else if (j >= kmin && j < kmax) {
                     place = page_quot(c.div, j);
@@ -678,42 +722,56 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
         const int see = seen_slots(vs, a.dvis, t, c.cap);
         const int *sel = a.sel + (((long long)s * a.nq + t) * c.HKV + g) * a.nsel;
         const long long q = ((long long)s * a.nq + t) * a.H + g * a.G;
-        for (int j = threadIdx.x; j < n; j += 256) {
-            const int e = page_quot(c.div, j), place = sel[e];
-            if (place < 0 || (e > 0 && place <= sel[e - 1])) continue;
-            if (page_id(c.table, c.ts, s, place, c.mp, c.n_pages) < 0) continue;
+        auto add = [&](int j, int e, int place) {   // no other thread has this slot: a page counts once
+            if (page_id(c.table, c.ts, s, place, c.mp, c.n_pages) < 0) return;
             const int k = place * c.page + j - e * c.page;
-            if (k >= see) continue;
+            if (k >= see) return;
             float sum = 0.0f;
             for (int h = 0; h < a.G; h++) sum += weight(__ldcg(a.score + (q + h) * a.score_row + j), __ldcg(a.lse2 + q + h));
             row[k] += sum;
+        };
+        if (list_plain<256>(sel, a.nsel, c.mp)) {
+            for (int j = threadIdx.x; j < n; j += 256) {
+                const int e = page_quot(c.div, j);
+                add(j, e, sel[e]);
+            }
+        } else {   // a warp per 32 entries, page by page
+            for (int e0 = threadIdx.x & ~31; e0 < a.nsel; e0 += 256) {
+                const int mine = list_counts(sel, e0, a.nsel, c.mp);
+                for (int x = 0; x < min(32, a.nsel - e0); x++) {
+                    const int place = __shfl_sync(kAll, mine, x);
+                    for (int i = threadIdx.x & 31; place >= 0 && i < c.page; i += 32) add((e0 + x) * c.page + i, e0 + x, place);
+                }
+            }
         }
         __syncthreads();   // the next token may choose the same pages
     }
 }
 
-template <int DP, int NT, bool W>
+template <int DP, int NT, bool W, bool SEL>
 int paged_one(const PagedArgs &a, const KvCall &call, bool plan, int *ctas) {
     using C = PagedCfg<DP, NT, W>;
     static bool attr[kMaxDevices] = {};
     static int occ[kMaxDevices] = {};
     if (plan) {   // the resident CTAs of the device
-        G9_CU(smem_limit_once(attn_paged_k<DP, NT, W>, C::SMEM, attr));
+        G9_CU(smem_limit_once(attn_paged_k<DP, NT, W, SEL>, C::SMEM, attr));
         if (!occ[call.d->dev])
-            G9_CU(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ[call.d->dev], attn_paged_k<DP, NT, W>, AW * 32, C::SMEM));
+            G9_CU(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ[call.d->dev], attn_paged_k<DP, NT, W, SEL>, AW * 32, C::SMEM));
         *ctas = std::max(occ[call.d->dev], 1) * call.d->sm_count;
         return 0;
     }
     // Not launched early: the CTAs fill an SM's registers, and one that finds a CTA of the kernel before among them leaves a hole
     // too small for the last one, which then waits for a whole run (8 streams of 4193 to 8193 keys behind an append 53 µs
     // against 42, the same with weights 62 against 48). Without a wave to fill, starting early saves 0.5 µs.
-    attn_paged_k<DP, NT, W><<<(unsigned)*ctas, AW * 32, C::SMEM, call.st>>>(a);
+    attn_paged_k<DP, NT, W, SEL><<<(unsigned)*ctas, AW * 32, C::SMEM, call.st>>>(a);
     return launched("attn_paged");
 }
 
+// Chosen pages have kernels of their own: what they take of the registers slows the others (D 128, two row tiles, weights 207 -> 224 µs).
 template <int DP, int NT>
 int paged_either(const PagedArgs &a, const KvCall &call, bool weights, bool plan, int *ctas) {
-    return weights ? paged_one<DP, NT, true>(a, call, plan, ctas) : paged_one<DP, NT, false>(a, call, plan, ctas);
+    if (a.sel) return weights ? paged_one<DP, NT, true, true>(a, call, plan, ctas) : paged_one<DP, NT, false, true>(a, call, plan, ctas);
+    return weights ? paged_one<DP, NT, true, false>(a, call, plan, ctas) : paged_one<DP, NT, false, false>(a, call, plan, ctas);
 }
 
 // The kernel of a padded head size and a number of 8-row tiles; plan: only its resident CTAs.
@@ -806,9 +864,12 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     a.score_row = ((sel ? (long long)a.nsel * c->page : a.c.cap) + 3) / 4 * 4;   // rows of whole float4
     const size_t lse2 = acc ? up256((size_t)heads * 4) : 0;
     if (acc && (__int128)heads * a.score_row * 4 > kKvMost) return kv_too_large(who);
-    const size_t score = acc ? (size_t)heads * a.score_row * 4 : 0;
+    const size_t score = acc ? up256((size_t)heads * a.score_row * 4) : 0;
+    if ((__int128)units * a.nsel * 4 > kKvMost) return kv_too_large(who);
+    const size_t list = sel ? up256(((size_t)units * a.nsel + ctas + units) * 4) : 0;
     void *buf = nullptr;
-    G9_TRY(kv_workspace(ws, call, who, part + lse2 + score, (size_t)units, &buf, &a.cnt));
+    G9_TRY(kv_workspace(ws, call, who, part + lse2 + score + list, (size_t)units, &buf, &a.cnt));
+    if (sel) a.list = (int *)((char *)buf + part + lse2 + score);
     a.part = (float *)buf;
     if (c->n_pages == 0) a.c.K = a.c.V = (__half *)buf;   // named by copies of no bytes
     if (acc) {

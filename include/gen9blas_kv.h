@@ -67,7 +67,8 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
  * What lies in slots that a token does not see (NaN, infinities) does not enter its result; a seen key or value that is
  * not finite enters as the formula has it (NaN, as a rule; a score of -inf has no weight), for the heads that see it only.
  * sel (NULL or int [s][t][HKV][nsel]): only the slots of the listed pages, given by their place k / page in the stream,
- * ascending; an entry that is negative, not below mp or not above the one before it is skipped. Not with window > 0.
+ * ascending; an entry that is negative or not below mp is skipped, and so is one that is not above every earlier entry that
+ * was not (a page counts once). Not with window > 0.
  * acc (NULL or as in kv_append): acc[k] += the softmax weights that slot k got from all tokens and query heads of the
  * key-value head (sums in a fixed order: the same bits each time). Meant for few tokens (decoding, drafts); any nq >= 1
  * works. */

@@ -24,11 +24,11 @@ def visible_slots(cache, s, vis, step, t, window=0, sel=None):
     if sel is None:
         ks = range(max(0, n - window) if window else 0, n)
     else:
-        ks, before = [], -1
-        for i, e in enumerate(sel):
-            if e >= 0 and e < cache["table"].shape[1] and (i == 0 or e > before):
+        ks, top = [], -1
+        for e in sel:
+            if top < e < cache["table"].shape[1]:       # above every earlier one that counts: each page once
                 ks += [k for k in range(e * page, (e + 1) * page) if k < n]
-            before = e
+                top = e
     return [k for k in ks if place_of(cache, s, k) is not None]
 
 

@@ -168,6 +168,17 @@ def test_reference_attention_of_one_slot_returns_its_value():
     assert kv_ref.visible_slots(cache, 0, 8, 1, 0, sel=[0, 0, -1]) == [0, 1, 2, 3]
 
 
+def test_reference_lists_count_a_page_once():
+    cache = {"K": np.zeros((9, 1, 2, 8), np.float16), "table": np.arange(8, dtype=np.int32)[None]}
+
+    def places(sel):
+        ks = kv_ref.visible_slots(cache, 0, 16, 1, 0, sel=sel)
+        assert ks == sorted(set(ks)) and len(ks) % 2 == 0
+        return [k // 2 for k in ks[::2]]
+    assert places([3, -1, 3]) == [3] and places([5, 2, 5]) == [5] and places([5, 3, 4, 5, 6]) == [5, 6]
+    assert places([8, 3, 2 ** 31 - 1, 4, -2 ** 31, 4, 7]) == [3, 4, 7] and places([-1, 0, 0, 1]) == [0, 1] and places([]) == []
+
+
 def test_reference_eviction_keeps_the_heaviest():
     cache = {"K": np.arange(24, dtype=np.float16).reshape(3, 1, 8, 1).repeat(8, 3), "table": np.array([[2, 0]], np.int32)}
     cache["V"] = -cache["K"]

@@ -951,3 +951,43 @@ def test_captured_writes_are_seen_by_captured_early_readers(kv, gpu_lib):
         W = torch.stack([kn[0].half().amin(0), kn[0].half().amax(0)], 1).reshape(heads * 2, D).double()   # FP16 products, as above
         want, mass = A.double() @ W.T, A.double().abs() @ W.abs().T
         assert bool(((C.double() - want).abs() <= mass * D * 2.0 ** -24 + want.abs() * 2.0 ** -11 + 2.0 ** -24).all()), it
+
+
+def _unordered(rng, mp, m, kind):
+    """Lists of m entries whose pages come twice, out of order or between entries that name no page."""
+    if kind == "short":
+        return [[3, -1, 3], [5, 2, 5], [5, 3, 4, 5], [mp, 3, 2 ** 31 - 1, 4], [-1, -2 ** 31, 2, 2], [0, 0, 1, 0, 1, 2], [7, 6, 5, 4, 3, 8]]
+    x = np.sort(rng.integers(0, mp, m)).astype(np.int64)
+    back = rng.integers(1, m, m // 8)
+    x[back] = x[rng.integers(0, back)]                                  # an earlier one again
+    x[rng.integers(0, m, m // 8)] = rng.choice([-1, mp, 2 ** 31 - 1, -2 ** 31], m // 8)
+    return x
+
+
+@pytest.mark.parametrize("page,group,D,nq,m,kind", [(16, 4, 64, 2, 6, "short"), (1, 2, 64, 2, 6, "short"), (5, 12, 128, 1, 6, "short"),
+                                                    (64, 4, 256, 1, 6, "short"), (16, 4, 128, 3, 100, "long"), (3, 9, 64, 1, 200, "long"),
+                                                    (1, 1, 64, 1, 700, "long"), (128, 4, 64, 2, 40, "long")])
+def test_lists_that_name_a_page_twice(kv, page, group, D, nq, m, kind):
+    """A page counts once wherever its other mentions stand; its weights are added once, and the same bits each time."""
+    rng = np.random.default_rng(page + m)
+    heads, mp = 2, max(10, m)
+    host, K, V, table, _ = make(rng, [mp * page - nq, mp * page - nq - 3], page, heads, D, extra=nq)
+    assert table.shape[1] == mp
+    sel = np.full((2, nq, heads, m), -1, np.int32)
+    flat = sel.reshape(-1, m)
+    for i in range(len(flat)):
+        x = _unordered(rng, mp, m, kind)
+        x = x[(i + page) % len(x)] if kind == "short" else x
+        flat[i, :len(x)] = x
+    vis = np.array([mp * page - nq, mp * page - nq - 3])
+    q = rng.standard_normal((2, nq, heads * group, D)).astype(np.float32)
+    ref = kv_ref.attend(host, q, vis, sel=sel)
+    accs = []
+    for _ in range(3):
+        acc = torch.zeros(2, heads, mp * page, device="cuda")
+        got = kv.PagedKV(K, V, table).attend(torch.from_numpy(q).cuda(), ints(vis), sel=torch.from_numpy(sel).cuda(), acc=acc, lse=True)
+        attend_close(got, ref, D)
+        accs.append(acc)
+    assert torch.equal(accs[0], accs[1]) and torch.equal(accs[0], accs[2])
+    e = ref[3].max() * (2.0 ** -21 + (D + 4) * 2.0 ** -24)
+    assert np.all(np.abs(accs[0].cpu().numpy() - ref[2]) <= (4 * e + 2.0 ** -19 + nq * group * 2.0 ** -23) * ref[2] + 1e-30)
