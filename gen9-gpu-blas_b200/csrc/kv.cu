@@ -94,22 +94,40 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     return 0;
 }
 
+// Whether rows of `row` elements, n[i] of them `st[i]` apart in each of the dimensions, share no element: the strides nest, each
+// at least what the rows of the dimensions with smaller ones span together.
+static bool rows_nest(int dims, const long long *n, const int64_t *st, long long row) {
+    bool done[3] = {};
+    __int128 span = row;
+    for (int k = 0; k < dims; k++) {
+        int at = -1;
+        for (int i = 0; i < dims; i++)
+            if (!done[i] && (at < 0 || st[i] < st[at])) at = i;
+        done[at] = true;
+        if (n[at] <= 1) continue;
+        if (st[at] < span) return false;
+        span += (__int128)(n[at] - 1) * st[at];
+    }
+    return true;
+}
+
 int kv_marks_apart(const gen9blas_kv_cache *c, bool used, int64_t ms, int64_t mh, const char *who) {
     if (!c || !used) return 0;
-    const long long cap = (long long)c->mp * c->page;
-    if ((c->ns > 1 && ms < cap) || (c->HKV > 1 && mh < cap))
+    const long long cap = (long long)c->mp * c->page, n[2] = {c->ns, c->HKV};
+    const int64_t st[2] = {ms, mh};
+    if (!rows_nest(2, n, st, cap))
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: rows of acc or pos overlap: strides %lld and %lld, %lld slots", who,
                     (long long)ms, (long long)mh, cap);
     return 0;
 }
 
 int kv_rows_apart(const gen9blas_kv_cache *c, const char *who) {
-    if (!c) return 0;
-    const int64_t st[6] = {c->kp, c->kk, c->kh, c->vp, c->vk, c->vh};
-    const int n[3] = {c->n_pages, c->page, c->HKV};
-    for (int i = 0; i < 6; i++)
-        if (n[i % 3] > 1 && c->n_pages > 0 && st[i] < c->D)
-            return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: rows of K or V overlap: a stride of %lld elements", who, (long long)st[i]);
+    if (!c || c->n_pages <= 0) return 0;
+    const long long n[3] = {c->n_pages, c->page, c->HKV};
+    const int64_t ks[3] = {c->kp, c->kk, c->kh}, vs[3] = {c->vp, c->vk, c->vh};
+    if (!rows_nest(3, n, ks, c->D) || !rows_nest(3, n, vs, c->D))
+        return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: rows of K or V overlap: strides %lld, %lld, %lld and %lld, %lld, %lld elements", who,
+                    (long long)c->kp, (long long)c->kk, (long long)c->kh, (long long)c->vp, (long long)c->vk, (long long)c->vh);
     return 0;
 }
 

@@ -46,7 +46,8 @@ struct KvCall {
 // Starts a call: checks the cache's description and the shape (H = HKV for calls without query heads), then the device
 // and the stream. Returns 0, GEN9BLAS_DECLINED or an error; a cache without streams or slots returns 0 with ns = 0.
 int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev *dev, KvCall *call);
-// What a call writes must not overlap itself: rows of acc and pos (used: either given), and of the pool. 0 or an error.
+// What a call writes must not overlap itself: rows of acc and pos (used: either given), and of the pool. Strides have to nest:
+// each at least what the dimensions with smaller ones span. 0 or an error.
 int kv_marks_apart(const gen9blas_kv_cache *c, bool used, int64_t ms, int64_t mh, const char *who);
 int kv_rows_apart(const gen9blas_kv_cache *c, const char *who);
 // p is device or managed memory of the current device.

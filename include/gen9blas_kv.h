@@ -12,7 +12,8 @@
  * Memory: every operand is device or managed memory of the current device (GEN9BLAS_ERR_INVALID_ARG otherwise); lengths,
  * counts and tables are read on the device, so that a captured call follows them at each replay. Calls are queued;
  * sync = 1 waits (not while the stream is being captured: GEN9BLAS_ERR_INVALID_ARG). Operands of one call that are
- * written overlap no other operand, unless said.
+ * written overlap no other operand, unless said, nor themselves: the strides of K, V, acc and pos nest where a call writes
+ * them, each at least what the dimensions with smaller ones span (GEN9BLAS_ERR_INVALID_ARG otherwise).
  *
  * Shapes: D a multiple of 8 up to 256, H a multiple of HKV (gen9blas_kv_supported; other shapes return
  * GEN9BLAS_DECLINED, nothing written); K, V and bounds 16-byte aligned, their strides multiples of 8 elements. */

@@ -146,6 +146,33 @@ def test_what_a_call_writes_must_not_overlap_itself(kv):
         assert attn(c, 4, 1, q, 256, 64, 256, q, 1, 0, None, 0, 1.0, q, None, q, ms, mh, None, 0) == -3 and b"overlap" in kv._fn["error"]()
 
 
+def test_strides_that_are_long_enough_each_but_overlap_together(kv):
+    """Rows of one dimension lie apart, but some of two dimensions are the same; layouts whose strides nest are not refused."""
+    buf = ctypes.create_string_buffer(40000)
+    c, q = _cache(kv, buf), ctypes.addressof(buf)
+    append, evict, attn = kv._fn["kv_append"], kv._fn["kv_evict"], kv._fn["attn_paged"]
+    tokens = (1, q, 64, 64, 64, q, 64, 64, 64, q, None)
+
+    def overlap(status):
+        return status == -3 and b"overlap" in kv._fn["error"]()
+    for over in (dict(kp=64), dict(kk=64, kh=64), dict(vp=512), dict(vh=64), dict(kp=1016), dict(vp=64, vk=256, vh=128)):
+        bad = _cache(kv, buf, **over)
+        assert overlap(append(bad, *tokens, None, None, 0, 0, None, 0, None)), over
+        assert overlap(evict(bad, q, 8, 0, 0, q, None, 64, 32, q, None, 0)), over
+    for over in (dict(kk=128, kh=64), dict(kp=64, kk=256, kh=2048), dict(vk=72, vh=576, vp=1152, v_bytes=16384), dict(kp=0, n_pages=1)):
+        assert not overlap(append(_cache(kv, buf, **{**dict(k_bytes=16384, v_bytes=16384), **over}), *tokens, None, None, 0, 0, None, 0,
+                                  None)), over
+    for ms, mh in ((32, 32), (63, 32), (32, 63), (48, 40)):
+        assert overlap(append(c, *tokens, q, None, ms, mh, None, 0, None))
+        assert overlap(append(c, *tokens, None, q, ms, mh, None, 0, None))
+        assert overlap(evict(c, q, 8, 0, 0, q, None, ms, mh, q, None, 0))
+        assert overlap(attn(c, 4, 1, q, 256, 64, 256, q, 1, 0, None, 0, 1.0, q, None, q, ms, mh, None, 0))
+    for ms, mh in ((64, 32), (32, 64), (100, 40), (33, 70)):
+        assert not overlap(append(c, *tokens, q, None, ms, mh, None, 0, None))
+    one = _cache(kv, buf, ns=1)
+    assert not overlap(append(one, *tokens, q, None, 0, 32, None, 0, None)) and overlap(append(one, *tokens, q, None, 0, 31, None, 0, None))
+
+
 def test_python_face_checks_types(kv):
     torch = pytest.importorskip("torch")
     with pytest.raises(ValueError, match="float16"):
