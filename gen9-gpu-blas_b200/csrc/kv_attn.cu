@@ -120,6 +120,16 @@ __device__ __forceinline__ int list_counts(const int *sel, int i, int n, int mp)
     return e > max(top, lane ? before : -1) ? e : -1;
 }
 
+// The score, in base 2, of query row q (its place among all (s, t, h)) and a key row in shared memory, whose 16-byte pieces are
+// exchanged by `swap`: element by element.
+__device__ __noinline__ float plain_score(const PagedArgs &a, int q, const uint8_t *key, int swap) {
+    const int h = q % a.H, st = q / a.H, t = st % a.nq, s = st / a.nq;
+    const float *qp = a.Q + s * a.qs + t * a.qt + h * a.qh;
+    float x = 0.0f;
+    for (int d = 0; d < a.c.D; d++) x = fmaf(qp[d], __half2float(reinterpret_cast<const __half *>(key)[((d >> 3) ^ swap) * 8 + (d & 7)]), x);
+    return x * a.qscale;
+}
+
 // Elements d .. d + 3 of output row q from the sum L of its weights, the greatest score M and the sums x of PSCALE-fold weights.
 __device__ __forceinline__ void paged_out(const PagedArgs &a, long long q, int d, float M, float L, float4 x) {
     const bool none = L == 0.0f;   // the row sees nothing
@@ -432,17 +442,6 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                         if (kc >= see[nt][j] || kc < from[nt][j]) sc[nt][2 + j] = -INFINITY;
                     }
             }
-            if constexpr (W) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
-                        float *sr = NT == 1 ? srow[j] : a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
-                        if (r < live_rows && at0 < k1) sr[at0] = sc[nt][j] * inv[nt][j];
-                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = sc[nt][2 + j] * inv[nt][j];
-                    }
-            }
             // Weights are 2^(score - m) with m a greatest score of before: it is raised, and the sums scaled down, only when
             // a score passes it by more than 8, so that most steps need no maximum over the lanes.
             float p[NT][2][2];   // of (key gq + 8e, row 8nt + 2tq + j), at most 2^8
@@ -453,9 +452,21 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                 for (int j = 0; j < 2; j++) {
                     p[nt][0][j] = fmaf(sc[nt][j], inv[nt][j], -m[nt][j]);
                     p[nt][1][j] = fmaf(sc[nt][2 + j], inv[nt][j], -m[nt][j]);
-                    over = over || fmaxf(p[nt][0][j], p[nt][1][j]) > 8.0f;
+                    over = over || !(p[nt][0][j] <= 8.0f) || !(p[nt][1][j] <= 8.0f);   // also NaN
                 }
             if (__any_sync(kAll, over)) {
+                // An infinite element of a key meets the query's two parts separately, and infinity times a part of zero is NaN:
+                // what came out as NaN is computed again by the formula, for a score of -inf has no weight.
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int r = 8 * nt + 2 * tq + j, q = __shfl_sync(kAll, my_q, r);
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            if (sc[nt][2 * e + j] != sc[nt][2 * e + j] && r < live_rows)
+                                sc[nt][2 * e + j] = plain_score(a, q, wring + stage * C::STAGE + (gq + 8 * e) * PITCH, gq) / inv[nt][j];
+                    }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -474,6 +485,17 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                             o[dt][nt][j] *= alpha;
                             o[dt][nt][2 + j] *= alpha;
                         }
+                    }
+            }
+            if constexpr (W) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
+                        float *sr = NT == 1 ? srow[j] : a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
+                        if (r < live_rows && at0 < k1) sr[at0] = sc[nt][j] * inv[nt][j];
+                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = sc[nt][2 + j] * inv[nt][j];
                     }
             }
 #pragma unroll

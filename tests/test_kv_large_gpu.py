@@ -207,3 +207,63 @@ def test_select_long_rows(kv, n, m, ns, heads, group, kind):
     got = kv.PagedKV(K, K, ints(table), bounds=torch.from_numpy(bounds).cuda()).select(torch.from_numpy(q).cuda(), ints([n] * ns), m,
                                                                                        first=2, last=3)
     assert np.array_equal(got.cpu().numpy(), select_ref(bounds, table, q, n, m, 2, 3))
+
+
+def by_slots(host):
+    """The same cache in pages of one slot."""
+    K, page = host["K"], host["K"].shape[2]
+    out = {x: host[x].transpose(0, 2, 1, 3).reshape(-1, K.shape[1], 1, K.shape[3]) for x in "KV"}
+    t = host["table"].astype(np.int64)
+    out["table"] = np.where(t[:, :, None] >= 0, t[:, :, None] * page + np.arange(page), -1).reshape(len(t), -1).astype(np.int32)
+    return out
+
+
+@pytest.mark.parametrize("group,D,nq,room", [(4, 128, 1, 0), (3, 80, 4, 0), (4, 256, 2, 0), (4, 64, 5, 120000), (12, 128, 1, 30000), (5, 256, 3, 30000)])
+@pytest.mark.parametrize("chosen", [False, True])
+def test_scores_of_minus_infinity_have_no_weight(kv, group, D, nq, room, chosen):
+    """Keys with elements of -inf (and +inf against a negative query): their scores are -inf, whatever the parts of the query that
+    meet them, and their slots are as if they were not seen. Query elements there from normal ones to ones that fall below all
+    FP16 parts; a row all of whose scores are -inf gives 0 and -inf."""
+    rng = np.random.default_rng(group + D)
+    lens, heads, page = [300, 40, 16], 2, 16
+    host, K, V, table, _ = make(rng, [n + nq - 1 for n in lens], page, heads, D)
+    if room and not chosen:
+        table = wide_table(host, table, room)
+        assert two_tiles(3, heads, group * nq, room, D)
+    q = rng.standard_normal((3, nq, heads * group, D)).astype(np.float32)
+    q[..., 5] = np.abs(q[..., 5]) + 0.1
+    q[..., 6] = -2.0 ** -10                               # exact in one part: the second part is zero
+    q[..., 7] = 1e-12
+    ref = by_slots(host)
+    gone = [sorted(rng.permutation(n)[:n // 3]) for n in lens[:2]] + [range(lens[2])]
+    for s, ks in enumerate(gone):
+        for k in ks:
+            p, i = host["table"][s, k // page], k % page
+            d = rng.choice([5, 6, 7])
+            K[int(p), :, i, int(d)] = float("inf") if d == 6 else -float("inf")
+            if k % 3 == 0:
+                K[int(p), :, i, 5] = -float("inf")
+            ref["table"][s, k] = -1
+    for s, n in enumerate(lens):
+        ref["table"][s, n:] = -1
+    sel = None
+    rsel = None
+    if chosen:
+        mp = host["table"].shape[1]
+        sel = np.full((3, nq, heads, 9), -1, np.int32)
+        for i in np.ndindex(3, nq, heads):
+            m = rng.integers(1, 10)
+            sel[i][:m] = np.sort(rng.permutation(mp)[:m])
+        rsel = np.where(sel[..., None] >= 0, sel[..., None] * page + np.arange(page), -1).reshape(3, nq, heads, -1)
+    vis = [lens[0], lens[1], lens[2]]
+    want = kv_ref.attend(ref, q, vis, step=0, sel=rsel)
+    acc = torch.full((3, heads, table.shape[1] * page), 0.25, device="cuda")
+    got = kv.PagedKV(K, V, table).attend(torch.from_numpy(q).cuda(), ints(vis), step=0, acc=acc, lse=True,
+                                         sel=None if sel is None else torch.from_numpy(sel).cuda())
+    attend_close(got, want, D)
+    assert np.isneginf(want[1][2]).all() and not got[0][2].any()
+    a, W = acc.cpu().numpy(), np.zeros(acc.shape)
+    W[:, :, :want[2].shape[2]] = want[2]
+    e = want[3].max() * (2.0 ** -21 + (D + 4) * 2.0 ** -24)
+    assert np.all(np.abs(a - (0.25 + W)) <= (4 * e + 2.0 ** -19 + nq * group * 2.0 ** -23) * W + 2.0 ** -23 * (0.25 + W))
+    assert np.all(a[W == 0] == 0.25)
