@@ -8,6 +8,7 @@
 #include "sm100.cuh"
 #include <cooperative_groups.h>
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <new>
@@ -966,7 +967,8 @@ __global__ void __launch_bounds__(CT) kv_choose_k(const __grid_constant__ Select
     const bool full = at == kAll;   // enough pages that are always taken: the lowest of them
     const float tau = __uint_as_float(at & 0x80000000u ? at & 0x7fffffffu : ~at);
     const bool know = E < INFINITY && at != 0u && !full;   // otherwise every page that is not always taken is ranked by hand
-    const float above = know ? tau + 2.0f * E : 3.4e38f, below = know ? tau - 2.0f * E : -INFINITY;
+    // finite, so that pages taken by hand (infinity, see decide) lie above it; scores are finite where E is
+    const float above = know ? fminf(tau + 2.0f * E, FLT_MAX) : FLT_MAX, below = know ? tau - 2.0f * E : -INFINITY;
     // 1: taken for sure, 0: not, -1: between
     auto side = [&](int i, float y) { return always(i) || (know && y > above) ? 1 : !know || y >= below ? -1 : 0; };
     auto decide = [&](int i, bool take) {

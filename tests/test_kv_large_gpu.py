@@ -267,3 +267,23 @@ def test_scores_of_minus_infinity_have_no_weight(kv, group, D, nq, room, chosen)
     e = want[3].max() * (2.0 ** -21 + (D + 4) * 2.0 ** -24)
     assert np.all(np.abs(a - (0.25 + W)) <= (4 * e + 2.0 ** -19 + nq * group * 2.0 ** -23) * W + 2.0 ** -23 * (0.25 + W))
     assert np.all(a[W == 0] == 0.25)
+
+
+@pytest.mark.parametrize("q,hi", [(float(np.finfo(np.float32).max), 1.0), (-float(np.finfo(np.float32).max), -1.0), (3e38, 1.0)])
+@pytest.mark.parametrize("n,m", [(9000, 8500), (9000, 9), (20000, 19000), (600, 550)])
+def test_select_long_rows_with_scores_at_the_end_of_float32(kv, q, hi, n, m):
+    """Equal scores near FP32's largest number, where the border plus the error bound of the scores passes it: every place of the
+    list is written, the lowest ones. Some pages lie below by a step of FP16."""
+    D = 8
+    K = torch.zeros(n, 1, 1, D, dtype=torch.float16, device="cuda")
+    bounds = np.zeros((n, 1, 2, D), np.float16)
+    bounds[:, 0, :, 0] = hi
+    low = np.arange(7, n, 100)
+    bounds[low, 0, :, 0] = hi * (1 - 2.0 ** -11)
+    qs = np.zeros((1, 1, 1, D), np.float32)
+    qs[..., 0] = q
+    out = torch.full((1, 1, 1, m), -7, dtype=torch.int32, device="cuda")
+    table = np.arange(n, dtype=np.int32)[None]
+    got = kv.PagedKV(K, K, ints(table), bounds=torch.from_numpy(bounds).cuda()).select(torch.from_numpy(qs).cuda(), ints([n]), m, first=0,
+                                                                                       last=0, out=out)
+    assert np.array_equal(got.cpu().numpy(), select_ref(bounds, table, qs, n, m, 0, 0))
