@@ -713,6 +713,11 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
         const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
         if (k >= seen_slots(vs, a.dvis, a.nq - 1, c.cap) || k + 3 < first_slot(seen_slots(vs, a.dvis, 0, c.cap), a.window)) return;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        unsigned got = 0;   // which of the four some row sees: the others stay as they are
+        auto add = [&](float &to, int i, float score, float l2) {
+            to += weight(score, l2);
+            got |= (unsigned)(score != -INFINITY) << i;
+        };
         for (int t = 0; t < a.nq; t++) {
             const int see = seen_slots(vs, a.dvis, t, c.cap), from = first_slot(see, a.window);
             if (k >= see || k + 3 < from) continue;
@@ -722,20 +727,20 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
                 const float l2 = __ldcg(a.lse2 + q + h);
                 const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.score + (q + h) * a.score_row + k));
                 // scores outside [from, see) were not written for this token where its whole step lies outside
-                if (k >= from) sum.x += weight(x.x, l2);
-                if (k + 1 >= from && k + 1 < see) sum.y += weight(x.y, l2);
-                if (k + 2 >= from && k + 2 < see) sum.z += weight(x.z, l2);
-                if (k + 3 >= from && k + 3 < see) sum.w += weight(x.w, l2);
+                if (k >= from) add(sum.x, 0, x.x, l2);
+                if (k + 1 >= from && k + 1 < see) add(sum.y, 1, x.y, l2);
+                if (k + 2 >= from && k + 2 < see) add(sum.z, 2, x.z, l2);
+                if (k + 3 >= from && k + 3 < see) add(sum.w, 3, x.w, l2);
             }
         }
-        if (v4 && k + 3 < c.cap) {
+        if (v4 && got == 15u) {
             float4 w = *reinterpret_cast<const float4 *>(row + k);
             *reinterpret_cast<float4 *>(row + k) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
         } else {
-            row[k] += sum.x;
-            if (k + 1 < c.cap) row[k + 1] += sum.y;
-            if (k + 2 < c.cap) row[k + 2] += sum.z;
-            if (k + 3 < c.cap) row[k + 3] += sum.w;
+            if (got & 1u) row[k] += sum.x;
+            if (got & 2u) row[k + 1] += sum.y;
+            if (got & 4u) row[k + 2] += sum.z;
+            if (got & 8u) row[k + 3] += sum.w;
         }
         return;
     }

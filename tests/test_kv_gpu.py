@@ -991,3 +991,17 @@ def test_lists_that_name_a_page_twice(kv, page, group, D, nq, m, kind):
     assert torch.equal(accs[0], accs[1]) and torch.equal(accs[0], accs[2])
     e = ref[3].max() * (2.0 ** -21 + (D + 4) * 2.0 ** -24)
     assert np.all(np.abs(accs[0].cpu().numpy() - ref[2]) <= (4 * e + 2.0 ** -19 + nq * group * 2.0 ** -23) * ref[2] + 1e-30)
+
+
+@pytest.mark.parametrize("nq,step,window", [(1, 1, 0), (3, 1, 5), (2, 20, 7)])
+def test_weights_leave_slots_that_no_token_sees_as_they_were(kv, nq, step, window):
+    """Bit for bit, a negative zero among them: behind the last slot seen, before and between the windows, without a page."""
+    rng = np.random.default_rng(50)
+    host, K, V, table, _ = make(rng, [64, 50], 8, 2, 64, holes=[(0, 1), (1, 4)])
+    q = rng.standard_normal((2, nq, 8, 64)).astype(np.float32)
+    acc = torch.full((2, 2, 64), -0.0, device="cuda")
+    vis = [13, 34]
+    kv.PagedKV(K, V, table).attend(torch.from_numpy(q).cuda(), ints(vis), step=step, window=window, acc=acc)
+    W = kv_ref.attend(host, q, vis, step=step, window=window)[2]
+    bits = acc.cpu().numpy().view(np.int32)
+    assert np.all(bits[W == 0] == -2 ** 31) and np.all(acc.cpu().numpy()[W > 0] > 0)
