@@ -12,7 +12,8 @@ K and V: float16 [pages, kv heads, page size, head size], unit stride in the las
 elements (so both [page][head][slot] and [page][slot][head] pools serve, the latter as a permuted view). table: int32
 [streams, pages per stream], -1 where a stream has no page. q, k, v: float32 [streams, tokens, heads, head size], unit
 stride in the last dimension. Everything lies on one GPU; calls run on torch's current stream and do not wait. They are for
-serving: results carry no gradient. Shape and type errors raise ValueError, library errors RuntimeError with gen9blas_error().
+serving: results carry no gradient, and a tensor that requires one is refused unless gradients are off (torch.no_grad()). Shape and
+type errors raise ValueError, library errors RuntimeError with gen9blas_error().
 
 One cache object is used by one thread at a time, as the library is. A captured call (torch.cuda.graph) needs a workspace
 of its own: pass `workspace=g9kv.Workspace()` to the constructor and make one call of each shape before the capture. The
@@ -56,6 +57,7 @@ if _raw_stream is None:
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 _capturing = torch.cuda.is_current_stream_capturing
+_grad_enabled = torch.is_grad_enabled
 _f32, _i32 = torch.float32, torch.int32
 _END = 2 ** 31   # of the library's counts; ctypes would cut larger ones short without a word
 
@@ -118,6 +120,7 @@ class PagedKV:
         self.device, self.streams, self.slots = K.device, table.shape[0], table.shape[1] * page
         self.heads, self.page, self.dim = heads, page, dim
         self._index = K.device.index
+        self._leaf = K.requires_grad or V.requires_grad
         self._per_stream = torch.Size([self.streams])
         self._logs = torch.empty(0, device=K.device)
 
@@ -133,6 +136,8 @@ class PagedKV:
 
     def _run(self, what, fn, *args):
         """One library call on torch's current stream of this cache's device."""
+        if self._leaf and _grad_enabled():
+            raise ValueError("K or V requires a gradient, which the paged cache does not give: call it under torch.no_grad()")
         self._c.stream = _raw_stream(self._index) or _LEGACY
         status = fn(self._ref, *args)
         if status:
@@ -156,6 +161,8 @@ class PagedKV:
                 and (heads is None or n[2] == heads) and st[3] == 1):
             raise ValueError(f"{name}: float32 [{self.streams}, tokens, {heads or 'heads'}, {self.dim}] on {self.device}, unit "
                              f"stride last; got {x.dtype} {list(n)} on {x.device}")
+        if x.requires_grad and _grad_enabled():
+            raise ValueError(f"{name} requires a gradient, which the paged cache does not give: call it under torch.no_grad()")
         return n, st
 
     def _ints(self, name, x):

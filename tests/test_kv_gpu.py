@@ -1005,3 +1005,27 @@ def test_weights_leave_slots_that_no_token_sees_as_they_were(kv, nq, step, windo
     W = kv_ref.attend(host, q, vis, step=step, window=window)[2]
     bits = acc.cpu().numpy().view(np.int32)
     assert np.all(bits[W == 0] == -2 ** 31) and np.all(acc.cpu().numpy()[W > 0] > 0)
+
+
+def test_tensors_that_require_a_gradient_are_refused(kv):
+    """The operators give none: rather an error than a gradient that is lost without a word. Without gradients they serve."""
+    rng = np.random.default_rng(51)
+    _, K, V, table, bounds = make(rng, [40], 8, 2, 64)
+    n, q, k = ints([30]), torch.randn(1, 1, 4, 64, device="cuda"), torch.randn(1, 1, 2, 64, device="cuda")
+    cache = kv.PagedKV(K, V, table, bounds=bounds)
+    want, pages = cache.attend(q, n), cache.select(q, n, 2)
+    wq, wk = q.clone().requires_grad_(), k.clone().requires_grad_()
+    for call in (lambda: cache.attend(wq, n), lambda: cache.attend(wq * 2, n), lambda: cache.select(wq, n, 2),
+                 lambda: cache.append(wk, k, n), lambda: cache.append(k, wk, n)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    leaf = kv.PagedKV(K.clone().requires_grad_(), V, table, bounds=bounds)
+    with pytest.raises(ValueError, match="gradient"):
+        leaf.attend(q, n)
+    with torch.no_grad():
+        assert torch.equal(cache.attend(wq, n), want) and torch.equal(cache.select(wq, n, 2), pages)
+        assert torch.equal(leaf.attend(q, n), want) and not cache.attend(wq, n).requires_grad
+        cache.append(wk, wk, n)
+    with torch.inference_mode():
+        cache.attend(wq, n)
+    assert torch.equal(cache.attend(wq.detach(), n), cache.attend(q, n))
