@@ -80,12 +80,19 @@ def set_device(index):
     _check(_fn["set_device"](index), "set_device")
 
 
+_dead = []   # workspaces whose last reference went during a capture
+
+
 class Workspace:
     """Device memory for attend, select and evict of calls that run one after the other (see gen9blas_kv_ws_create). One that
-    a captured call has used keeps its memory until `free`, whether or not anything still refers to it: its graph may."""
+    a captured call has used keeps its memory until `free`, whether or not anything still refers to it: its graph may. `free`
+    waits for the device, so not during a capture; a workspace that is collected during one is freed behind it."""
 
     def __init__(self):
         self.captured = False
+        if _dead and not _capturing():
+            while _dead:
+                _fn["kv_ws_free"](_dead.pop())
         self.handle = _fn["kv_ws_create"]()
         if not self.handle:
             raise RuntimeError(_fn["error"]().decode(errors="replace"))
@@ -97,7 +104,10 @@ class Workspace:
 
     def __del__(self):
         if getattr(self, "handle", None) and _fn and not self.captured:
-            self.free()
+            if _capturing():
+                _dead.append(self.handle)
+            else:
+                self.free()
 
 
 class PagedKV:

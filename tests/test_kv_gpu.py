@@ -1029,3 +1029,28 @@ def test_tensors_that_require_a_gradient_are_refused(kv):
     with torch.inference_mode():
         cache.attend(wq, n)
     assert torch.equal(cache.attend(wq.detach(), n), cache.attend(q, n))
+
+
+def test_a_workspace_collected_during_a_capture_does_not_end_it(kv):
+    """Freeing waits for the device, which a capture does not allow: it is put off to the next workspace."""
+    rng = np.random.default_rng(52)
+    host, K, V, table, _ = make(rng, [40], 16, 1, 64)
+    q, n = torch.randn(1, 1, 4, 64, device="cuda"), ints([40])
+    kept, other = (kv.PagedKV(K, V, table, workspace=kv.Workspace()) for _ in range(2))
+    want = kept.attend(q, n)
+    assert torch.equal(other.attend(q, n), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = kept.attend(q, n)
+        del other
+        assert len(kv._dead) == 1
+        second = kept.attend(q, n)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    kv.Workspace()
+    assert not kv._dead
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(second, want)
