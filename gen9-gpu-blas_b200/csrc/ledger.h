@@ -53,6 +53,8 @@ public:
         }
     }
 
+    bool empty() const { return !n_ && !lost_n_; }
+
     // st has been waited for: its writes are done.
     void clear(Stream st) {
         for (int i = n_ - 1; i >= 0; i--)
@@ -172,6 +174,8 @@ public:
             }
         }
     }
+
+    bool empty() const { return !n_; }
 
     bool overlap(const void *p, size_t bytes, unsigned long long capture) const {
         if (lost(capture)) return true;

@@ -355,6 +355,7 @@ void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
 // Within a capture only captured writes count: whatever else is queued has ended when a replay starts, as a replay has when a
 // call outside a capture starts. (And what is queued cannot be asked about there: the query would end the capture.)
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
+    if (d->queued.empty() && d->queued_captured.empty()) return false;   // waiting calls only: no question to the stream
     const unsigned long long capture = capture_of(stream());
     if (capture) return capture == kCaptureUnknown || d->queued_captured.overlap(p, bytes, capture);
     return d->queued.overlap(p, bytes);
