@@ -53,7 +53,13 @@ public:
         }
     }
 
-    bool empty() const { return !n_ && !lost_n_; }
+    // Whether overlap() has to look at events.
+    bool touches(const void *p, size_t bytes) const {
+        const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+        for (int i = 0; i < n_; i++)
+            if (lo < e_[i].hi && e_[i].lo < hi) return true;
+        return lost_n_ > 0;
+    }
 
     // st has been waited for: its writes are done.
     void clear(Stream st) {
@@ -175,7 +181,14 @@ public:
         }
     }
 
-    bool empty() const { return !n_; }
+    // Whether the answer of overlap() depends on the capture.
+    bool touches(const void *p, size_t bytes) const {
+        const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+        for (int i = 0; i < n_; i++)
+            for (int k = 0; k < r_[i].n; k++)
+                if (lo < r_[i].hi[k] && r_[i].lo[k] < hi) return true;
+        return gone_ > 0;
+    }
 
     bool overlap(const void *p, size_t bytes, unsigned long long capture) const {
         if (lost(capture)) return true;

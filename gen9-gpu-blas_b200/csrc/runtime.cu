@@ -339,11 +339,11 @@ void LedgerApi::wait(Stream st) {
 unsigned long long capture_of(cudaStream_t st) {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
-    if (cudaStreamGetCaptureInfo(st, &cs, &id) != cudaSuccess) {
-        cudaGetLastError();
-        return kCaptureUnknown;
-    }
-    return cs == cudaStreamCaptureStatusNone ? 0 : cs == cudaStreamCaptureStatusActive && id ? id : kCaptureUnknown;
+    cudaError_t e = cudaStreamIsCapturing(st, &cs);   // the quicker question of the two
+    if (e == cudaSuccess && cs == cudaStreamCaptureStatusNone) return 0;
+    if (e == cudaSuccess) e = cudaStreamGetCaptureInfo(st, &cs, &id);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e == cudaSuccess && cs == cudaStreamCaptureStatusActive && id ? id : kCaptureUnknown;
 }
 
 void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st, unsigned long long capture) {
@@ -355,7 +355,7 @@ void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
 // Within a capture only captured writes count: whatever else is queued has ended when a replay starts, as a replay has when a
 // call outside a capture starts. (And what is queued cannot be asked about there: the query would end the capture.)
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
-    if (d->queued.empty() && d->queued_captured.empty()) return false;   // waiting calls only: no question to the stream
+    if (!d->queued.touches(p, bytes) && !d->queued_captured.touches(p, bytes)) return false;   // most often: no question to the stream
     const unsigned long long capture = capture_of(stream());
     if (capture) return capture == kCaptureUnknown || d->queued_captured.overlap(p, bytes, capture);
     return d->queued.overlap(p, bytes);
@@ -368,7 +368,8 @@ int finish_op(Operand *ops, int n) {
     bool all_zc = true;
     for (int i = 0; i < n; i++) all_zc = all_zc && ops[i].zc;
     if (G.nowait && all_zc) {
-        const unsigned long long capture = capture_of(st);
+        // the library's own stream and the legacy one are in no capture
+        const unsigned long long capture = st == d->own_stream || st == cudaStreamLegacy ? 0 : capture_of(st);
         for (int i = 0; i < n; i++)
             if (ops[i].written) {
                 const QueuedWrite w = {ops[i].dptr, ops[i].bytes};
