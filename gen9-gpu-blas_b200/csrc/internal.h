@@ -24,6 +24,12 @@ enum : unsigned { kDevErrNone = 0, kDevErrWaitTimeout = 1, kDevErrTmemAlloc = 2 
 struct LedgerApi {
     using Stream = cudaStream_t;
     using Event = cudaEvent_t;
+    // Asking for an event ends another stream's capture of this thread, unless the thread says that it means no harm.
+    struct Quiet {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        Quiet() { cudaThreadExchangeStreamCaptureMode(&mode); }
+        ~Quiet() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    };
     static bool record(Event &e, Stream st);
     static bool done(Event e);
     static void wait(Stream st);

@@ -14,7 +14,8 @@ struct QueuedWrite {
 
 // Api: Stream and Event types (a default Event is "not made yet") and, all static,
 //   bool record(Event &, Stream)   records the event behind all work queued on the stream so far (makes it on first use); false: cannot
-//   bool done(Event)               whether that work has ended (false also where it cannot tell)
+//   bool done(Event)               whether that work has ended (false also where it cannot tell), asked while a Quiet is alive
+//   Quiet                          such questions do no harm in its scope
 //   void wait(Stream)              waits for the stream
 template <typename Api>
 class QueuedLedger {
@@ -71,6 +72,7 @@ public:
 
     // Whether queued work may still write some of [p, p + bytes): by the entries, or always while a write without one is under way.
     bool overlap(const void *p, size_t bytes) {
+        const typename Api::Quiet quiet;
         for (int i = lost_n_ - 1; i >= 0; i--)
             if (Api::done(lost_[i].ev)) lost_drop(i);
         if (lost_n_) return true;
@@ -106,9 +108,7 @@ private:
     int slot(uintptr_t lo, uintptr_t hi, Stream st) {
         for (int i = 0; i < n_; i++)
             if (lo <= e_[i].hi && e_[i].lo <= hi && e_[i].st == st) return i;
-        if (n_ == kRanges)
-            for (int i = n_ - 1; i >= 0; i--)   // full: forget the writes that have completed
-                if (Api::done(ev_[e_[i].ev])) drop(i);
+        if (n_ == kRanges) forget_ended();
         if (n_ < kRanges) return n_;
         int best = -1;
         size_t least = SIZE_MAX;
@@ -121,6 +121,16 @@ private:
             }
         }
         return best;
+    }
+
+    // Drops the entries whose calls have ended, asking once for each call.
+    void forget_ended() {
+        const typename Api::Quiet quiet;
+        for (int ev = 0; ev <= kRanges; ev++) {
+            if (!used_[ev] || !Api::done(ev_[ev])) continue;
+            for (int i = n_ - 1; i >= 0; i--)
+                if (e_[i].ev == ev) drop(i);
+        }
     }
 
     // The last entry takes the place of one that is dropped.
@@ -136,6 +146,7 @@ private:
 
     // A write on st that has no entry: overlap() answers true until it has ended. Where that could not be told, it is waited for.
     void lost(Stream st) {
+        const typename Api::Quiet quiet;
         for (int i = lost_n_ - 1; i >= 0; i--)
             if (Api::done(lost_[i].ev)) lost_drop(i);
         int i = 0;

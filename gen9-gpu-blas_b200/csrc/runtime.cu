@@ -323,11 +323,7 @@ bool LedgerApi::record(Event &e, Stream st) {
     return false;
 }
 bool LedgerApi::done(Event e) {
-    // asking for an event ends another stream's capture of this thread, unless the thread says that it means no harm
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
     const cudaError_t r = cudaEventQuery(e);
-    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     if (r == cudaErrorNotReady) return false;
     cudaGetLastError();
     return r == cudaSuccess;
