@@ -21,12 +21,14 @@ constexpr int AKEYS = 16;    // keys of a step
 // Units: a head's queries of one stream -- (stream s, key-value head g, tile of at most 8·NT rows (token, query head)) --
 // or, with chosen pages, of one token. `outer` counts streams, or (stream, token) pairs; unit u = outer·inner + g·tiles +
 // tile. Steps of 16 keys are counted over all units in order, fewer than 2^31 in all.
-struct PagedArgs {
+// 352 bytes: the size of a kernel's parameters moves the host's time for its launch (a call through g9kv 11.7 µs; 12.1 with 344 or
+// 360 bytes, 12.7 with 384).
+struct alignas(16) PagedArgs {
     KvDev c;
     int H, G, nq, dvis, window;
     int qn;                   // tokens of a unit: nq, or 1 with chosen pages
     int tiles, inner, outer;  // row tiles, HKV·tiles, streams (· nq)
-    PageDiv by_g, by_tiles, by_nq;
+    PageDiv by_g, by_tiles;
     const float *Q;
     long long qt, qh, qs;
     int q2, o4;               // pairs of a query's elements are 8-byte aligned, fours of an output's 16-byte
@@ -41,6 +43,8 @@ struct PagedArgs {
     long long score_row;
     float *lse2;              // log2 of the sum of 2^score, [(s, t, h)], with weights
 };
+
+static_assert(sizeof(PagedArgs) == 352, "see above");
 
 constexpr float PSCALE = 64.0f;   // of the weights as FP16
 
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
         // the unit's nsl slots, one a CTA, follow one another from slot0 on in key order
         const int slot = b + u, slot0 = rs0 / chunk + u, nsl = (rs0 + n - 1) / chunk + u - slot0 + 1;
         const int g = page_quot(a.by_tiles, iu), row0 = (iu - g * a.tiles) * ROWS;
-        const int s = SEL ? page_quot(a.by_nq, outer) : outer, t0 = SEL ? outer - s * a.nq : 0;
+        const int s = SEL ? outer / a.nq : outer, t0 = SEL ? outer - s * a.nq : 0;
         const int live_rows = min(ROWS, a.qn * a.G - row0);
         const int vs = a.vis[s];
         if constexpr (SEL) {   // the entries that count, from this segment's first one to its last
@@ -875,7 +879,6 @@ GEN9BLAS_API int gen9blas_attn_paged(const gen9blas_kv_cache *c, int H, int nq, 
     a.outer = (int)outer;
     a.by_g = page_div(a.G);
     a.by_tiles = page_div(a.tiles);
-    a.by_nq = page_div(nq);
     a.o4 = ((uintptr_t)O & 15) == 0;
     a.q2 = ((uintptr_t)Q & 7) == 0 && ((qt | qh | qs) & 1) == 0;
     const long long units = outer * a.inner;
