@@ -84,6 +84,9 @@ int kv_begin(const gen9blas_kv_cache *c, int H, int sync, const char *who, KvDev
     call->d = dev_state();
     call->st = c->stream ? (cudaStream_t)c->stream : stream();
     call->capture = capture_of(call->st);
+    if (call->capture == kCaptureUnknown)   // a launch would end that other capture, too
+        return fail(GEN9BLAS_ERR, "%s: the capture of the call's stream has failed, or that of a stream which synchronises with it "
+                    "is under way", who);
     if (call->capture && sync)
         return fail(GEN9BLAS_ERR_INVALID_ARG, "%s: sync = 1 while the stream is being captured", who);
     if (c->n_pages > 0) {

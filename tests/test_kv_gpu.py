@@ -1054,3 +1054,33 @@ def test_a_workspace_collected_during_a_capture_does_not_end_it(kv):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(second, want)
+
+
+def test_the_legacy_stream_beside_a_blocking_stream_s_capture(kv, gpu_lib):
+    """A call on the legacy stream is refused while a stream that synchronises with it is captured, and the capture goes on."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    rng = np.random.default_rng(53)
+    _, K, V, table, _ = make(rng, [40], 16, 1, 64)
+    cache = kv.PagedKV(K, V, table, workspace=kv.Workspace())
+    q, k, n, x = torch.randn(1, 1, 4, 64, device="cuda"), torch.randn(1, 1, 1, 64, device="cuda"), ints([40]), torch.zeros(64, device="cuda")
+    want, zero = cache.attend(q, n), ints([0])
+    before = K.clone()
+    torch.cuda.synchronize()
+    err, stream = rt.cudaStreamCreate()
+    assert err == 0
+    try:
+        assert rt.cudaStreamBeginCapture(stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed)[0] == 0
+        assert rt.cudaMemsetAsync(x.data_ptr(), 1, 256, stream)[0] == 0
+        for call in (lambda: cache.append(k, k, zero, count=zero), lambda: kv._fn["attn_paged"](cache._ref, 4, 1, q.data_ptr(), 256, 64, 256,
+                     n.data_ptr(), 1, 0, None, 0, 0.125, q.data_ptr(), None, None, 0, 0, cache.workspace.handle, 0)):
+            try:
+                assert call() not in (0, None)
+            except RuntimeError as e:
+                assert "capture" in str(e)
+        err, graph = rt.cudaStreamEndCapture(stream)
+        assert err == 0                                       # the capture has not been ended by the calls
+        assert rt.cudaGraphDestroy(graph)[0] == 0
+    finally:
+        rt.cudaStreamDestroy(stream)
+    torch.cuda.synchronize()
+    assert torch.equal(cache.attend(q, n), want) and torch.equal(K, before) and not x.any()
