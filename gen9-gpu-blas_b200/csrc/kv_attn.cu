@@ -54,6 +54,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// the larger one, NaN if either is
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float z;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+    return z;
+}
 __device__ __forceinline__ void cp16(unsigned dst, const void *src, int bytes) {   // bytes 16, or 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -126,13 +132,18 @@ __device__ __forceinline__ int list_counts(const int *sel, int i, int n, int mp)
 
 // The score, in base 2, of query row q (its place among all (s, t, h)) and a key row in shared memory, whose 16-byte pieces are
 // exchanged by `swap`: element by element.
-__device__ __noinline__ float plain_score(const PagedArgs &a, int q, const uint8_t *key, int swap) {
+__device__ __forceinline__ float plain_score(const PagedArgs &a, int q, const uint8_t *key, int swap) {
     const int h = q % a.H, st = q / a.H, t = st % a.nq, s = st / a.nq;
     const float *qp = a.Q + s * a.qs + t * a.qt + h * a.qh;
     float x = 0.0f;
+#pragma unroll 1
     for (int d = 0; d < a.c.D; d++) x = fmaf(qp[d], __half2float(reinterpret_cast<const __half *>(key)[((d >> 3) ^ swap) * 8 + (d & 7)]), x);
     return x * a.qscale;
 }
+
+// The same as a call, where the loop's code in line would cost the kernel registers (windows of D 64: 22.5 µs, 24.6 in line; D 256
+// with two row tiles: 144.6 in line, 149.4 with the call).
+__device__ __noinline__ float plain_score_call(const PagedArgs &a, int q, const uint8_t *key, int swap) { return plain_score(a, q, key, swap); }
 
 // Elements d .. d + 3 of output row q from the sum L of its weights, the greatest score M and the sums x of PSCALE-fold weights.
 __device__ __forceinline__ void paged_out(const PagedArgs &a, long long q, int d, float M, float L, float4 x) {
@@ -446,6 +457,20 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                         if (kc >= see[nt][j] || kc < from[nt][j]) sc[nt][2 + j] = -INFINITY;
                     }
             }
+            // For the weights. With one tile before the scores are looked at (8 streams of 8192 keys 51.0 µs, 51.9 behind that), with two
+            // behind it (D 128, 64 streams of 4096 keys 208 µs, 214 before it).
+            auto keep_scores = [&]() {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
+                        float *sr = NT == 1 ? srow[j] : a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
+                        if (r < live_rows && at0 < k1) sr[at0] = sc[nt][j] * inv[nt][j];
+                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = sc[nt][2 + j] * inv[nt][j];
+                    }
+            };
+            if constexpr (W && NT == 1) keep_scores();
             // Weights are 2^(score - m) with m a greatest score of before: it is raised, and the sums scaled down, only when
             // a score passes it by more than 8, so that most steps need no maximum over the lanes.
             float p[NT][2][2];   // of (key gq + 8e, row 8nt + 2tq + j), at most 2^8
@@ -456,21 +481,27 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                 for (int j = 0; j < 2; j++) {
                     p[nt][0][j] = fmaf(sc[nt][j], inv[nt][j], -m[nt][j]);
                     p[nt][1][j] = fmaf(sc[nt][2 + j], inv[nt][j], -m[nt][j]);
-                    over = over || !(p[nt][0][j] <= 8.0f) || !(p[nt][1][j] <= 8.0f);   // also NaN
+                    over = over || !(max_nan(p[nt][0][j], p[nt][1][j]) <= 8.0f);   // also NaN
                 }
             if (__any_sync(kAll, over)) {
                 // An infinite element of a key meets the query's two parts separately, and infinity times a part of zero is NaN:
                 // what came out as NaN is computed again by the formula, for a score of -inf has no weight.
+                bool nan = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int r = 8 * nt + 2 * tq + j, q = __shfl_sync(kAll, my_q, r);
+                    for (int e = 0; e < 4; e++) nan = nan || sc[nt][e] != sc[nt][e];
+                if (__any_sync(kAll, nan)) {
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (sc[nt][2 * e + j] != sc[nt][2 * e + j] && r < live_rows)
-                                sc[nt][2 * e + j] = plain_score(a, q, wring + stage * C::STAGE + (gq + 8 * e) * PITCH, gq) / inv[nt][j];
-                    }
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {   // key gq + 8·(e / 2), row 8nt + 2tq + e % 2
+                            const int r = 8 * nt + 2 * tq + (e & 1), q = __shfl_sync(kAll, my_q, r);
+                            if (sc[nt][e] != sc[nt][e] && r < live_rows)
+                                sc[nt][e] = (DP == 256 ? plain_score : plain_score_call)(a, q, wring + stage * C::STAGE + (gq + 8 * (e >> 1)) * PITCH, gq) / inv[nt][e & 1];
+                        }
+                    if constexpr (W && NT == 1) keep_scores();
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -491,17 +522,7 @@ __global__ void __launch_bounds__(AW * 32, PagedCfg<DP, NT, W>::CTAS) attn_paged
                         }
                     }
             }
-            if constexpr (W) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int r = 8 * nt + 2 * tq + j, at0 = k0 + (sb + warp + AW * i) * AKEYS + gq;
-                        float *sr = NT == 1 ? srow[j] : a.score + (long long)__shfl_sync(kAll, my_q, r) * a.score_row;
-                        if (r < live_rows && at0 < k1) sr[at0] = sc[nt][j] * inv[nt][j];
-                        if (r < live_rows && at0 + 8 < k1) sr[at0 + 8] = sc[nt][2 + j] * inv[nt][j];
-                    }
-            }
+            if constexpr (W && NT == 2) keep_scores();
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -715,13 +736,11 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
     const int vs = a.vis[s];
     if (!a.sel) {
         const int k = (blockIdx.x * 256 + threadIdx.x) * 4;
-        if (k >= seen_slots(vs, a.dvis, a.nq - 1, c.cap) || k + 3 < first_slot(seen_slots(vs, a.dvis, 0, c.cap), a.window)) return;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        unsigned got = 0;   // which of the four some row sees: the others stay as they are
-        auto add = [&](float &to, int i, float score, float l2) {
-            to += weight(score, l2);
-            got |= (unsigned)(score != -INFINITY) << i;
-        };
+        const int k0 = first_slot(seen_slots(vs, a.dvis, 0, c.cap), a.window), k1 = seen_slots(vs, a.dvis, a.nq - 1, c.cap);
+        if (k >= k1 || k + 3 < k0) return;
+        const bool whole = v4 && k >= k0 && k + 3 < k1;
+        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f), sum = w;
+        if (whole) w = *reinterpret_cast<const float4 *>(row + k);   // together with the scores
         for (int t = 0; t < a.nq; t++) {
             const int see = seen_slots(vs, a.dvis, t, c.cap), from = first_slot(see, a.window);
             if (k >= see || k + 3 < from) continue;
@@ -731,20 +750,22 @@ __global__ void __launch_bounds__(256) kv_weigh_k(const __grid_constant__ PagedA
                 const float l2 = __ldcg(a.lse2 + q + h);
                 const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.score + (q + h) * a.score_row + k));
                 // scores outside [from, see) were not written for this token where its whole step lies outside
-                if (k >= from) add(sum.x, 0, x.x, l2);
-                if (k + 1 >= from && k + 1 < see) add(sum.y, 1, x.y, l2);
-                if (k + 2 >= from && k + 2 < see) add(sum.z, 2, x.z, l2);
-                if (k + 3 >= from && k + 3 < see) add(sum.w, 3, x.w, l2);
+                if (k >= from) sum.x += weight(x.x, l2);
+                if (k + 1 >= from && k + 1 < see) sum.y += weight(x.y, l2);
+                if (k + 2 >= from && k + 2 < see) sum.z += weight(x.z, l2);
+                if (k + 3 >= from && k + 3 < see) sum.w += weight(x.w, l2);
             }
         }
-        if (v4 && got == 15u) {
-            float4 w = *reinterpret_cast<const float4 *>(row + k);
-            *reinterpret_cast<float4 *>(row + k) = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
+        // Slots that gain nothing stay as they are, bit for bit; those behind the last one seen or before the first, which are
+        // other calls' to write, are not written at all.
+        auto gain = [](float w, float x) { return x == 0.0f ? w : w + x; };
+        if (whole) {
+            *reinterpret_cast<float4 *>(row + k) = make_float4(gain(w.x, sum.x), gain(w.y, sum.y), gain(w.z, sum.z), gain(w.w, sum.w));
         } else {
-            if (got & 1u) row[k] += sum.x;
-            if (got & 2u) row[k + 1] += sum.y;
-            if (got & 4u) row[k + 2] += sum.z;
-            if (got & 8u) row[k + 3] += sum.w;
+            if (sum.x != 0.0f) row[k] += sum.x;
+            if (sum.y != 0.0f) row[k + 1] += sum.y;
+            if (sum.z != 0.0f) row[k + 2] += sum.z;
+            if (sum.w != 0.0f) row[k + 3] += sum.w;
         }
         return;
     }
