@@ -82,7 +82,9 @@ struct PagedCfg {
     static constexpr int KIDX = AW * NST * AKEYS * 4;
     static constexpr int ROWOFF = AW * AKEYS * 16;
     static constexpr int SMEM = RING + QF + KIDX + ROWOFF + ROWS * 4;
-    static constexpr int COST = 16;                                          // steps that a CTA reads in the time of a segment's latencies
+    // Steps that a CTA reads in the time of a segment's latencies: found with D 128 and one row tile (see where the run is cut). A
+    // step of D 64 is half the bytes and one of D 256 twice; their own numbers have not been measured.
+    static constexpr int COST = 16;
 };
 
 // Steps of one outer index: its slots [k0, k1) from the first visible one on, held to a multiple of a step; at least one,

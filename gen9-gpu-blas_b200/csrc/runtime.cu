@@ -349,7 +349,9 @@ void queued_writes_add(DevState *d, const QueuedWrite *w, int n, cudaStream_t st
 }
 void queued_writes_clear(DevState *d, cudaStream_t st) { d->queued.clear(st); }
 // Within a capture only captured writes count: whatever else is queued has ended when a replay starts, as a replay has when a
-// call outside a capture starts. (And what is queued cannot be asked about there: the query would end the capture.)
+// call outside a capture starts: behind a kernel of 60 µs, one that may start early did so 57 to 60 µs before that one's end in the same
+// stream or graph, and 1.3 µs or more behind it across the border of a graph. What is queued cannot be asked about there: the query
+// would end the capture.
 bool queued_writes_overlap(DevState *d, const void *p, size_t bytes) {
     if (!d->queued.touches(p, bytes) && !d->queued_captured.touches(p, bytes)) return false;   // most often: no question to the stream
     const unsigned long long capture = capture_of(stream());

@@ -16,7 +16,8 @@
  * them, each at least what the dimensions with smaller ones span (GEN9BLAS_ERR_INVALID_ARG otherwise).
  *
  * Shapes: D a multiple of 8 up to 256, H a multiple of HKV (gen9blas_kv_supported; other shapes return
- * GEN9BLAS_DECLINED, nothing written); K, V and bounds 16-byte aligned, their strides multiples of 8 elements. */
+ * GEN9BLAS_DECLINED, nothing written); K, V and bounds 16-byte aligned, their strides multiples of 8 elements. kv_append and
+ * attn_paged with acc take up to 65535 streams, and as many heads or (stream, head) rows (GEN9BLAS_ERR_INVALID_ARG past that). */
 #pragma once
 #include "gen9blas_ml.h"
 #ifdef __cplusplus
@@ -66,7 +67,8 @@ GEN9BLAS_API int gen9blas_kv_append(const gen9blas_kv_cache *c, int nt, const fl
  * at Q[t·qt + h·qh + s·qs + d]; query head h reads key-value head h / (H / HKV). lse (NULL or [s][t][h]): log of the sum of
  * exp(score). A token that sees nothing gets O = 0, lse = -inf. dvis and window >= 0.
  * What lies in slots that a token does not see (NaN, infinities) does not enter its result; a seen key or value that is
- * not finite enters as the formula has it (NaN, as a rule; a score of -inf has no weight), for the heads that see it only.
+ * not finite enters as the formula has it, for the heads that see it only: NaN, as a rule (where the formula gives an infinite
+ * output, NaN may stand for it); a score of -inf has no weight.
  * sel (NULL or int [s][t][HKV][nsel]): only the slots of the listed pages, given by their place k / page in the stream,
  * ascending; an entry that is negative or not below mp is skipped, and so is one that is not above every earlier entry that
  * was not (a page counts once). Not with window > 0.

@@ -136,7 +136,7 @@ CASES = [   # lens, page, heads, group, D, tokens, window, layout
     ([500, 17, 64], 64, 1, 4, 128, 4, 33, "pshd"),
     ([130, 0, 1], 1, 1, 2, 256, 2, 0, "phsd"),
     ([300], 128, 2, 16, 256, 1, 0, "phsd"),
-    ([1500], 16, 2, 4, 128, 9, 0, "phsd"),          # 36 rows of a head: two row tiles
+    ([1500], 16, 2, 4, 128, 9, 0, "phsd"),          # 36 rows of a head: five units (units of two tiles: test_kv_large_gpu.py)
     ([64, 200], 48, 1, 5, 8, 13, 10, "phsd"),
     ([200] * 40, 16, 2, 4, 64, 1, 0, "phsd"),       # more units than CTAs split evenly over
     ([2000, 0, 0, 5, 0, 1999], 16, 4, 4, 128, 1, 0, "phsd"),
