@@ -72,6 +72,7 @@ public:
 
     // Whether queued work may still write some of [p, p + bytes): by the entries, or always while a write without one is under way.
     bool overlap(const void *p, size_t bytes) {
+        if (!touches(p, bytes)) return false;
         const typename Api::Quiet quiet;
         for (int i = lost_n_ - 1; i >= 0; i--)
             if (Api::done(lost_[i].ev)) lost_drop(i);
