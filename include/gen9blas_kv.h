@@ -43,7 +43,9 @@ typedef struct gen9blas_kv_cache {
 GEN9BLAS_API int gen9blas_kv_supported(int D, int H, int HKV);
 
 /* Workspace of attn_paged, kv_select and kv_evict. NULL in a call means the library's own one of the device: calls that
- * share a workspace run one after the other (one on another stream than the last first waits for the device). A call
+ * share a workspace run one after the other (one on another stream than the last first waits for the device; that, and the
+ * allocation when a workspace grows, would end a capture under way on some other stream: beside one, call with a workspace that
+ * the call's stream has used before). A call
  * that is captured into a CUDA graph needs a workspace of its own here, large enough from an earlier call of the same
  * shape outside the capture (GEN9BLAS_ERR_INVALID_ARG otherwise); a replay must not run at the same time as another
  * replay or call that uses its workspace: the library does not see replays, so that order is the caller's.
